@@ -32,7 +32,7 @@ typedef enum pp_status {
   PP_E_MISSING = 7      /* a parameter of the shard was never loaded */
 } pp_status;
 
-typedef enum pp_dtype { PP_F32 = 0, PP_BF16 = 1 } pp_dtype;
+typedef enum pp_dtype { PP_F32 = 0, PP_BF16 = 1, PP_F16 = 2 /* paged operators only */ } pp_dtype;
 
 /* Model geometry: src/qwen/model.rs:11-21 (QwenConfig), field for field. */
 typedef struct pp_config {
@@ -72,7 +72,8 @@ pp_status pp_shard_create(const pp_shard_desc* desc, pp_shard** out);
 void pp_shard_destroy(pp_shard* shard);
 
 /* One parameter by checkpoint name and shape (src/qwen/hf.rs:227-272 load_inputs): matrices
- * as BF16 bits or F32 (rounded to BF16), names containing "norm" as F32 or BF16 (widened).
+ * as BF16 bits or F32 (rounded to BF16), names containing "norm" as F32 or BF16 (widened);
+ * PP_F16 is refused.
  * Names of other shards' parameters are accepted and ignored. */
 pp_status pp_shard_set_tensor(pp_shard* shard, const char* name, pp_dtype dtype,
                               const void* host_data, uint64_t elements);
@@ -314,6 +315,155 @@ uint32_t pp_shard_tap_layers(const pp_shard* shard, uint32_t* layers, uint32_t c
  * BF16 bits rounded to nearest even into bf16 (LayerTap::from_f32, the wire form); either may
  * be NULL. Synchronises the shard's stream. */
 pp_status pp_shard_read_taps(pp_shard* shard, uint32_t m, float* f32, uint16_t* bf16);
+
+/* ---- Operators over a paged K/V cache ------------------------------------------------------
+ * Speculation with a tree of drafts and decoding with beams, over one cache that many sequences
+ * share (the reference has neither: its shard owns one contiguous cache, src/qwen/model.rs:244-302,
+ * and drafts a chain, src/specdecode.rs:41-125). Device-pointer operators: every call only
+ * enqueues on `stream` (a cudaStream_t of the cache's device, NULL = default), allocates nothing,
+ * may be captured into a CUDA graph, and leaves the caller's current device as it was. Work
+ * buffers and outputs are the caller's; calls that may overlap on the device need work buffers
+ * of their own. Arguments that the host can see are checked before the launch (PP_E_INVALID,
+ * PP_E_UNSUPPORTED; message in pp_last_error(NULL)). What only the device sees is checked there:
+ * *err (device memory, zero before the call, or NULL) gets bit 1 when a length or a page table
+ * entry points outside the table or the cache. Such a position is neither read nor written, and
+ * a sequence whose kv_len is below its number of rows or above table_stride * page_size is left
+ * out whole. No call reads a position at or past kv_len, whatever the page holds there. */
+
+/* A cache: `layers` layers of n_pages pages of page_size positions. Element (layer, page, row,
+ * head, dim) of K is at k + layer * layer_stride + page * page_stride + row * row_stride +
+ * head * head_stride + dim, in elements, and V's likewise, so rows-first [page][row][head][dim]
+ * and heads-first [page][head][row][dim] pools, and pools that interleave K and V, are all
+ * strides. Pointers and strides are multiples of 16 bytes; head_dim a multiple of 8, <= 256. */
+typedef struct pp_paged_cache {
+  void* k;
+  void* v;
+  uint32_t dtype; /* a pp_dtype */
+  uint32_t layers, n_pages, page_size, n_kv_heads, head_dim;
+  int64_t layer_stride, page_stride, row_stride, head_stride;
+  int32_t cuda_device;
+} pp_paged_cache;
+
+/* A batch of sequences with new rows. Sequence b owns rows cu_rows[b] .. cu_rows[b + 1] - 1 of
+ * the call's row arrays, n_b of them (0 is fine), which are the last n_b of its kv_len[b] cached
+ * positions; position s is row s % page_size of page page_table[b * table_stride + s / page_size].
+ * cu_rows ([batch + 1], not decreasing, cu_rows[0] = 0), kv_len ([batch]) and page_table are
+ * device memory. `rows` bounds cu_rows[batch]: rows of the arrays past cu_rows[batch] are padding
+ * and are neither read nor written. max_rows and max_len are the host's bounds on n_b and kv_len:
+ * they choose kernels and grids, results do not depend on them. batch <= 4096. */
+typedef struct pp_paged_batch {
+  uint32_t batch, rows, max_rows, max_len, table_stride;
+  const int32_t* cu_rows;
+  const int32_t* kv_len;
+  const int32_t* page_table;
+} pp_paged_batch;
+
+/* New rows for pp_paged_append. k and v are [rows][n_kv_heads][head_dim] and q, optional,
+ * [rows][n_heads][head_dim] of `dtype`, with their row strides in elements and heads adjacent
+ * (the parts of a fused QKV projection's rows qualify). */
+typedef struct pp_append_rows {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out; /* [rows][n_heads][head_dim], contiguous, the cache's dtype */
+  uint32_t dtype, n_heads;
+  int64_t q_stride, k_stride, v_stride;
+  const int32_t* positions; /* [rows] rotation positions, or NULL: the cache position */
+  const double* inv_freq;   /* [rotary_dim / 2] radians per position, or NULL: no rotation */
+  uint32_t rotary_dim;      /* even, <= head_dim: the leading dims that rotate */
+  uint32_t interleaved;     /* 0: dims (i, i + rotary_dim / 2) rotate together; 1: (2i, 2i + 1) */
+  const float* q_norm;      /* [head_dim] per-head RMSNorm weights, or NULL: none */
+  const float* k_norm;
+  float eps;
+  uint32_t layer;
+} pp_append_rows;
+
+/* Append rows to the cache with the rotation applied on the way (the QK-norm, RoPE and KV write
+ * of src/qwen/model.rs:265-302, for a batch over pages): every k row, RMS-normed by head when
+ * k_norm is given, rotated and rounded once to the cache's type, and every v row rounded, go to
+ * their positions; q rows, normed and rotated likewise, to q_out (q_out may be q where the types
+ * and strides agree). The angle position * inv_freq is formed in 64 bits, so far positions
+ * rotate as exactly as near ones. A draft tree gives each node its depth as position. Two rows
+ * written to the same cache slot (one page in two sequences' tables) leave either there. */
+pp_status pp_paged_append(const pp_paged_cache* cache, const pp_paged_batch* batch,
+                          const pp_append_rows* rows, uint32_t* err, void* stream);
+
+/* Queries for pp_tree_attention. q and out are [rows][n_heads][head_dim] of the cache's type, q
+ * with a row stride in elements (a multiple of 16 bytes), out contiguous. */
+typedef struct pp_tree_query {
+  const void* q;
+  void* out;
+  float* lse; /* [rows][n_heads], or NULL: log of the softmax's sum (-inf for an empty row) */
+  int64_t q_stride;
+  uint32_t n_heads; /* a multiple of n_kv_heads */
+  uint32_t layer;
+  const uint32_t* mask; /* [rows][mask_words], or NULL */
+  uint32_t mask_words;
+  float scale;
+} pp_tree_query;
+
+/* Attention of a tree of drafted tokens over the cache: row i of sequence b sees all of the
+ * context (positions below kv_len[b] - n_b) and those nodes j < n_b (position kv_len[b] - n_b + j)
+ * whose bit j % 32 of mask word j / 32 of its row is set, whatever order the tree has; without a
+ * mask the rows are a chain and row i sees nodes 0..i (a verify chunk; one row is plain decode).
+ *   out = softmax over the seen positions of (q . k * scale) times v
+ * Query heads h * n_heads / n_kv_heads .. share cached head h. Sums and the softmax are F32. A
+ * row that sees nothing gives zeros. NaN and infinities in K or V of unseen positions have no
+ * effect. Nodes past 32 * mask_words are unseen. The result of a row does not depend on
+ * atomics' order: equal calls give equal bits. `work` (16-byte aligned) holds the partial results
+ * of split caches: at least pp_tree_attention_work_bytes. */
+uint64_t pp_tree_attention_work_bytes(const pp_paged_cache* cache, const pp_paged_batch* batch,
+                                      uint32_t n_heads);
+pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_paged_batch* batch,
+                            const pp_tree_query* query, void* work, uint64_t work_bytes,
+                            uint32_t* err, void* stream);
+
+/* Commit the accepted path of every tree (the accept compare of src/specdecode.rs:92-98 on a
+ * tree, and the rollback): the path starts at node 0 (the current token) and goes on to the
+ * lowest-numbered node whose parent is the path's last node and whose token is that node's pick,
+ * as long as there is one. parents[row] is the node's parent inside its sequence (below the node;
+ * any other value hangs the node on nothing), tokens[row] its token, picks[row] the target's
+ * greedy token after it. Outputs: path[b][path_stride] the nodes, -1 behind them; accepted[b] the
+ * nodes after node 0; correction[b] the pick of the last one; new_len[b] = kv_len[b] - n_b + 1 +
+ * accepted[b]. In every layer the path's K/V rows move to the front of the tree's, in order, so
+ * the first new_len[b] positions are a contiguous cache. A sequence without rows gives accepted 0,
+ * correction -1 and its kv_len. max_rows must bound n_b (a longer tree is left out, error bit 1;
+ * <= 1024), path_stride >= max_rows; new_len must not be the batch's kv_len. */
+pp_status pp_tree_commit(const pp_paged_cache* cache, const pp_paged_batch* batch,
+                         const int32_t* tokens, const int32_t* parents, const int32_t* picks,
+                         int32_t* path, uint32_t path_stride, int32_t* accepted,
+                         int32_t* correction, int32_t* new_len, uint32_t* err, void* stream);
+
+/* Beam search's selection. logits are [groups][beams][vocab] of `dtype` with a row stride between
+ * beams in elements, scores [groups][beams] F32 running log-probabilities (-inf: beam not in
+ * use). The candidates of a group are its beams' tokens with value score + logit - log sum exp of
+ * the beam's logits; the k best (k, beams <= 64) go out in order, ties to the lower beam, then the
+ * lower token: out_scores (F32), out_beams, out_tokens, each [groups][k]. A logit of -inf is never
+ * chosen; a beam with finished[g][b] != 0 (NULL: none) has one candidate, token `pad` at its score
+ * unchanged; a beam whose score or any of whose logits is NaN or +inf is left out and sets bit 2
+ * of *err. Where fewer than k candidates remain the rest are -inf, -1, -1. Values are formed
+ * and compared in 64 bits. work: 16-byte aligned, pp_beam_select_work_bytes. cuda_device: the
+ * device of the pointers and the stream. */
+uint64_t pp_beam_select_work_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k);
+pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t row_stride,
+                         const float* scores, const uint8_t* finished, int32_t pad,
+                         uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k,
+                         float* out_scores, int32_t* out_beams, int32_t* out_tokens, void* work,
+                         uint64_t work_bytes, uint32_t* err, int32_t cuda_device, void* stream);
+
+/* Reorder the beams' states after a selection: new beam j of group g continues old beam
+ * p = beams[g][j] (0 <= p < old_beams; -1: nothing to continue, its table row becomes -1 and its
+ * length 0). new_table[g][j] = table[g][p] and new_len[g][j] = len[g][p]: full pages are shared.
+ * The last page, where it is only part full and will be written by its owner, stays with the
+ * first child (the lowest j); every other child takes page spare[g][j] for it, the part's rows
+ * of every layer are copied there and taken[g][j] is 1 (0 elsewhere: the spare page is unused).
+ * Tables are [..][table_stride]; outputs must not be the inputs. Spare pages must be in nobody's
+ * table. Entries of the table past the length are copied as they are. */
+pp_status pp_beam_reorder(const pp_paged_cache* cache, const int32_t* table, const int32_t* len,
+                          uint32_t groups, uint32_t old_beams, uint32_t new_beams,
+                          uint32_t table_stride, const int32_t* beams, const int32_t* spare,
+                          int32_t* new_table, int32_t* new_len, int32_t* taken, uint32_t* err,
+                          void* stream);
 
 /* Message of the last error on the handle (or of the last failed create when NULL). */
 size_t pp_last_error(const pp_shard* shard, char* buf, size_t len);

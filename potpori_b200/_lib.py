@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "libpotpori_b200.so")
 
 PP_OK, PP_E_INVALID, PP_E_NONFINITE, PP_E_CUDA, PP_E_TIMEOUT, PP_E_OOM, PP_E_UNSUPPORTED, \
     PP_E_MISSING = range(8)
-PP_F32, PP_BF16 = 0, 1
+PP_F32, PP_BF16, PP_F16 = 0, 1, 2
 STATUS_NAMES = {
     PP_OK: "PP_OK", PP_E_INVALID: "PP_E_INVALID", PP_E_NONFINITE: "PP_E_NONFINITE",
     PP_E_CUDA: "PP_E_CUDA", PP_E_TIMEOUT: "PP_E_TIMEOUT", PP_E_OOM: "PP_E_OOM",
@@ -37,7 +37,9 @@ EXPORTS = [
     "pp_rows_gemm_work_bytes", "pp_rows_gemm", "pp_norm_gemv_static", "pp_shard_set_taps",
     "pp_shard_tap_layers", "pp_shard_read_taps", "pp_shard_set_wait_test", "pp_shard_inbox_export", "pp_shard_outbox_open",
     "pp_shard_send", "pp_shard_recv", "pp_shard_send_result", "pp_host_register",
-    "pp_host_unregister", "pp_last_error", "pp_version",
+    "pp_host_unregister", "pp_paged_append", "pp_tree_attention_work_bytes", "pp_tree_attention",
+    "pp_tree_commit", "pp_beam_select_work_bytes", "pp_beam_select", "pp_beam_reorder",
+    "pp_last_error", "pp_version",
 ]
 
 KERNEL_KINDS = ["begin", "embed", "qkv", "attn", "attn_combine", "o_proj", "gate_up", "down",
@@ -77,6 +79,40 @@ class VerifyOut(ctypes.Structure):
         ("correction", ctypes.c_int32),
         ("nonfinite_rows", ctypes.c_int32),
     ]
+
+
+class PagedCacheDesc(ctypes.Structure):
+    """pp_paged_cache"""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
+        (n, ctypes.c_uint32) for n in ("dtype", "layers", "n_pages", "page_size", "n_kv_heads",
+                                       "head_dim")] + [
+        (n, ctypes.c_int64) for n in ("layer_stride", "page_stride", "row_stride",
+                                      "head_stride")] + [("cuda_device", ctypes.c_int32)]
+
+
+class PagedBatchDesc(ctypes.Structure):
+    """pp_paged_batch"""
+    _fields_ = [(n, ctypes.c_uint32) for n in ("batch", "rows", "max_rows", "max_len",
+                                               "table_stride")] + [
+        (n, ctypes.c_void_p) for n in ("cu_rows", "kv_len", "page_table")]
+
+
+class AppendRows(ctypes.Structure):
+    """pp_append_rows"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out")] + [
+        ("dtype", ctypes.c_uint32), ("n_heads", ctypes.c_uint32)] + [
+        (n, ctypes.c_int64) for n in ("q_stride", "k_stride", "v_stride")] + [
+        ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p),
+        ("rotary_dim", ctypes.c_uint32), ("interleaved", ctypes.c_uint32),
+        ("q_norm", ctypes.c_void_p), ("k_norm", ctypes.c_void_p), ("eps", ctypes.c_float),
+        ("layer", ctypes.c_uint32)]
+
+
+class TreeQuery(ctypes.Structure):
+    """pp_tree_query"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "out", "lse")] + [
+        ("q_stride", ctypes.c_int64), ("n_heads", ctypes.c_uint32), ("layer", ctypes.c_uint32),
+        ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_uint32), ("scale", ctypes.c_float)]
 
 
 _lib = None
@@ -151,6 +187,14 @@ def load() -> ctypes.CDLL:
         "pp_shard_send_result": (I32, [P, P, P, U32]),
         "pp_host_register": (I32, [P, SZ]),
         "pp_host_unregister": (I32, [P]),
+        "pp_paged_append": (I32, [P, P, P, P, P]),
+        "pp_tree_attention_work_bytes": (U64, [P, P, U32]),
+        "pp_tree_attention": (I32, [P, P, P, P, U64, P, P]),
+        "pp_tree_commit": (I32, [P, P, P, P, P, P, U32, P, P, P, P, P]),
+        "pp_beam_select_work_bytes": (U64, [U32, U32, U32, U32]),
+        "pp_beam_select": (I32, [P, I32, ctypes.c_int64, P, P, I32, U32, U32, U32, U32, P, P, P, P,
+                                 U64, P, I32, P]),
+        "pp_beam_reorder": (I32, [P, P, P, U32, U32, U32, U32, P, P, P, P, P, P, P]),
         "pp_last_error": (SZ, [P, ctypes.c_char_p, SZ]),
         "pp_version": (ctypes.c_char_p, []),
     }

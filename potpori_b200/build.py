@@ -10,19 +10,22 @@ import glob
 import os
 import shutil
 import subprocess
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libpotpori_b200.so")
-SOURCES = [os.path.join(HERE, "csrc", "pp_shard.cu"), os.path.join(HERE, "csrc", "pp_static_gemv.cu"),
-           os.path.join(HERE, "csrc", "pp_prefill.cu")]
+SOURCES = [os.path.join(HERE, "csrc", f) for f in (
+    "pp_shard.cu", "pp_static_gemv.cu", "pp_prefill.cu", "pp_paged_rows.cu", "pp_tree_attn.cu",
+    "pp_beam.cu")]
 DEPS = SOURCES + glob.glob(os.path.join(HERE, "csrc", "*.cuh")) + [
     os.path.join(ROOT, "include", "potpori_b200.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
+    "-Xcompiler", "-fPIC", "-cudart", "static",
     "--expt-relaxed-constexpr",
 ]
 
@@ -44,12 +47,16 @@ def stale() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not stale():
         return LIB
-    cmd = [nvcc(), *NVCC_FLAGS, "-o", LIB + ".tmp", *SOURCES]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
     env = dict(os.environ)
     env.pop("CC", None)  # the image's CC points at a gcc without the host runtime nvcc wants
-    subprocess.run(cmd, check=True, env=env)
+    verb = ["-Xptxas=-v"] if verbose else []
+    with tempfile.TemporaryDirectory() as tmp:  # the sources side by side, then one link
+        objects = [os.path.join(tmp, os.path.basename(s) + ".o") for s in SOURCES]
+        jobs = [[nvcc(), *verb, *NVCC_FLAGS, "-c", "-o", o, s] for s, o in zip(SOURCES, objects)]
+        with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            list(pool.map(lambda j: subprocess.run(j, check=True, env=env), jobs))
+        subprocess.run([nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB + ".tmp", *objects], check=True,
+                       env=env)
     os.replace(LIB + ".tmp", LIB)
     return LIB
 

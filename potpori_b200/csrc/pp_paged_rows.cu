@@ -1,0 +1,536 @@
+// Row movers of the paged K/V cache: appending rotated rows (pp_paged_append), committing the
+// accepted path of a draft tree (pp_tree_commit) and reordering the states of beams
+// (pp_beam_reorder). All are bound by the bytes they move; the small calls by the chain of
+// dependent loads from a row to its page.
+#include <cuda_runtime.h>
+
+#include "../../include/potpori_b200.h"
+#include "pp_paged.cuh"
+
+using namespace pp;
+
+namespace pp {
+
+// ---- append -------------------------------------------------------------------------------
+struct AppendArgs {
+  PagedView c;
+  BatchView b;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  int64_t q_stride, k_stride, v_stride;  // elements
+  const int32_t* positions;
+  const double* inv_freq;
+  const float* q_norm;
+  const float* k_norm;
+  float eps;
+  int32_t nh, rot, interleaved;
+  int32_t tph;  // lanes per head: 8, 16 or 32, 8 dims each
+  uint32_t* err;
+};
+
+constexpr int kAppendThreads = 256;
+
+// cos and sin of position * inv_freq. The angle in turns is formed in 64 bits and reduced to
+// (-0.5, 0.5] before it is rounded, so the error stays near 2^-24 of a turn up to positions of
+// 2^31 (in 32 bits position 131072 would be off by 2^-7 radians already).
+__device__ __forceinline__ float2 rotation(int32_t pos, double inv_freq) {
+  double turns = (double)pos * inv_freq * 0.15915494309189533577;
+  turns -= rint(turns);
+  float s, c;
+  sincospif((float)(2.0 * turns), &s, &c);
+  return make_float2(c, s);
+}
+
+// Where row t goes: its sequence, cache index and page. By warp 0 into shared memory; index -1
+// marks a row of no sequence.
+struct RowPlace {
+  int64_t offset;  // -1: no valid page
+  int32_t in_batch, pos;
+};
+__device__ __forceinline__ void place_row(const AppendArgs& a, int t, int lane, RowPlace* out) {
+  const int b = find_sequence(a.b.cu_rows, a.b.batch, t, lane);
+  if (lane != 0) return;
+  RowPlace r = {-1, 0, 0};
+  if (b >= 0) {
+    const int first = a.b.cu_rows[b], n = a.b.cu_rows[b + 1] - first, len = a.b.kv_len[b];
+    const int32_t given = a.positions ? a.positions[t] : 0;
+    const int index = len - n + (t - first);
+    r.in_batch = 1;
+    r.pos = a.positions ? given : index;
+    const int64_t room = (int64_t)a.b.table_stride * a.c.page.d;
+    if (len >= n && len <= room)
+      r.offset = paged_offset(a.c, a.b.table + (int64_t)b * a.b.table_stride, a.b.table_stride, index);
+    if (r.offset < 0 && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
+  }
+  *out = r;
+}
+
+// One CTA per row and share of its heads. A head is taken by tph lanes of 8 dims each, so loads
+// and stores are 16-byte units in address order; the rotation partner of a rotate-half pair is
+// rotary_dim / 16 lanes away (a shuffle), an interleaved pair sits in one lane. The row's
+// rotary_dim / 2 angles are formed once in shared memory and serve every head.
+template <typename TI, typename TC>
+__global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendArgs a) {
+  __shared__ float2 cs[128];
+  __shared__ RowPlace place;
+  const int t = blockIdx.x, tid = threadIdx.x;
+  const int D = a.c.head_dim, K = a.c.n_kv, heads = a.nh + 2 * K;
+  const int per = kAppendThreads / a.tph, grp = tid / a.tph, j = tid % a.tph;
+  const bool dims = 8 * j < D;
+  auto source = [&](int slot) -> const TI* {
+    if (slot < a.nh) return (const TI*)a.q + (int64_t)t * a.q_stride + (int64_t)slot * D + 8 * j;
+    if (slot < a.nh + K)
+      return (const TI*)a.k + (int64_t)t * a.k_stride + (int64_t)(slot - a.nh) * D + 8 * j;
+    return (const TI*)a.v + (int64_t)t * a.v_stride + (int64_t)(slot - a.nh - K) * D + 8 * j;
+  };
+  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int first = blockIdx.y * per;
+
+  if (tid < 32) place_row(a, t, tid, &place);
+  __syncthreads();
+  if (!place.in_batch) return;
+  if (a.inv_freq && tid < a.rot / 2) cs[tid] = rotation(place.pos, a.inv_freq[tid]);
+  __syncthreads();
+
+  for (int s0 = first; s0 < heads; s0 += per * gridDim.y) {
+    const int slot = s0 + grp;
+    const bool live = slot < heads && dims;
+    if (live) load8(source(slot), x);
+    const bool isq = slot < a.nh, isv = slot >= a.nh + K;
+    const float* w = isq ? a.q_norm : a.k_norm;
+    // Per-head RMSNorm; the sum of squares over the head's lanes.
+    float ss = 0.f;
+    if (live)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+    for (int o = a.tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (live && !isv && w) {
+      const float rms = sqrtf(ss / (float)D + a.eps);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = x[i] / rms * w[8 * j + i];
+    }
+    if (a.inv_freq) {
+      float y[8];
+      if (a.interleaved) {
+        if (8 * j < a.rot) {
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) {
+            const float2 r = cs[4 * j + i / 2];
+            y[i] = x[i] * r.x - x[i + 1] * r.y;
+            y[i + 1] = x[i + 1] * r.x + x[i] * r.y;
+          }
+        }
+      } else {
+        const int hl = a.rot / 16;  // lanes of half the rotated dims
+        const int lane = tid & 31;
+        const int from = j < hl ? lane + hl : j < 2 * hl ? lane - hl : lane;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], from);
+        if (j < 2 * hl) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 r = cs[(j < hl ? 8 * j : 8 * (j - hl)) + i];
+            y[i] = j < hl ? x[i] * r.x - y[i] * r.y : x[i] * r.x + y[i] * r.y;
+          }
+        }
+      }
+      if (!isv && 8 * j < a.rot)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = y[i];
+    }
+    if (!live) continue;
+    if (isq) {
+      store8((TC*)a.q_out + ((int64_t)t * a.nh + slot) * D + 8 * j, x);
+    } else if (place.offset >= 0) {
+      const int h = isv ? slot - a.nh - K : slot - a.nh;
+      uint8_t* row = (isv ? a.c.v : a.c.k) + place.offset + (int64_t)h * a.c.head_bytes;
+      store8((TC*)row + 8 * j, x);
+    }
+  }
+}
+
+// The same for rows whose pointers, strides or rotation do not fit 8-element units: a warp per
+// head, lane l the dims l, l + 32, ...
+template <typename TI, typename TC>
+__global__ void __launch_bounds__(kAppendThreads) pp_append_any_kernel(const AppendArgs a) {
+  __shared__ float2 cs[128];
+  __shared__ RowPlace place;
+  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int D = a.c.head_dim, K = a.c.n_kv, heads = a.nh + 2 * K;
+  if (warp == 0) place_row(a, t, lane, &place);
+  __syncthreads();
+  if (!place.in_batch) return;
+  if (a.inv_freq && tid < a.rot / 2) cs[tid] = rotation(place.pos, a.inv_freq[tid]);
+  __syncthreads();
+  for (int slot = blockIdx.y * 8 + warp; slot < heads; slot += 8 * gridDim.y) {
+    const bool isq = slot < a.nh, isv = slot >= a.nh + K;
+    const TI* src = isq ? (const TI*)a.q + (int64_t)t * a.q_stride + (int64_t)slot * D
+                  : isv ? (const TI*)a.v + (int64_t)t * a.v_stride + (int64_t)(slot - a.nh - K) * D
+                        : (const TI*)a.k + (int64_t)t * a.k_stride + (int64_t)(slot - a.nh) * D;
+    const float* w = isv ? nullptr : isq ? a.q_norm : a.k_norm;
+    const int rot = a.inv_freq && !isv ? a.rot : 0;
+    float x[8], p[8];  // a dim and its rotation partner
+    float ss = 0.f;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      const int e = lane + 32 * m;
+      const int pe = e >= rot ? e : a.interleaved ? e ^ 1 : e < rot / 2 ? e + rot / 2 : e - rot / 2;
+      x[m] = e < D ? Elem<TI>::get(src[e]) : 0.f;
+      p[m] = e < rot ? Elem<TI>::get(src[pe]) : 0.f;
+      ss += x[m] * x[m];
+    }
+    const float rms = sqrtf(warp_sum(ss) / (float)D + a.eps);  // also: every load before a store
+    int64_t off = 0;
+    uint8_t* row = nullptr;
+    if (!isq) {
+      if (place.offset < 0) continue;
+      off = place.offset + (int64_t)(isv ? slot - a.nh - K : slot - a.nh) * a.c.head_bytes;
+      row = (isv ? a.c.v : a.c.k) + off;
+    } else {
+      row = (uint8_t*)((TC*)a.q_out + ((int64_t)t * a.nh + slot) * D);
+    }
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      const int e = lane + 32 * m;
+      if (e >= D) continue;
+      float y = x[m];
+      if (w) y = y / rms * w[e];
+      if (e < rot) {
+        const bool head_of_pair = a.interleaved ? !(e & 1) : e < rot / 2;
+        const int pe = a.interleaved ? e ^ 1 : head_of_pair ? e + rot / 2 : e - rot / 2;
+        const float2 r = cs[a.interleaved ? e / 2 : head_of_pair ? e : pe];
+        float o = p[m];
+        if (w) o = o / rms * w[pe];
+        y = head_of_pair ? y * r.x - o * r.y : y * r.x + o * r.y;
+      }
+      ((TC*)row)[e] = Elem<TC>::put(y);
+    }
+  }
+}
+
+// ---- commit -------------------------------------------------------------------------------
+struct CommitArgs {
+  PagedView c;  // layer 0
+  BatchView b;
+  const int32_t* tokens;
+  const int32_t* parents;
+  const int32_t* picks;
+  int32_t* path;
+  int32_t* accepted;
+  int32_t* correction;
+  int32_t* new_len;
+  int32_t path_stride, max_rows, units;  // units: 16-byte units of a row of one head
+  uint32_t* err;
+};
+constexpr int kCommitThreads = 128;
+constexpr int kCommitMaxRows = 1024;
+constexpr int kCommitBatch = 8;  // rows a thread holds between its loads and its stores
+
+// Grid (slices of the 2 * layers planes, batch). Every CTA walks its sequence's tree itself (a
+// few hundred cycles) and moves the path's rows in its planes. A thread keeps one 16-byte unit of
+// a row and moves it down row after row: the rows before the first gap stay, and as path[d] >= d
+// and both ascend, a row is written only after every row that it covers has been read.
+__global__ void __launch_bounds__(kCommitThreads) pp_tree_commit_kernel(const CommitArgs a) {
+  __shared__ int32_t follow[kCommitMaxRows];  // the node that continues a path ending here
+  __shared__ int32_t path[kCommitMaxRows];
+  __shared__ int64_t from[kCommitMaxRows], to[kCommitMaxRows];
+  __shared__ int32_t s_count;
+  const int b = blockIdx.y, tid = threadIdx.x;
+  const int first = a.b.cu_rows[b], n = a.b.cu_rows[b + 1] - first, len = a.b.kv_len[b];
+  const bool lead = blockIdx.x == 0;
+  const bool bad = n < 0 || n > a.max_rows || len < n ||
+                   (int64_t)len > (int64_t)a.b.table_stride * a.c.page.d;
+  if (n <= 0 || bad) {
+    if (lead) {
+      for (int d = tid; d < a.path_stride; d += kCommitThreads) a.path[(int64_t)b * a.path_stride + d] = -1;
+      if (tid == 0) {
+        a.accepted[b] = 0;
+        a.correction[b] = -1;
+        a.new_len[b] = len;
+        if (bad && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
+      }
+    }
+    return;
+  }
+  for (int i = tid; i < n; i += kCommitThreads) follow[i] = n;
+  __syncthreads();
+  for (int i = 1 + tid; i < n; i += kCommitThreads) {
+    const int p = a.parents[first + i];
+    if (p >= 0 && p < i && a.tokens[first + i] == a.picks[first + p]) atomicMin(&follow[p], i);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int count = 0;
+    for (int node = 0; node < n; node = follow[node]) path[count++] = node;
+    s_count = count;
+  }
+  __syncthreads();
+  const int count = s_count;
+  const int32_t* table = a.b.table + (int64_t)b * a.b.table_stride;
+  for (int d = tid; d < count; d += kCommitThreads) {
+    const int base = len - n;
+    const bool moves = path[d] != d;
+    from[d] = moves ? paged_offset(a.c, table, a.b.table_stride, base + path[d]) : -1;
+    to[d] = moves ? paged_offset(a.c, table, a.b.table_stride, base + d) : -1;
+    if (moves && (from[d] < 0 || to[d] < 0)) {
+      from[d] = to[d] = -1;
+      if (lead && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
+    }
+  }
+  if (lead) {
+    for (int d = tid; d < a.path_stride; d += kCommitThreads)
+      a.path[(int64_t)b * a.path_stride + d] = d < count ? path[d] : -1;
+    if (tid == 0) {
+      a.accepted[b] = count - 1;
+      a.correction[b] = a.picks[first + path[count - 1]];
+      a.new_len[b] = len - n + count;
+    }
+  }
+  __syncthreads();
+  int gap = 0;  // the first row that moves
+  while (gap < count && path[gap] == gap) ++gap;
+  if (gap == count) return;
+  const int per_row = a.c.n_kv * a.units;
+  for (int plane = blockIdx.x; plane < 2 * a.c.layers; plane += gridDim.x) {
+    uint8_t* base = (plane & 1 ? a.c.v : a.c.k) + (int64_t)(plane >> 1) * a.c.layer_bytes;
+    for (int u = tid; u < per_row; u += kCommitThreads) {
+      const int h = u / a.units;
+      uint8_t* col = base + (int64_t)h * a.c.head_bytes + (int64_t)(u - h * a.units) * 16;
+      for (int d0 = gap; d0 < count; d0 += kCommitBatch) {
+        uint4 hold[kCommitBatch];
+#pragma unroll
+        for (int i = 0; i < kCommitBatch; ++i)
+          if (d0 + i < count && from[d0 + i] >= 0) hold[i] = *(const uint4*)(col + from[d0 + i]);
+#pragma unroll
+        for (int i = 0; i < kCommitBatch; ++i)
+          if (d0 + i < count && from[d0 + i] >= 0) *(uint4*)(col + to[d0 + i]) = hold[i];
+      }
+    }
+  }
+}
+
+// ---- beam reorder -------------------------------------------------------------------------
+struct ReorderArgs {
+  PagedView c;  // layer 0
+  const int32_t* table;
+  const int32_t* len;
+  const int32_t* beams;
+  const int32_t* spare;
+  int32_t* new_table;
+  int32_t* new_len;
+  int32_t* taken;
+  int32_t old_beams, new_beams, stride, units;
+  uint32_t* err;
+};
+constexpr int kReorderThreads = 128;
+
+// Grid (slices of the 2 * layers planes, new beams, groups). Only beams that take their spare
+// page copy: a warp per cached row, lanes over its 16-byte units.
+__global__ void __launch_bounds__(kReorderThreads) pp_beam_reorder_kernel(const ReorderArgs a) {
+  const int j = blockIdx.y, g = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int32_t* mine = a.beams + (int64_t)g * a.new_beams;
+  const int64_t out = (int64_t)g * a.new_beams + j;
+  const int p = mine[j];
+  const bool lead = blockIdx.x == 0, known = p >= 0 && p < a.old_beams;
+  const int64_t src = (int64_t)g * a.old_beams + (known ? p : 0);
+  const int len = known ? a.len[src] : 0;
+  bool elder = false;  // an earlier child of the same beam
+  for (int i = tid; i < j; i += kReorderThreads) elder |= mine[i] == p;
+  const bool again = __syncthreads_or(elder);
+  bool bad = (!known && p != -1) || len < 0 || (int64_t)len > (int64_t)a.stride * a.c.page.d;
+  const int last = bad ? 0 : (int)a.c.page.div((uint32_t)len);
+  const int part = bad ? 0 : len - last * (int)a.c.page.d;
+  const bool take = known && !bad && again && part > 0;
+  int from = -1, to = -1;
+  if (take) {
+    from = a.table[src * a.stride + last];
+    to = a.spare[out];
+    if ((uint32_t)from >= (uint32_t)a.c.n_pages || (uint32_t)to >= (uint32_t)a.c.n_pages) {
+      bad = true;
+      from = -1;
+    }
+  }
+  if (lead) {
+    for (int e = tid; e < a.stride; e += kReorderThreads)
+      a.new_table[out * a.stride + e] =
+          !known ? -1 : take && e == last ? to : a.table[src * a.stride + e];
+    if (tid == 0) {
+      a.new_len[out] = len;
+      a.taken[out] = take ? 1 : 0;
+      if (bad && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
+    }
+  }
+  if (from < 0) return;
+  const int per_row = a.c.n_kv * a.units;
+  for (int plane = blockIdx.x; plane < 2 * a.c.layers; plane += gridDim.x) {
+    uint8_t* base = (plane & 1 ? a.c.v : a.c.k) + (int64_t)(plane >> 1) * a.c.layer_bytes;
+    const uint8_t* sp = base + (int64_t)from * a.c.page_bytes;
+    uint8_t* dp = base + (int64_t)to * a.c.page_bytes;
+    for (int row = warp; row < part; row += kReorderThreads / 32)
+#pragma unroll 4
+      for (int u = lane; u < per_row; u += 32) {
+        const int h = u / a.units;
+        const int64_t off = (int64_t)row * a.c.row_bytes + (int64_t)h * a.c.head_bytes +
+                            (int64_t)(u - h * a.units) * 16;
+        *(uint4*)(dp + off) = *(const uint4*)(sp + off);
+      }
+  }
+}
+
+template <typename TI, typename TC>
+void launch_append(const AppendArgs& a, bool vec, int rows, cudaStream_t st, int sms) {
+  const int heads = a.nh + 2 * a.c.n_kv;
+  const int per = vec ? kAppendThreads / a.tph : 8;
+  // Few rows: a row's heads over several CTAs, as long as that fills the SMs.
+  int y = (heads + per - 1) / per;
+  while (y > 1 && (int64_t)rows * y > 2 * (int64_t)sms) --y;
+  const dim3 grid(rows, y);
+  if (vec)
+    pp_append_kernel<TI, TC><<<grid, kAppendThreads, 0, st>>>(a);
+  else
+    pp_append_any_kernel<TI, TC><<<grid, kAppendThreads, 0, st>>>(a);
+}
+template <typename TI>
+void launch_append_to(const AppendArgs& a, uint32_t cache, bool vec, int rows, cudaStream_t st,
+                      int sms) {
+  if (cache == PP_F32) launch_append<TI, float>(a, vec, rows, st, sms);
+  else if (cache == PP_BF16) launch_append<TI, __nv_bfloat16>(a, vec, rows, st, sms);
+  else launch_append<TI, __half>(a, vec, rows, st, sms);
+}
+
+}  // namespace pp
+
+extern "C" pp_status pp_paged_append(const pp_paged_cache* cache, const pp_paged_batch* batch,
+                                     const pp_append_rows* r, uint32_t* err, void* stream) {
+  if (const char* m = cache_problem(cache)) return paged_fail(PP_E_INVALID, m);
+  if (const char* m = batch_problem(batch)) return paged_fail(PP_E_INVALID, m);
+  if (!r || !r->k || !r->v) return paged_fail(PP_E_INVALID, "null rows");
+  if (r->dtype != PP_F32 && r->dtype != PP_BF16 && r->dtype != PP_F16)
+    return paged_fail(PP_E_INVALID, "the rows' dtype must be PP_F32, PP_BF16 or PP_F16");
+  if ((r->q != nullptr) != (r->q_out != nullptr))
+    return paged_fail(PP_E_INVALID, "q and q_out come together");
+  if (r->q && (r->n_heads == 0 || r->n_heads > 4096))
+    return paged_fail(PP_E_INVALID, "n_heads must be 1..4096 with q");
+  if (r->layer >= cache->layers) return paged_fail(PP_E_INVALID, "layer outside the cache");
+  const int64_t D = cache->head_dim, K = cache->n_kv_heads;
+  const int nh = r->q ? (int)r->n_heads : 0;
+  if (r->inv_freq && (r->rotary_dim == 0 || r->rotary_dim % 2 || r->rotary_dim > D))
+    return paged_fail(PP_E_INVALID, "rotary_dim must be even and within head_dim");
+  if (batch->rows > 1 && (r->k_stride < K * D || r->v_stride < K * D || (nh && r->q_stride < nh * D)))
+    return paged_fail(PP_E_INVALID, "row strides shorter than the rows");
+  const int e = dtype_bytes(r->dtype);
+  const uintptr_t natural = (uintptr_t)r->k | (uintptr_t)r->v | (uintptr_t)r->q;
+  if (natural % e || (uintptr_t)r->q_out % dtype_bytes(cache->dtype))
+    return paged_fail(PP_E_INVALID, "rows must be aligned to their element");
+  if (r->q_out == r->q && r->q && (r->dtype != cache->dtype || (batch->rows > 1 && r->q_stride != nh * D)))
+    return paged_fail(PP_E_INVALID, "q_out may be q only with equal types and adjacent rows");
+  if (batch->rows == 0) return PP_OK;
+  DeviceScope dev(cache->cuda_device);
+  const int sms = dev.ok ? sm_count(cache->cuda_device) : 0;
+  if (!sms) return paged_fail(PP_E_CUDA, "cannot use the cache's device");
+  AppendArgs a = {};
+  a.c = paged_view(*cache, r->layer);
+  a.b = batch_view(*batch);
+  a.q = r->q;
+  a.k = r->k;
+  a.v = r->v;
+  a.q_out = r->q_out;
+  a.q_stride = r->q_stride;
+  a.k_stride = r->k_stride;
+  a.v_stride = r->v_stride;
+  a.positions = r->positions;
+  a.inv_freq = r->inv_freq;
+  a.q_norm = r->q_norm;
+  a.k_norm = r->k_norm;
+  a.eps = r->eps;
+  a.nh = nh;
+  a.rot = r->inv_freq ? (int)r->rotary_dim : 0;
+  a.interleaved = r->interleaved != 0;
+  a.tph = D <= 64 ? 8 : D <= 128 ? 16 : 32;
+  a.err = err;
+  const int64_t unit = 16 / e;
+  const bool vec = (natural | (uintptr_t)r->q_out) % 16 == 0 && r->k_stride % unit == 0 &&
+                   r->v_stride % unit == 0 && (!nh || r->q_stride % unit == 0) &&
+                   a.rot % (a.interleaved ? 8 : 16) == 0;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int rows = (int)batch->rows;
+  if (r->dtype == PP_F32) launch_append_to<float>(a, cache->dtype, vec, rows, st, sms);
+  else if (r->dtype == PP_BF16) launch_append_to<__nv_bfloat16>(a, cache->dtype, vec, rows, st, sms);
+  else launch_append_to<__half>(a, cache->dtype, vec, rows, st, sms);
+  return launch_status("pp_paged_append");
+}
+
+extern "C" pp_status pp_tree_commit(const pp_paged_cache* cache, const pp_paged_batch* batch,
+                                    const int32_t* tokens, const int32_t* parents,
+                                    const int32_t* picks, int32_t* path, uint32_t path_stride,
+                                    int32_t* accepted, int32_t* correction, int32_t* new_len,
+                                    uint32_t* err, void* stream) {
+  if (const char* m = cache_problem(cache)) return paged_fail(PP_E_INVALID, m);
+  if (const char* m = batch_problem(batch)) return paged_fail(PP_E_INVALID, m);
+  if (!tokens || !parents || !picks || !path || !accepted || !correction || !new_len)
+    return paged_fail(PP_E_INVALID, "null argument");
+  if (batch->max_rows > (uint32_t)kCommitMaxRows)
+    return paged_fail(PP_E_UNSUPPORTED, "trees of more than 1024 nodes");
+  if (path_stride < batch->max_rows || path_stride == 0 || path_stride > (1u << 24))
+    return paged_fail(PP_E_INVALID, "path_stride must be at least max_rows and 1");
+  if (new_len == batch->kv_len || accepted == batch->kv_len || correction == batch->kv_len)
+    return paged_fail(PP_E_INVALID, "outputs must not be the batch's kv_len");
+  DeviceScope dev(cache->cuda_device);
+  const int sms = dev.ok ? sm_count(cache->cuda_device) : 0;
+  if (!sms) return paged_fail(PP_E_CUDA, "cannot use the cache's device");
+  CommitArgs a = {};
+  a.c = paged_view(*cache, 0);
+  a.b = batch_view(*batch);
+  a.tokens = tokens;
+  a.parents = parents;
+  a.picks = picks;
+  a.path = path;
+  a.accepted = accepted;
+  a.correction = correction;
+  a.new_len = new_len;
+  a.path_stride = (int32_t)path_stride;
+  a.max_rows = (int32_t)batch->max_rows;
+  a.units = (int32_t)(cache->head_dim * dtype_bytes(cache->dtype) / 16);
+  a.err = err;
+  const dim3 grid(2 * cache->layers, batch->batch);
+  pp_tree_commit_kernel<<<grid, kCommitThreads, 0, (cudaStream_t)stream>>>(a);
+  return launch_status("pp_tree_commit");
+}
+
+extern "C" pp_status pp_beam_reorder(const pp_paged_cache* cache, const int32_t* table,
+                                     const int32_t* len, uint32_t groups, uint32_t old_beams,
+                                     uint32_t new_beams, uint32_t table_stride,
+                                     const int32_t* beams, const int32_t* spare,
+                                     int32_t* new_table, int32_t* new_len, int32_t* taken,
+                                     uint32_t* err, void* stream) {
+  if (const char* m = cache_problem(cache)) return paged_fail(PP_E_INVALID, m);
+  if (!table || !len || !beams || !spare || !new_table || !new_len || !taken)
+    return paged_fail(PP_E_INVALID, "null argument");
+  if (groups == 0 || groups > 65535 || old_beams == 0 || old_beams > 65535 || new_beams == 0 ||
+      new_beams > 65535 || table_stride == 0 || table_stride > 0x7fffffffu)
+    return paged_fail(PP_E_INVALID, "groups, beams and the table's width must be positive, at most 65535 beams and groups");
+  if (new_table == table || new_len == len || new_len == beams || taken == beams || taken == len)
+    return paged_fail(PP_E_INVALID, "outputs must not be the inputs");
+  DeviceScope dev(cache->cuda_device);
+  const int sms = dev.ok ? sm_count(cache->cuda_device) : 0;
+  if (!sms) return paged_fail(PP_E_CUDA, "cannot use the cache's device");
+  ReorderArgs a = {};
+  a.c = paged_view(*cache, 0);
+  a.table = table;
+  a.len = len;
+  a.beams = beams;
+  a.spare = spare;
+  a.new_table = new_table;
+  a.new_len = new_len;
+  a.taken = taken;
+  a.old_beams = (int32_t)old_beams;
+  a.new_beams = (int32_t)new_beams;
+  a.stride = (int32_t)table_stride;
+  a.units = (int32_t)(cache->head_dim * dtype_bytes(cache->dtype) / 16);
+  a.err = err;
+  const dim3 grid(2 * cache->layers, new_beams, groups);
+  pp_beam_reorder_kernel<<<grid, kReorderThreads, 0, (cudaStream_t)stream>>>(a);
+  return launch_status("pp_beam_reorder");
+}

@@ -1351,6 +1351,8 @@ static pp_status resolve(pp_shard* s, const char* name, Target& t) {
 pp_status pp_shard_set_tensor(pp_shard* s, const char* name, pp_dtype dtype, const void* data,
                               uint64_t elements) {
   if (!s || !name || !data) return fail(s, PP_E_INVALID, "null argument");
+  if (dtype != PP_F32 && dtype != PP_BF16)
+    return fail(s, PP_E_INVALID, "%s: parameters are PP_F32 or PP_BF16", name);
   CK(cudaSetDevice(s->dev));
   Target t;
   pp_status r = resolve(s, name, t);
