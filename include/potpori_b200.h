@@ -325,10 +325,10 @@ pp_status pp_shard_read_taps(pp_shard* shard, uint32_t m, float* f32, uint16_t* 
  * buffers and outputs are the caller's; calls that may overlap on the device need work buffers
  * of their own. Arguments that the host can see are checked before the launch (PP_E_INVALID,
  * PP_E_UNSUPPORTED; message in pp_last_error(NULL)). What only the device sees is checked there:
- * *err (device memory, zero before the call, or NULL) gets bit 1 when a length or a page table
+ * *err (device memory, zero before the call, or NULL) gets bit value 1 when a length or a page table
  * entry points outside the table or the cache. Such a position is neither read nor written, and
  * a sequence whose kv_len is below its number of rows or above table_stride * page_size is left
- * out whole. No call reads a position at or past kv_len, whatever the page holds there. */
+ * out whole; value 4 when a bounded wait on the device expired (the output is then undefined). No call reads a position at or past kv_len, whatever the page holds there. */
 
 /* A cache: `layers` layers of n_pages pages of page_size positions. Element (layer, page, row,
  * head, dim) of K is at k + layer * layer_stride + page * page_stride + row * row_stride +

@@ -18,7 +18,7 @@ ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libpotpori_b200.so")
 SOURCES = [os.path.join(HERE, "csrc", f) for f in (
     "pp_shard.cu", "pp_static_gemv.cu", "pp_prefill.cu", "pp_paged_rows.cu", "pp_tree_attn.cu",
-    "pp_beam.cu")]
+    "pp_tree_tc.cu", "pp_beam.cu")]
 DEPS = SOURCES + glob.glob(os.path.join(HERE, "csrc", "*.cuh")) + [
     os.path.join(ROOT, "include", "potpori_b200.h")]
 

@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) pp_beam_merge_kernel(const B
         m = nm;
       }
     }
-    if (bad && lane == 0 && a.err) atomicOr(a.err, 2u);
+    if (bad && lane == 0 && a.err) atomicOr(a.err, PAGED_NONFINITE);
     const int state = bad || score == -INFINITY ? 2 : fin ? 1 : 0;
     if (lane == 0) {
       s_state[b] = state;

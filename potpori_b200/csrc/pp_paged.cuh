@@ -181,7 +181,8 @@ __device__ __forceinline__ int find_sequence(const int32_t* cu, int batch, int t
   return lo < batch ? lo : -1;
 }
 
-enum : uint32_t { PAGED_BAD_PAGE = 1u };  // bit of the caller's error word
+// Bits of the caller's error word.
+enum : uint32_t { PAGED_BAD_PAGE = 1u, PAGED_NONFINITE = 2u, PAGED_TIMEOUT = 4u };
 
 // Element types: load one as F32, store one rounded to nearest even.
 template <typename T>

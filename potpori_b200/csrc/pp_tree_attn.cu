@@ -5,6 +5,7 @@
 #include "../../include/potpori_b200.h"
 #include "pp_attn.cuh"
 #include "pp_tree_attn.cuh"
+#include "pp_tree_plan.cuh"
 
 using namespace pp;
 
@@ -19,6 +20,7 @@ namespace pp {
 // the loop has no CTA barrier.
 constexpr int kTreeThreads = 128;
 constexpr int kTreeBN = 64;
+constexpr uint64_t kTreeTcAbove = 32;  // more query vectors of a head than this: pp_tree_tc.cu
 
 template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -92,22 +94,28 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_mma_kernel(const TreeArg
     const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
     const int NR = s.n * a.G;
 
-    // A thread's share of tile t: KW rows by a warp (WM = 1) or 64 by the CTA.
-    auto load_tile = [&](int t, int stage) {
-      constexpr int LT = WM == 1 ? 32 : kTreeThreads, ROWS = WM == 1 ? KW : BN, RP = LT / UR;
-      const int lid = WM == 1 ? lane : tid, base = WM == 1 ? wn * KW : 0;
-      const int u = lid % UR;
+    // A warp fetches 16 rows of every tile (with WM = 1 those that it consumes). Lane l < 16 looks
+    // row l's page up a tile ahead of the copies, so that no copy waits for the page table.
+    auto look = [&](int t) -> int64_t {
+      const int idx = t * BN + warp * 16 + (lane & 15);
+      if (t >= s.t1 || idx >= s.len) return -1;
+      const int64_t off = paged_offset(a.c, table, a.b.table_stride, idx);
+      if (off < 0) {
+        if (a.err && lane < 16) atomicOr(a.err, PAGED_BAD_PAGE);
+        return -1;
+      }
+      return off + (int64_t)s.h * a.c.head_bytes;
+    };
+    auto load_tile = [&](int stage, int64_t mine) {
+      constexpr int RP = 32 / UR;
+      const int u = lane % UR, sub = lane / UR;
       uint8_t* kd = ring + stage * C::kStage;
 #pragma unroll
-      for (int i = 0; i < ROWS / RP; ++i) {
-        const int r = base + i * RP + lid / UR, idx = t * BN + r;
-        int64_t off = -1;
-        if (idx < s.len) {
-          off = paged_offset(a.c, table, a.b.table_stride, idx);
-          if (off < 0 && a.err && u == 0) atomicOr(a.err, PAGED_BAD_PAGE);
-        }
+      for (int i = 0; i < 16 / RP; ++i) {
+        const int l = i * RP + sub, r = warp * 16 + l;
+        const int64_t off = __shfl_sync(0xffffffffu, mine, l);
         const bool read = off >= 0 && 8 * u < D;
-        const int64_t at = read ? off + (int64_t)s.h * a.c.head_bytes + 16 * u : 0;
+        const int64_t at = read ? off + 16 * u : 0;
         const int dst = r * RB + ((u ^ (r & 7)) << 4);
         cp_async16(kd + dst, a.c.k + at, read);
         cp_async16(kd + C::kTile + dst, a.c.v + at, read);
@@ -120,9 +128,10 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_mma_kernel(const TreeArg
 
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i) {
-      if (s.t0 + i < s.t1) load_tile(s.t0 + i, i);
+      if (s.t0 + i < s.t1) load_tile(i, look(s.t0 + i));
       cp_async_commit();
     }
+    int64_t ahead = look(s.t0 + NS - 1);
     // Queries: BM rows, zero past the unit's.
     for (int e = tid; e < BM * UR; e += kTreeThreads) {
       const int r = e / UR, u = e % UR, R = s.rt * BM + r;
@@ -157,8 +166,9 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_mma_kernel(const TreeArg
       const int stage = (t - s.t0) % NS;
       cp_async_wait<NS - 2>();
       sync();
-      if (t + NS - 1 < s.t1) load_tile(t + NS - 1, (t - s.t0 + NS - 1) % NS);
+      if (t + NS - 1 < s.t1) load_tile((t - s.t0 + NS - 1) % NS, ahead);
       cp_async_commit();
+      ahead = look(t + NS);
       const uint8_t* kt = ring + stage * C::kStage;
       const uint8_t* vt = kt + C::kTile;
       const int kb = wn * KW;
@@ -542,21 +552,22 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
 }
 
 // ---- host ----------------------------------------------------------------------------------
+// Which kernel and how many CTAs, by the query vectors that share a cached head.
 struct TreePlan {
   int dp, bm, bn, ctas;
+  bool tc;
   uint64_t work;
 };
-// Rows of a tile by the query vectors that share a cached head; CTAs for two on an SM, no more
-// than there can be tiles.
-inline TreePlan tree_plan(const pp_paged_cache& c, const pp_paged_batch& b, uint32_t n_heads, int sms) {
+inline TreePlan tree_plan(const pp_paged_cache& c, const pp_paged_batch& b, uint32_t n_heads, int sms, bool tc_ok) {
   TreePlan p;
   p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   const uint64_t G = n_heads / c.n_kv_heads, vectors = (uint64_t)(b.max_rows ? b.max_rows : 1) * G;
+  p.tc = tc_ok && c.dtype != PP_F32 && vectors > kTreeTcAbove;
   if (c.dtype == PP_F32) {
     p.bm = kTreeFBM;
     p.bn = kTreeFBN;
   } else {
-    p.bm = vectors <= 16 ? 16 : vectors <= 32 ? 32 : 64;
+    p.bm = p.tc ? 128 : vectors <= 16 ? 16 : vectors <= 32 ? 32 : 64;
     p.bn = kTreeBN;
   }
   const uint64_t units = ((uint64_t)b.rows * G / p.bm + b.batch) * c.n_kv_heads;
@@ -567,34 +578,10 @@ inline TreePlan tree_plan(const pp_paged_cache& c, const pp_paged_batch& b, uint
   return p;
 }
 
-template <typename K>
-pp_status launch_tree(K kernel, const TreeArgs& a, size_t smem, cudaStream_t st) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return paged_fail(PP_E_CUDA, "cannot reserve the attention's shared memory");
-  kernel<<<a.ctas, kTreeThreads, smem, st>>>(a);
-  return launch_status("pp_tree_attention");
-}
-template <typename K>
-pp_status launch_join(K kernel, const TreeArgs& a, int bm, cudaStream_t st) {
-  const size_t smem = 8 * (size_t)(a.b.batch + 1);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.ctas, bm / 4);
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, (const TreeArgs)a) != cudaSuccess)
-    return launch_status("pp_tree_attention join");
-  return PP_OK;
-}
 template <typename T, int DP, int WM>
 pp_status run_tree_mma(const TreeArgs& a, cudaStream_t st) {
   using C = TreeCfg<DP, WM>;
-  const pp_status r = launch_tree(pp_tree_mma_kernel<T, DP, WM>, a, C::smem(a.b.batch), st);
+  const pp_status r = launch_tree(pp_tree_mma_kernel<T, DP, WM>, a, kTreeThreads, C::smem(a.b.batch), st);
   if (r != PP_OK || a.ctas == 1) return r;
   return launch_join(pp_tree_join_kernel<T, DP, C::BM, C::BN>, a, C::BM, st);
 }
@@ -612,7 +599,7 @@ pp_status run_tree_16(const TreeArgs& a, int dp, int bm, cudaStream_t st) {
 }
 template <int DP>
 pp_status run_tree_f32(const TreeArgs& a, cudaStream_t st) {
-  const pp_status r = launch_tree(pp_tree_f32_kernel<DP>, a, TreeFCfg<DP>::smem(a.b.batch), st);
+  const pp_status r = launch_tree(pp_tree_f32_kernel<DP>, a, kTreeThreads, TreeFCfg<DP>::smem(a.b.batch), st);
   if (r != PP_OK || a.ctas == 1) return r;
   return launch_join(pp_tree_join_kernel<float, DP, kTreeFBM, kTreeFBN>, a, kTreeFBM, st);
 }
@@ -634,8 +621,11 @@ extern "C" uint64_t pp_tree_attention_work_bytes(const pp_paged_cache* cache, co
     paged_fail(PP_E_INVALID, m);
     return 0;
   }
-  const int sms = sm_count(cache->cuda_device);
-  return tree_plan(*cache, *batch, n_heads, sms ? sms : 148).work;
+  const int found = sm_count(cache->cuda_device), sms = found ? found : 148;
+  // Enough for either kernel: which one runs also depends on the query.
+  const uint64_t x = tree_plan(*cache, *batch, n_heads, sms, true).work;
+  const uint64_t y = tree_plan(*cache, *batch, n_heads, sms, false).work;
+  return x > y ? x : y;
 }
 
 extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_paged_batch* batch,
@@ -656,7 +646,8 @@ extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_pag
   DeviceScope dev(cache->cuda_device);
   const int sms = dev.ok ? sm_count(cache->cuda_device) : 0;
   if (!sms) return paged_fail(PP_E_CUDA, "cannot use the cache's device");
-  const TreePlan p = tree_plan(*cache, *batch, q->n_heads, sms);
+  // The tcgen05 kernel takes the maximum before the scale.
+  const TreePlan p = tree_plan(*cache, *batch, q->n_heads, sms, q->scale > 0.f);
   if ((uintptr_t)work % 16 || work_bytes < p.work)
     return paged_fail(PP_E_INVALID, "work must be 16-byte aligned and pp_tree_attention_work_bytes long");
   if (batch->rows == 0) return PP_OK;
@@ -682,6 +673,7 @@ extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_pag
     if (p.dp == 128) return run_tree_f32<128>(a, st);
     return run_tree_f32<256>(a, st);
   }
+  if (p.tc) return run_tree_tc(a, cache->dtype, p.dp, st);
   if (cache->dtype == PP_BF16) return run_tree_16<__nv_bfloat16>(a, p.dp, p.bm, st);
   return run_tree_16<__half>(a, p.dp, p.bm, st);
 }

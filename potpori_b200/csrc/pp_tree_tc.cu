@@ -1,0 +1,533 @@
+// Tree attention on the 5th-generation tensor cores (tcgen05, accumulators in TMEM): the kernel
+// of pp_tree_attention for 16-bit caches when many query vectors share a cached head (a tree, or
+// a chunk of a wide group). Row tiles of 128 vectors, key tiles of 64; the work split is
+// pp_tree_attn.cuh's.
+//
+// One CTA, 224 threads, two CTAs on an SM (one at head_dim 256), so that one's softmax runs under
+// the other's products:
+//  * warps 4 and 5, producers: the K and V rows of every key tile, each from wherever its page is, by
+//    16-byte asynchronous copies into a ring of tile-sized slots, in the order in which the
+//    products need them (K0, K1, V0, K2, V1, ...). A slot holds 64-dim blocks of 64 rows x 128
+//    bytes, the 16-byte unit u of row r at u ^ (r & 7): read K-major it is the B operand of
+//    Q K^T, read MN-major the B operand of P V.
+//  * warp 6, one thread: S = Q K^T (128 x 64, both operands in shared memory) and O += P V (P in
+//    TMEM), each returned by a commit on an mbarrier. S of the next tile is issued as soon as the
+//    softmax has taken S of this one.
+//  * warps 0-3, softmax: thread = row = TMEM lane. S of the row into 64 registers; mask; running
+//    maximum; exp2; P back to TMEM. The output in TMEM is rescaled only when a row's maximum has
+//    grown by more than 2^8 (until then the old maximum serves: P <= 256 and the sums are F32), so
+//    after the first tiles hardly ever. At the end of a segment the rows leave from TMEM.
+// P is carried as two parts of the cache's type, hi + lo, and both multiply V: rounded to one part
+// it would add as much error as the rounding of the output.
+// Every wait is bounded; one that expires sets bit 4 of the caller's error word, and the CTA still
+// lets its copies and products land and frees its TMEM before it leaves.
+#include <cuda_runtime.h>
+
+#include "../../include/potpori_b200.h"
+#include "pp_tree_attn.cuh"
+#include "pp_tree_plan.cuh"
+
+using namespace pp;
+
+namespace pp {
+
+constexpr int kTcThreads = 224;  // 7 warps: 14 on an SM leave 128 registers a thread
+constexpr int kTcBM = 128, kTcBN = 64;
+constexpr int kTcLag = 3;  // items a producer keeps in flight behind the one it issues
+
+template <int DP>
+struct TcCfg {
+  static constexpr int kQ = kTcBM * DP * 2;
+  static constexpr int kItem = kTcBN * DP * 2;  // a K or V tile
+  static constexpr int kSlots = DP == 256 ? 4 : DP == 128 ? 5 : 8;
+  static constexpr int kPerSm = DP == 256 ? 1 : 2;
+  static constexpr int kCols = DP == 256 ? 512 : 256;  // TMEM: O [DP], S [64], P hi [32], P lo [32]
+  static constexpr int kBars = 256;
+  // Two CTAs share 228 KB less 1 KB each: with 5 slots, 1 KB is left for barriers and up to 95
+  // sequences' prefix; larger batches give up a slot.
+  static int slots(int batch) { return DP == 128 && batch > 88 ? 4 : kSlots; }
+  static size_t smem(int batch) {
+    return kQ + (size_t)slots(batch) * kItem + kBars + 8 * (size_t)(batch + 1);
+  }
+};
+
+struct TcBars {
+  uint64_t full[8], free[8];
+  uint64_t q_full, s_full, s_free, p_full, pv_done, end;
+  int64_t scan[8];
+  uint64_t pad;
+  uint32_t tmem, dirty;
+};
+static_assert(sizeof(TcBars) <= 256, "barriers");
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+// SWIZZLE_128B operand at byte address saddr: `lead` bytes between 64-element blocks of a
+// MN-major operand (unused K-major), 1024 between 8-row atoms.
+__device__ __forceinline__ uint64_t tc_desc(uint32_t saddr, uint32_t lead) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) | ((uint64_t)64 << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16, F32 accumulator, A and B both of T, M = 128, N = n, B MN-major when mn.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool mn) {
+  constexpr uint32_t t = __is_same(T, __half) ? 0u : 1u;
+  return (1u << 4) | (t << 7) | (t << 10) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// 32 columns of the thread's lane.
+__device__ __forceinline__ void tc_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t* r = (uint32_t*)v;
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bounded wait of a whole warp: the same answer in every lane, so that a warp leaves together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// 64 bits: which of the positions j0 .. j0 + 63 row i (array row `row`) sees.
+__device__ __forceinline__ uint64_t seen64(const TreeArgs& a, const Segment& s, int row, int i, int j0) {
+  const int node0 = j0 - s.ctx;  // may be negative: context
+  const int skip = node0 < 0 ? -node0 : 0;
+  if (skip >= 64) return ~0ull;
+  const int first = node0 < 0 ? 0 : node0;
+  uint64_t m = 0;
+  if (i < s.n) {
+    if (a.mask) {
+      const uint32_t* w = a.mask + (int64_t)row * a.mask_words;
+      const int k = first >> 5, sh = first & 31;
+      const uint64_t w0 = k < a.mask_words ? w[k] : 0u, w1 = k + 1 < a.mask_words ? w[k + 1] : 0u,
+                     w2 = k + 2 < a.mask_words ? w[k + 2] : 0u;
+      m = (w0 | w1 << 32) >> sh;
+      if (sh) m |= w2 << (64 - sh);
+    } else if (i >= first) {
+      m = i - first >= 63 ? ~0ull : (1ull << (i - first + 1)) - 1;
+    }
+    const int left = s.n - first;  // nodes from `first` on
+    if (left < 64) m &= left <= 0 ? 0ull : (1ull << left) - 1;
+  }
+  return skip ? m << skip | ((1ull << skip) - 1) : m;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t tc_nonfinite(uint32_t v) {
+  constexpr uint32_t E = __is_same(T, __half) ? 0x7c00u : 0x7f80u;
+  return ((v & E) == E ? 0xffffu : 0u) | ((v >> 16 & E) == E ? 0xffff0000u : 0u);
+}
+__device__ __forceinline__ uint32_t tc_pack(float a, float b, __nv_bfloat16*) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *(const uint32_t*)&v;
+}
+__device__ __forceinline__ uint32_t tc_pack(float a, float b, __half*) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *(const uint32_t*)&v;
+}
+__device__ __forceinline__ float2 tc_unpack(uint32_t v, __nv_bfloat16*) { return make_float2(bf16lo(v), bf16hi(v)); }
+__device__ __forceinline__ float2 tc_unpack(uint32_t v, __half*) { return __half22float2(*(const __half2*)&v); }
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kernel(const TreeArgs a, const int slots) {
+  using C = TcCfg<DP>;
+  constexpr int BM = kTcBM, BN = kTcBN, UR = DP / 8;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  uint8_t* qs = sm;
+  uint8_t* ring = sm + C::kQ;
+  TcBars* bars = (TcBars*)(ring + (size_t)slots * C::kItem);
+  int64_t* prefix = (int64_t*)((uint8_t*)bars + C::kBars);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int D = a.c.head_dim;
+  if (smem_u32(sm) & 1023u) {  // the swizzle counts from 1024-byte boundaries
+    if (tid == 0 && a.err) atomicOr(a.err, PAGED_TIMEOUT);
+    return;
+  }
+
+  if (tid == 0) {
+    for (int i = 0; i < slots; ++i) {
+      mbar_init(&bars->full[i], 64);
+      mbar_init(&bars->free[i], 1);
+    }
+    mbar_init(&bars->q_full, 128);
+    mbar_init(&bars->s_full, 1);
+    mbar_init(&bars->s_free, 128);
+    mbar_init(&bars->p_full, 128);
+    mbar_init(&bars->pv_done, 1);
+    mbar_init(&bars->end, 1);
+    bars->dirty = 0;
+    fence_barrier_init();
+  }
+  if (warp == 6) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem)),
+                 "r"(C::kCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pdl_launch_dependents();
+  tc_fence_before();
+  tile_prefix<BM, BN, kTcThreads>(a, prefix, bars->scan, blockIdx.x == 0);  // with CTA barriers
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem;
+  const uint32_t tO = tmem, tS = tmem + DP, tP = tmem + DP + 64;
+  const int64_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
+  const int64_t begin = blockIdx.x * per, end = min(total, begin + per);
+  bool ok = true;
+
+  if (warp == 4 || warp == 5) {
+    // ---- producers: warp pw the rows 32 pw .. + 31 of every tile
+    const int pw = warp - 4;
+    constexpr int RPP = 32 / UR;  // rows of one pass of a warp
+    const int u = lane % UR, sub = lane / UR;
+    int n = 0;
+    for (int64_t w = begin; w < end && ok;) {
+      const Segment s = segment_at<BM, BN>(a, prefix, w, end);
+      const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
+      const int cnt = s.t1 - s.t0;
+      // Lane l looks the tile's row l of the warp up, a tile ahead of its copies.
+      auto look = [&](int i) -> int64_t {
+        const int idx = (s.t0 + i) * BN + pw * 32 + lane;
+        if (i >= cnt || idx >= s.len) return -1;
+        const int64_t off = paged_offset(a.c, table, a.b.table_stride, idx);
+        if (off < 0) {
+          if (a.err) atomicOr(a.err, PAGED_BAD_PAGE);
+          return -1;
+        }
+        return off + (int64_t)s.h * a.c.head_bytes;
+      };
+      // Rows of tile i (V's turn), i + 1 (K's) and i + 2.
+      int64_t prev = -1, cur = look(0), next = look(1);
+      for (int j = 0; j < 2 * cnt; ++j, ++n) {
+        const bool isv = j == 2 * cnt - 1 || (j > 0 && !(j & 1));
+        const int slot = n % slots;
+        if (n >= slots && !warp_wait(&bars->free[slot], (uint32_t)(n / slots - 1) & 1u)) {
+          ok = false;
+          break;
+        }
+        uint8_t* dst = ring + (size_t)slot * C::kItem;
+        const uint8_t* base = isv ? a.c.v : a.c.k;
+        const int64_t mine = isv ? prev : cur;
+#pragma unroll
+        for (int q = 0; q < 32 / RPP; ++q) {
+          const int l = q * RPP + sub, r = pw * 32 + l;
+          const int64_t off = __shfl_sync(0xffffffffu, mine, l);
+          const bool read = off >= 0 && 8 * u < D;
+          cp_async16(dst + (u >> 3) * (BN * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4), base + (read ? off + 16 * u : 0), read);
+        }
+        cp_async_commit();
+        if (j == 0 || isv) {
+          prev = cur;
+          cur = next;
+          next = look(j / 2 + 2);
+        }
+        if (n >= kTcLag) {
+          cp_async_wait<kTcLag>();
+          fence_async();
+          mbar_arrive(&bars->full[(n - kTcLag) % slots]);
+        }
+      }
+      w += cnt;
+    }
+    cp_async_wait<0>();
+    fence_async();
+    for (int i = n > kTcLag ? n - kTcLag : 0; i < n; ++i) mbar_arrive(&bars->full[i % slots]);
+  } else if (warp == 6) {
+    // ---- products
+    if (lane == 0) {
+      constexpr uint32_t iqk = tc_idesc<T>(BN, false), ipv = tc_idesc<T>(DP, true);
+      const uint32_t qb = smem_u32(qs), rb = smem_u32(ring);
+      int n = 0, g = 0, seg = 0;  // items, tiles, segments so far
+      auto take = [&]() -> bool { return mbar_wait(&bars->full[n % slots], (uint32_t)(n / slots) & 1u); };
+      auto qk = [&]() {  // S = Q K^T from the ring's next item
+        const uint32_t kb = rb + (uint32_t)(n % slots) * C::kItem;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks)
+          if (16 * ks < D)
+            tc_mma_ss(tS, tc_desc(qb + (ks >> 2) * (BM * 128) + (ks & 3) * 32, 16),
+                      tc_desc(kb + (ks >> 2) * (BN * 128) + (ks & 3) * 32, 16), iqk, ks != 0);
+        tc_commit(&bars->free[n % slots]);
+        tc_commit(&bars->s_full);
+        ++n;
+      };
+      for (int64_t w = begin; w < end && ok;) {
+        const Segment s = segment_at<BM, BN>(a, prefix, w, end);
+        const int cnt = s.t1 - s.t0;
+        ok = mbar_wait(&bars->q_full, (uint32_t)seg & 1u) && take() && (g == 0 || mbar_wait(&bars->s_free, (uint32_t)(g - 1) & 1u));
+        if (!ok) break;
+        tc_fence_after();
+        qk();
+        for (int i = 0; i < cnt; ++i, ++g) {
+          if (i + 1 < cnt) {
+            ok = take() && mbar_wait(&bars->s_free, (uint32_t)g & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            qk();
+          }
+          ok = take() && mbar_wait(&bars->p_full, (uint32_t)g & 1u);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t vb = rb + (uint32_t)(n % slots) * C::kItem;
+#pragma unroll
+          for (int ks = 0; ks < BN / 16; ++ks) {
+            const uint64_t vd = tc_desc(vb + ks * 2048, BN * 128);
+            tc_mma_ts(tO, tP + 8 * ks, vd, ipv, (i | ks) != 0);
+            tc_mma_ts(tO, tP + 32 + 8 * ks, vd, ipv, 1u);
+          }
+          tc_commit(&bars->free[n % slots]);
+          tc_commit(&bars->pv_done);
+          ++n;
+        }
+        ++seg;
+        w += cnt;
+      }
+      tc_commit(&bars->end);
+      mbar_wait(&bars->end, 0);  // no product of this CTA runs when TMEM is freed
+    }
+  } else {
+    // ---- softmax
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const float sc = soft_scale<T>(a.scale);
+    int n0 = 0, g = 0;  // items before this segment, tiles so far
+    uint32_t seg = 0;
+    for (int64_t w = begin; w < end && ok;) {
+      const Segment s = segment_at<BM, BN>(a, prefix, w, end);
+      const int cnt = s.t1 - s.t0, NR = s.n * a.G;
+      // The previous segment's products with Q are complete (its last S was taken).
+      for (int e = tid; e < BM * UR; e += 128) {
+        const int r = e / UR, u = e % UR, R = s.rt * BM + r;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (R < NR && 8 * u < D) {
+          const int i = R / a.G;
+          v = *(const uint4*)((const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(s.h * a.G + R - i * a.G) * D + 8 * u);
+        }
+        *(uint4*)(qs + (u >> 3) * (BM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = v;
+      }
+      fence_async();
+      mbar_arrive(&bars->q_full);
+
+      const int R = s.rt * BM + tid, i = R / a.G, row = s.row0 + i;
+      float m = -INFINITY, l = 0.f;
+      for (int t = 0; t < cnt; ++t, ++g) {
+        if (!warp_wait(&bars->s_full, (uint32_t)g & 1u)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        float x[2][32];
+        tc_ld32(tS + lanes, x[0]);
+        tc_ld32(tS + lanes + 32, x[1]);
+        tc_wait_ld();
+        tc_fence_before();
+        mbar_arrive(&bars->s_free);
+        const int j0 = (s.t0 + t) * BN;
+        const bool tree = j0 + BN > s.ctx;
+        if (tree) {
+          const uint64_t see = seen64(a, s, row, i, j0);
+#pragma unroll
+          for (int k = 0; k < 64; ++k)
+            if (!(see >> k & 1u)) x[k >> 5][k & 31] = -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < 64; ++k) mx = fmaxf(mx, x[k >> 5][k & 31]);
+        mx *= sc;  // scale > 0
+        const bool grown = mx > m + 8.f || (m == -INFINITY && mx > m);
+        float alpha = 1.f;
+        const bool rescale = __any_sync(0xffffffffu, grown);
+        if (rescale) {
+          const float mn = fmaxf(m, mx);
+          alpha = soft_exp<T>(m - (mn == -INFINITY ? 0.f : mn));
+          m = mn;
+          l *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 64; ++k) {
+          float& v = x[k >> 5][k & 31];
+          v = soft_exp<T>(fmaf(v, sc, -base));
+          sum[k & 3] += v;
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (tree && (a.mask || s.n > 1)) {
+          // A V that some row is blind to must not count even where it is not finite (0 * NaN):
+          // such values leave the tile here and come back, for the rows that see them, with the
+          // output. The slot stays until this tile's product, which waits for p_full.
+          const int item = n0 + (t == cnt - 1 ? 2 * cnt - 1 : 2 * t + 2), slot = item % slots;
+          if (!warp_wait(&bars->full[slot], (uint32_t)(item / slots) & 1u)) {
+            ok = false;
+            break;
+          }
+          uint32_t found = 0;
+          for (int e = tid; e < BN * UR; e += 128) {
+            uint4* p = (uint4*)(ring + (size_t)slot * C::kItem + e * 16);
+            uint4 v = *p;
+            const uint32_t b0 = tc_nonfinite<T>(v.x), b1 = tc_nonfinite<T>(v.y), b2 = tc_nonfinite<T>(v.z), b3 = tc_nonfinite<T>(v.w);
+            if (b0 | b1 | b2 | b3) {
+              found = 1;
+              *p = make_uint4(v.x & ~b0, v.y & ~b1, v.z & ~b2, v.w & ~b3);
+            }
+          }
+          if (found) bars->dirty = seg + 1;
+          fence_async();
+        }
+        if (g > 0 && !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (rescale && t > 0) {
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            float o[32];
+            tc_ld32(tO + lanes + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] *= alpha;
+            tc_st32(tO + lanes + c, *(const uint32_t(*)[32])o);
+          }
+        }
+        uint32_t p[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          float& v0 = x[k >> 4][(2 * k) & 31];
+          float& v1 = x[k >> 4][(2 * k + 1) & 31];
+          p[k] = tc_pack(v0, v1, (T*)nullptr);
+          const float2 h = tc_unpack(p[k], (T*)nullptr);
+          v0 -= h.x;
+          v1 -= h.y;
+        }
+        tc_st32(tP + lanes, p);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) p[k] = tc_pack(x[k >> 4][(2 * k) & 31], x[k >> 4][(2 * k + 1) & 31], (T*)nullptr);
+        tc_st32(tP + lanes + 32, p);
+        tc_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars->p_full);
+      }
+      if (!ok || !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      // Every softmax thread's mark of this segment is visible once all have handed their last P on;
+      // the next segment's come after all have passed here (its first S waits for all of Q).
+      if (!warp_wait(&bars->p_full, (uint32_t)(g - 1) & 1u)) {
+        ok = false;
+        break;
+      }
+      const bool dirty = *(volatile uint32_t*)&bars->dirty == seg + 1;
+      const bool whole = s.t0 == 0 && s.t1 == s.tiles, live = R < NR;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (w == begin ? 0 : 1);
+      const int head = s.h * a.G + R - i * a.G;
+      const bool empty = live && l == 0.f && !sees_any(a, row, s.n, s.ctx);
+      const float inv = 1.f / l;
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        if (c >= D && whole) break;
+        float o[32];
+        tc_ld32(tO + lanes + c, o);
+        tc_wait_ld();
+        if (dirty && live) {
+          const int last = min(s.len, s.t1 * BN);
+          for (int j = max(s.ctx, s.t0 * BN); j < last; ++j) {
+            if (!sees_node(a, row, i, j - s.ctx)) continue;
+            const int64_t off = paged_offset(a.c, a.b.table + (int64_t)s.b * a.b.table_stride, a.b.table_stride, j);
+            if (off < 0) continue;
+            const uint32_t* src = (const uint32_t*)(a.c.v + off + (int64_t)s.h * a.c.head_bytes + 2 * c);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              if (c + 2 * k >= D) break;
+              const uint32_t v = src[k], bad = tc_nonfinite<T>(v);
+              const float2 f = tc_unpack(v, (T*)nullptr);
+              if (bad & 1u) o[2 * k] += f.x;
+              if (bad >> 16) o[2 * k + 1] += f.y;
+            }
+          }
+        }
+        if (live && whole) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            if (c + k >= D) break;
+            float f[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) f[q] = empty ? 0.f : o[k + q] * inv;
+            store8((T*)a.out + ((int64_t)row * a.nh + head) * D + c + k, f);
+          }
+        } else if (live) {
+          float4* dst = (float4*)(a.part + (slot * BM + tid) * DP + c);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        }
+      }
+      if (live && whole && a.lse) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(m, l);
+      if (live && !whole) ((float2*)(a.part + (int64_t)2 * a.ctas * BM * DP))[slot * BM + tid] = make_float2(m, l);
+      tc_fence_before();  // O may be overwritten after the next p_full
+      ++seg;
+      n0 += 2 * cnt;
+      w += cnt;
+    }
+  }
+  if (!ok && a.err) atomicOr(a.err, PAGED_TIMEOUT);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 6) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::kCols));
+  }
+}
+
+template <typename T, int DP>
+static pp_status run_tc(const TreeArgs& a, cudaStream_t st) {
+  using C = TcCfg<DP>;
+  const int B = a.b.batch;
+  const pp_status r = launch_tree(pp_tree_tc_kernel<T, DP>, a, kTcThreads, C::smem(B), st, C::slots(B));
+  if (r != PP_OK || a.ctas == 1) return r;
+  return launch_join(pp_tree_join_kernel<T, DP, kTcBM, kTcBN>, a, kTcBM, st);
+}
+template <typename T>
+static pp_status run_tc_dim(const TreeArgs& a, int dp, cudaStream_t st) {
+  if (dp == 64) return run_tc<T, 64>(a, st);
+  if (dp == 128) return run_tc<T, 128>(a, st);
+  return run_tc<T, 256>(a, st);
+}
+pp_status run_tree_tc(const TreeArgs& a, uint32_t dtype, int dp, cudaStream_t st) {
+  return dtype == PP_BF16 ? run_tc_dim<__nv_bfloat16>(a, dp, st) : run_tc_dim<__half>(a, dp, st);
+}
+
+}  // namespace pp
