@@ -7,8 +7,8 @@
 // pp_beam_merge_kernel joins the slices of a row and then the rows of a group. The pair is one
 // 64-bit key, the logit's bits in ascending order above the inverted token, so keys are distinct,
 // the order is total (ties to the lower token) and the result is the same on every run. A slice's
-// sum is F32 over the few elements of a thread and 64-bit above that; lse, the values and their
-// comparisons are 64-bit, so that two candidates a rounding apart keep their order.
+// sum is F32; the sum over the slices, lse, the values and their comparisons are 64-bit, so that two
+// candidates keep the order of their logits and scores.
 #include <cuda_runtime.h>
 
 #include "../../include/potpori_b200.h"
@@ -19,19 +19,16 @@ using namespace pp;
 namespace pp {
 
 constexpr int kBeamThreads = 256;
-constexpr int kBeamPer = 16;                            // logits a thread holds
-constexpr int kBeamSlice = kBeamThreads * kBeamPer;     // logits of a slice
-constexpr int kBeamMax = 64;                            // beams, k
+constexpr int kBeamMax = 64;         // beams, k
+constexpr int kBeamList = 1024;      // keys of a slice at or above its bound
 constexpr int kMergeWarps = 16;
-constexpr int kCursors = 4;                             // slices a merging lane walks at once
+constexpr int kCursors = 4;          // slices a merging lane walks at once
 constexpr size_t kMergeSmem = 160 * 1024;
-constexpr int kBeamHeapMax = 2048;                      // keys of a slice at or above its bound
 
 // Of one slice of a row.
 struct SliceSum {
-  double sum;  // of exp(logit - max)
   float max;
-  int32_t bad;  // NaN or +inf seen
+  float sum;  // of exp(logit - max); NaN where a logit was NaN or +inf
 };
 
 struct BeamArgs {
@@ -67,30 +64,28 @@ __device__ __forceinline__ uint64_t warp_max_u64(uint64_t v) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// One slice of one row: grid (slices, rows). A bound that at least k keys reach: the slice is cut
-// into G >= k groups, and the k-th largest of the groups' largest keys has k keys at or above it.
-// Keys at or above the bound (k plus a few, at most kBeamHeapMax as they lie in k groups) are
-// gathered and put in order by counting.
-template <typename T, int G>
+// One slice of one row: grid (slices, rows); a thread holds PER logits, in 16-byte units adjacent
+// over the threads. A bound that at least k logits reach: the k-th largest among the maxima of G >= k
+// groups (G = 32: lane l of all warps; G = 256: every thread). Logits at or above the bound, k and a
+// few more, are gathered as keys and put in order by counting. Only where more than kBeamList logits
+// are equal at the bound (a slice of constants) are the k best found one by one.
+template <typename T, int G, int PER>
 __global__ void __launch_bounds__(kBeamThreads) pp_beam_rows_kernel(const BeamArgs a) {
-  __shared__ float s_max[kBeamThreads / 32];
-  __shared__ double s_sum[kBeamThreads / 32];
-  __shared__ int s_bad[kBeamThreads / 32];
-  __shared__ uint64_t s_group[G];
-  __shared__ uint64_t s_bound;
+  constexpr int W = kBeamThreads / 32, V = 16 / (int)sizeof(T), U = PER / V, SLICE = kBeamThreads * PER;
+  __shared__ uint32_t s_top[kBeamThreads];
+  __shared__ SliceSum s_part[W];
   __shared__ int s_n;
-  __shared__ uint64_t s_keys[kBeamHeapMax];
+  __shared__ uint64_t s_keys[kBeamList];
+  __shared__ uint64_t s_pick[W];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t row = blockIdx.y;
   const int64_t slice = row * a.slices + blockIdx.x;
-  const int first = blockIdx.x * kBeamSlice, n = min(kBeamSlice, a.vocab - first);
+  const int first = blockIdx.x * SLICE, n = min(SLICE, a.vocab - first);
   pdl_launch_dependents();
   if (a.finished && a.finished[row]) return;  // its one candidate needs no logits
   const T* src = (const T*)a.logits + row * a.row_stride + first;
 
-  // Thread t holds elements [e0(i), e0(i) + V) for unit i, units V wide and adjacent over threads.
-  constexpr int V = 16 / (int)sizeof(T), U = kBeamPer / V;
-  float x[kBeamPer];
+  float x[PER];
   const bool wide = ((uintptr_t)src & 15) == 0;
 #pragma unroll
   for (int i = 0; i < U; ++i) {
@@ -107,88 +102,107 @@ __global__ void __launch_bounds__(kBeamThreads) pp_beam_rows_kernel(const BeamAr
   }
   auto token = [&](int i) { return (uint32_t)(first + ((i / V) * kBeamThreads + tid) * V + i % V); };
 
-  float mx = -INFINITY;
-  int best = 0;
-  bool bad = false;
+  float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int i = 0; i < kBeamPer; ++i) {
-    bad |= !(x[i] < INFINITY);  // NaN and +inf
-    if (x[i] > mx) {
-      mx = x[i];
-      best = i;
-    }
-  }
-  uint64_t key = 0;
-#pragma unroll
-  for (int i = 0; i < kBeamPer; ++i)
-    if (i == best) key = beam_key(mx, token(i));
-  const float wm = warp_max(mx);
-  const uint32_t any_bad = __ballot_sync(0xffffffffu, bad);
-  if (lane == 0) {
-    s_max[warp] = wm;
-    s_bad[warp] = any_bad != 0;
-  }
-  // Groups: all the elements of G threads' worth each; group g = threads g, g + G, ...
-  if (tid < G) s_group[tid] = 0;
+  for (int i = 0; i < PER; ++i) part[i & 3] = fmaxf(part[i & 3], x[i]);
+  const float mx = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  const uint32_t top = mx == -INFINITY ? 0u : ordered(mx);
+  s_top[tid] = top;
   if (tid == 0) s_n = 0;
-  __syncthreads();
-  if (G == kBeamThreads) s_group[tid & (G - 1)] = key;
-  else atomicMax((unsigned long long*)&s_group[tid & (G - 1)], (unsigned long long)key);
-  float bm = s_max[0];
-  int bb = s_bad[0];
+  // The warp's sum, about its own maximum: F32 over the thread's few and the 32 lanes. The difference
+  // x - max is what is multiplied by log2 e, so the large terms are the exact ones. NaN or +inf
+  // among the logits make it NaN.
+  const uint32_t wt = __reduce_max_sync(0xffffffffu, top);
+  const float wm = wt ? from_ordered(wt) : 0.f;
+  float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int w = 1; w < kBeamThreads / 32; ++w) {
-    bm = fmaxf(bm, s_max[w]);
-    bb |= s_bad[w];
+  for (int i = 0; i < PER; ++i) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x[i] - wm) * 1.44269504088896341f));
+    sums[i & 3] += y;
   }
-  // exp over the thread's elements; -inf everywhere (or a bad row, which is dropped) adds nothing.
-  float sum = 0.f;
-  if (bm > -INFINITY && !bb) {
-#pragma unroll
-    for (int i = 0; i < kBeamPer; ++i) sum += expf(x[i] - bm);
-  }
-  double ds = sum;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ds += __shfl_xor_sync(0xffffffffu, ds, o);
-  if (lane == 0) s_sum[warp] = ds;
+  const float ws = warp_sum((sums[0] + sums[1]) + (sums[2] + sums[3]));
+  if (lane == 0) s_part[warp] = SliceSum{wt ? wm : -INFINITY, ws};
   __syncthreads();
   if (tid == 0) {
-    double t = 0;
-    for (int w = 0; w < kBeamThreads / 32; ++w) t += s_sum[w];
-    a.sums[slice] = SliceSum{t, bm, bb};
-  }
-  // The bound: a group key's rank is the number of larger ones.
-  if (tid < G) {
-    const uint64_t mine = s_group[tid];
-    int rank = 0;
-    for (int g = 0; g < G; ++g) {
-      const uint64_t other = s_group[g];
-      rank += other > mine || (other == mine && g < tid);
-    }
-    if (rank == a.k - 1) s_bound = mine;
-  }
-  __syncthreads();
-  const uint64_t bound = s_bound;
-  const uint32_t bound_hi = (uint32_t)(bound >> 32);
+    float m = s_part[0].max, t = 0.f;
 #pragma unroll
-  for (int i = 0; i < kBeamPer; ++i) {
-    if (x[i] == -INFINITY || ordered(x[i]) < bound_hi) continue;
-    const uint64_t c = beam_key(x[i], token(i));
-    if (c >= bound) {
+    for (int w = 1; w < W; ++w) m = fmaxf(m, s_part[w].max);
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < W; ++w) t += s_part[w].max == -INFINITY ? s_part[w].sum : s_part[w].sum * expf(s_part[w].max - base);
+    a.sums[slice] = SliceSum{m, t};
+  }
+  // The bound, by every warp for itself: k rounds of the largest of the groups' maxima.
+  uint32_t bound = 0;
+  if constexpr (G == 32) {
+    uint32_t g = s_top[lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) g = max(g, s_top[32 * w + lane]);
+    for (int i = 0; i < a.k; ++i) {
+      bound = __reduce_max_sync(0xffffffffu, g);
+      const uint32_t at = __ballot_sync(0xffffffffu, g == bound);
+      if (lane == __ffs(at) - 1) g = 0;
+    }
+  } else {
+    uint32_t g[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) g[w] = s_top[32 * w + lane];
+    for (int i = 0; i < a.k; ++i) {
+      uint32_t most = g[0];
+#pragma unroll
+      for (int w = 1; w < W; ++w) most = max(most, g[w]);
+      bound = __reduce_max_sync(0xffffffffu, most);
+      const uint32_t at = __ballot_sync(0xffffffffu, most == bound);
+      if (lane == __ffs(at) - 1) {
+        bool gone = false;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          if (!gone && g[w] == bound) {
+            g[w] = 0;
+            gone = true;
+          }
+      }
+    }
+  }
+  if (top && top >= bound) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (x[i] == -INFINITY || ordered(x[i]) < bound) continue;
       const int at = atomicAdd(&s_n, 1);
-      if (at < kBeamHeapMax) s_keys[at] = c;
+      if (at < kBeamList) s_keys[at] = beam_key(x[i], token(i));
     }
   }
   __syncthreads();
-  const int cnt = min(s_n, kBeamHeapMax);
+  const int cnt = s_n;
   uint64_t* out = a.keys + slice * a.k;
-  for (int i = tid; i < cnt; i += kBeamThreads) {
-    const uint64_t mine = s_keys[i];
-    int rank = 0;
-    for (int g = 0; g < cnt; ++g) rank += s_keys[g] > mine;
-    if (rank < a.k) out[rank] = mine;
+  if (cnt <= kBeamList) {
+    for (int i = tid; i < cnt; i += kBeamThreads) {
+      const uint64_t mine = s_keys[i];
+      int rank = 0;
+      for (int g = 0; g < cnt; ++g) rank += s_keys[g] > mine;
+      if (rank < a.k) out[rank] = mine;
+    }
+    for (int i = cnt + tid; i < a.k; i += kBeamThreads) out[i] = 0;
+  } else {
+    uint64_t last = ~0ull;
+    for (int r = 0; r < a.k; ++r) {
+      uint64_t best = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint64_t key = beam_key(x[i], token(i));
+        if (key < last && key > best) best = key;
+      }
+      best = warp_max_u64(best);
+      if (lane == 0) s_pick[warp] = best;
+      __syncthreads();
+      last = s_pick[0];
+#pragma unroll
+      for (int w = 1; w < W; ++w) last = max(last, s_pick[w]);
+      if (tid == 0) out[r] = last;
+      __syncthreads();
+    }
   }
-  for (int i = cnt + tid; i < a.k; i += kBeamThreads) out[i] = 0;
 }
 
 // A double's bits in the order of its value.
@@ -212,32 +226,27 @@ __global__ void __launch_bounds__(32 * kMergeWarps) pp_beam_merge_kernel(const B
     const float score = a.scores[row];
     const bool fin = a.finished && a.finished[row];
     bool bad = !(score < INFINITY);
-    double m = -INFINITY, sum = 0;
+    double lse = 0;
     if (!fin) {
-      int nf = 0;
+      const SliceSum* sums = a.sums + row * a.slices;
+      float m = -INFINITY;
+      for (int s = lane; s < a.slices; s += 32) m = fmaxf(m, __ldcg((const float2*)&sums[s]).x);
+      m = warp_max(m);
+      double sum = 0;
       for (int s = lane; s < a.slices; s += 32) {
-        const SliceSum t = a.sums[row * a.slices + s];
-        nf |= t.bad;
-        if (!t.bad && t.sum > 0) {
-          const double nm = fmax(m, (double)t.max);
-          sum = sum * exp(m - nm) + t.sum * exp((double)t.max - nm);
-          m = nm;
-        }
+        const float2 t = __ldcg((const float2*)&sums[s]);
+        sum += t.x == -INFINITY ? (double)t.y : (double)t.y * exp((double)t.x - (double)m);
       }
-      bad |= __any_sync(0xffffffffu, nf);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const double om = __shfl_xor_sync(0xffffffffu, m, o), os = __shfl_xor_sync(0xffffffffu, sum, o);
-        const double nm = fmax(m, om);
-        if (nm > -INFINITY) sum = sum * exp(m - nm) + os * exp(om - nm);
-        m = nm;
-      }
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      bad |= isnan(sum);
+      lse = (double)m + log(sum);
     }
     if (bad && lane == 0 && a.err) atomicOr(a.err, PAGED_NONFINITE);
     const int state = bad || score == -INFINITY ? 2 : fin ? 1 : 0;
     if (lane == 0) {
       s_state[b] = state;
-      s_lse[b] = state == 0 ? m + log(sum) : 0.0;
+      s_lse[b] = lse;
     }
     if (state != 0) continue;
     // The row's k best keys, from a copy in shared memory where it fits (a pop then waits for
@@ -346,19 +355,28 @@ __global__ void __launch_bounds__(32 * kMergeWarps) pp_beam_merge_kernel(const B
 
 struct BeamWork {
   uint64_t sums, keys, total;
+  uint32_t per, slices;
   BeamWork(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k) {
-    const uint64_t slices = (vocab + (uint64_t)kBeamSlice - 1) / kBeamSlice, rows = (uint64_t)groups * beams;
+    const uint64_t rows = (uint64_t)groups * beams;
+    // 32 logits a thread; 8, so that more CTAs share it, where that is not two a SM.
+    per = rows * ((vocab + 32ull * kBeamThreads - 1) / (32ull * kBeamThreads)) >= 2 * 148 ? 32 : 8;
+    slices = (uint32_t)((vocab + (uint64_t)per * kBeamThreads - 1) / ((uint64_t)per * kBeamThreads));
     sums = 0;
     keys = rows * slices * sizeof(SliceSum);
     total = keys + rows * slices * k * 8;
   }
 };
 
-template <typename T>
+template <typename T, int PER>
 void launch_rows(const BeamArgs& a, dim3 grid, cudaStream_t st) {
   // Up to 16 of a slice: 32 groups; above, a group per thread.
-  if (a.k <= 16) pp_beam_rows_kernel<T, 32><<<grid, kBeamThreads, 0, st>>>(a);
-  else pp_beam_rows_kernel<T, kBeamThreads><<<grid, kBeamThreads, 0, st>>>(a);
+  if (a.k <= 16) pp_beam_rows_kernel<T, 32, PER><<<grid, kBeamThreads, 0, st>>>(a);
+  else pp_beam_rows_kernel<T, kBeamThreads, PER><<<grid, kBeamThreads, 0, st>>>(a);
+}
+template <typename T>
+void launch_rows(const BeamArgs& a, uint32_t per, dim3 grid, cudaStream_t st) {
+  if (per == 32) launch_rows<T, 32>(a, grid, st);
+  else launch_rows<T, 8>(a, grid, st);
 }
 
 }  // namespace pp
@@ -398,7 +416,7 @@ extern "C" pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t 
   a.beams = (int32_t)beams;
   a.vocab = (int32_t)vocab;
   a.k = (int32_t)k;
-  a.slices = (int32_t)((vocab + kBeamSlice - 1) / kBeamSlice);
+  a.slices = (int32_t)w.slices;
   a.sums = (SliceSum*)((uint8_t*)work + w.sums);
   a.keys = (uint64_t*)((uint8_t*)work + w.keys);
   a.out_scores = out_scores;
@@ -407,9 +425,9 @@ extern "C" pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t 
   a.err = err;
   const cudaStream_t st = (cudaStream_t)stream;
   const dim3 grid(a.slices, groups * beams);
-  if (dtype == PP_F32) launch_rows<float>(a, grid, st);
-  else if (dtype == PP_BF16) launch_rows<__nv_bfloat16>(a, grid, st);
-  else launch_rows<__half>(a, grid, st);
+  if (dtype == PP_F32) launch_rows<float>(a, w.per, grid, st);
+  else if (dtype == PP_BF16) launch_rows<__nv_bfloat16>(a, w.per, grid, st);
+  else launch_rows<__half>(a, w.per, grid, st);
   const pp_status r = launch_status("pp_beam_select");
   if (r != PP_OK) return r;
   const size_t base = (size_t)beams * k * 8 + (size_t)beams * 8, copy = (size_t)a.slices * k * 8;
@@ -418,9 +436,8 @@ extern "C" pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t 
   a.staged = base + warps * copy <= kMergeSmem;
   if (!a.staged) warps = (int)(beams < (uint32_t)kMergeWarps ? beams : kMergeWarps);
   const size_t smem = base + (a.staged ? warps * copy : 0);
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(pp_beam_merge_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)kMergeSmem) != cudaSuccess)
+  static bool done[64] = {};
+  if (!reserve_smem(pp_beam_merge_kernel, (int)kMergeSmem, cuda_device, done))
     return paged_fail(PP_E_CUDA, "cannot reserve the merge's shared memory");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(groups);

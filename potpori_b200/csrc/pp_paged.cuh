@@ -57,6 +57,19 @@ inline int sm_count(int dev) noexcept {
   return n[dev];
 }
 
+// Lets `kernel` take up to `bytes` of dynamic shared memory on the current device, once per device
+// (`done`: one flag per device of this kernel).
+template <typename K>
+inline bool reserve_smem(K kernel, int bytes, int dev, bool (&done)[64]) noexcept {
+  if (dev < 0 || dev >= 64) return false;
+  if (!done[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    done[dev] = true;
+  }
+  return true;
+}
+constexpr int kMaxSmem = 232448;  // 227 KB: the most a CTA can have
+
 // The rules every paged operator shares; nullptr when the descriptor can be run.
 inline const char* cache_problem(const pp_paged_cache* c) noexcept {
   if (!c || !c->k || !c->v) return "null cache";
@@ -203,30 +216,35 @@ struct Elem<__half> {
   static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
 };
 
-// 8 consecutive elements in registers: 16 bytes of a 2-byte type, 32 of F32.
-template <typename T>
-struct alignas(16) Vec8 {
-  T e[8];
-};
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  Vec8<T> v;
-  const uint4* s = (const uint4*)p;
-  uint4* d = (uint4*)&v;
+// N consecutive elements (N * sizeof(T) a multiple of 8 bytes, aligned to the smaller of that and
+// 16) as F32.
+template <typename T, int N>
+__device__ __forceinline__ void load_n(const T* p, float* f) {
+  alignas(16) T v[N];
+  if constexpr (N * sizeof(T) % 16 == 0) {
 #pragma unroll
-  for (int i = 0; i < (int)sizeof(Vec8<T>) / 16; ++i) d[i] = s[i];
+    for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i) ((uint4*)v)[i] = ((const uint4*)p)[i];
+  } else {
+    *(uint2*)v = *(const uint2*)p;
+  }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = Elem<T>::get(v.e[i]);
+  for (int i = 0; i < N; ++i) f[i] = Elem<T>::get(v[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_n(T* p, const float* f) {
+  alignas(16) T v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = Elem<T>::put(f[i]);
+  if constexpr (N * sizeof(T) % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < (int)(N * sizeof(T) / 16); ++i) ((uint4*)p)[i] = ((const uint4*)v)[i];
+  } else {
+    *(uint2*)p = *(const uint2*)v;
+  }
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-  Vec8<T> v;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v.e[i] = Elem<T>::put(f[i]);
-  const uint4* s = (const uint4*)&v;
-  uint4* d = (uint4*)p;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(Vec8<T>) / 16; ++i) d[i] = s[i];
+  store_n<T, 8>(p, f);
 }
 
 }  // namespace pp

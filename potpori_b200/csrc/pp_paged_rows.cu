@@ -67,10 +67,11 @@ __device__ __forceinline__ void place_row(const AppendArgs& a, int t, int lane, 
   *out = r;
 }
 
-// One CTA per row and share of its heads. A head is taken by tph lanes of 8 dims each, so loads
-// and stores are 16-byte units in address order; the rotation partner of a rotate-half pair is
-// rotary_dim / 16 lanes away (a shuffle), an interleaved pair sits in one lane. The row's
-// rotary_dim / 2 angles are formed once in shared memory and serve every head.
+// One CTA per row and share of its heads. tph lanes take a head, 8 dims each, as two runs of 4: of
+// the rotated dims lane j holds both halves' run j, so that a pair never leaves its lane, of the
+// others 8 in a row. (Interleaved pairs: all dims 8 in a row.) The row's rotary_dim / 2 angles are
+// formed once, in shared memory, and a lane keeps its own for all heads; its first head is fetched
+// while the row's place and angles are found.
 template <typename TI, typename TC>
 __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendArgs a) {
   __shared__ float2 cs[128];
@@ -78,76 +79,73 @@ __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendA
   const int t = blockIdx.x, tid = threadIdx.x;
   const int D = a.c.head_dim, K = a.c.n_kv, heads = a.nh + 2 * K;
   const int per = kAppendThreads / a.tph, grp = tid / a.tph, j = tid % a.tph;
-  const bool dims = 8 * j < D;
-  auto source = [&](int slot) -> const TI* {
-    if (slot < a.nh) return (const TI*)a.q + (int64_t)t * a.q_stride + (int64_t)slot * D + 8 * j;
-    if (slot < a.nh + K)
-      return (const TI*)a.k + (int64_t)t * a.k_stride + (int64_t)(slot - a.nh) * D + 8 * j;
-    return (const TI*)a.v + (int64_t)t * a.v_stride + (int64_t)(slot - a.nh - K) * D + 8 * j;
+  const bool dims = 8 * j < D, turns = 8 * j < a.rot;
+  const int d0 = turns && !a.interleaved ? 4 * j : 8 * j;
+  const int d1 = turns && !a.interleaved ? a.rot / 2 + 4 * j : 8 * j + 4;
+  auto fetch = [&](int slot, float (&x)[8]) {
+    const TI* src;
+    if (slot < a.nh) src = (const TI*)a.q + (int64_t)t * a.q_stride + slot * D;
+    else if (slot < a.nh + K) src = (const TI*)a.k + (int64_t)t * a.k_stride + (slot - a.nh) * D;
+    else src = (const TI*)a.v + (int64_t)t * a.v_stride + (slot - a.nh - K) * D;
+    load_n<TI, 4>(src + d0, x);
+    load_n<TI, 4>(src + d1, x + 4);
   };
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  const int first = blockIdx.y * per;
+  float next[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int step = per * gridDim.y;
+  int slot = blockIdx.y * per + grp;
+  if (slot < heads && dims) fetch(slot, next);
 
   if (tid < 32) place_row(a, t, tid, &place);
   __syncthreads();
   if (!place.in_batch) return;
-  if (a.inv_freq && tid < a.rot / 2) cs[tid] = rotation(place.pos, a.inv_freq[tid]);
+  if (tid < a.rot / 2) cs[tid] = rotation(place.pos, a.inv_freq[tid]);
   __syncthreads();
+  float2 r[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = turns ? cs[4 * j + i] : make_float2(1.f, 0.f);
 
-  for (int s0 = first; s0 < heads; s0 += per * gridDim.y) {
-    const int slot = s0 + grp;
+  for (int s0 = blockIdx.y * per; s0 < heads; s0 += step, slot += step) {
     const bool live = slot < heads && dims;
-    if (live) load8(source(slot), x);
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = next[i];
+    if (slot + step < heads && dims) fetch(slot + step, next);
     const bool isq = slot < a.nh, isv = slot >= a.nh + K;
-    const float* w = isq ? a.q_norm : a.k_norm;
-    // Per-head RMSNorm; the sum of squares over the head's lanes.
-    float ss = 0.f;
-    if (live)
+    const float* w = isq ? a.q_norm : isv ? nullptr : a.k_norm;
+    if (a.q_norm || a.k_norm) {  // per-head RMSNorm; the sum of squares over the head's lanes
+      float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-    for (int o = a.tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (live && !isv && w) {
-      const float rms = sqrtf(ss / (float)D + a.eps);
+      for (int o = a.tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (live && w) {
+        const float rms = sqrtf(ss / (float)D + a.eps);
+        const float4 w0 = *(const float4*)(w + d0), w1 = *(const float4*)(w + d1);
+        const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] / rms * w[8 * j + i];
-    }
-    if (a.inv_freq) {
-      float y[8];
-      if (a.interleaved) {
-        if (8 * j < a.rot) {
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const float2 r = cs[4 * j + i / 2];
-            y[i] = x[i] * r.x - x[i + 1] * r.y;
-            y[i + 1] = x[i + 1] * r.x + x[i] * r.y;
-          }
-        }
-      } else {
-        const int hl = a.rot / 16;  // lanes of half the rotated dims
-        const int lane = tid & 31;
-        const int from = j < hl ? lane + hl : j < 2 * hl ? lane - hl : lane;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], from);
-        if (j < 2 * hl) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 r = cs[(j < hl ? 8 * j : 8 * (j - hl)) + i];
-            y[i] = j < hl ? x[i] * r.x - y[i] * r.y : x[i] * r.x + y[i] * r.y;
-          }
-        }
+        for (int i = 0; i < 8; ++i) x[i] = x[i] / rms * wv[i];
       }
-      if (!isv && 8 * j < a.rot)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = y[i];
     }
     if (!live) continue;
-    if (isq) {
-      store8((TC*)a.q_out + ((int64_t)t * a.nh + slot) * D + 8 * j, x);
-    } else if (place.offset >= 0) {
-      const int h = isv ? slot - a.nh - K : slot - a.nh;
-      uint8_t* row = (isv ? a.c.v : a.c.k) + place.offset + (int64_t)h * a.c.head_bytes;
-      store8((TC*)row + 8 * j, x);
+    if (turns && !isv) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float& p = a.interleaved ? x[2 * i] : x[i];
+        float& q = a.interleaved ? x[2 * i + 1] : x[4 + i];
+        const float p0 = p, q0 = q;
+        p = p0 * r[i].x - q0 * r[i].y;
+        q = q0 * r[i].x + p0 * r[i].y;
+      }
     }
+    TC* dst;
+    if (isq) {
+      dst = (TC*)a.q_out + ((int64_t)t * a.nh + slot) * D;
+    } else {
+      if (place.offset < 0) continue;
+      const int h = isv ? slot - a.nh - K : slot - a.nh;
+      dst = (TC*)((isv ? a.c.v : a.c.k) + place.offset + (int64_t)h * a.c.head_bytes);
+    }
+    store_n<TC, 4>(dst + d0, x);
+    store_n<TC, 4>(dst + d1, x + 4);
   }
 }
 
@@ -325,9 +323,11 @@ struct ReorderArgs {
   uint32_t* err;
 };
 constexpr int kReorderThreads = 128;
+constexpr int kReorderBatch = 4;  // units a lane holds between its loads and its stores
 
 // Grid (slices of the 2 * layers planes, new beams, groups). Only beams that take their spare
-// page copy: a warp per cached row, lanes over its 16-byte units.
+// page copy: lanes over the 16-byte units of a row, warps over the rows, four loads before
+// their stores.
 __global__ void __launch_bounds__(kReorderThreads) pp_beam_reorder_kernel(const ReorderArgs a) {
   const int j = blockIdx.y, g = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int32_t* mine = a.beams + (int64_t)g * a.new_beams;
@@ -368,14 +368,21 @@ __global__ void __launch_bounds__(kReorderThreads) pp_beam_reorder_kernel(const 
     uint8_t* base = (plane & 1 ? a.c.v : a.c.k) + (int64_t)(plane >> 1) * a.c.layer_bytes;
     const uint8_t* sp = base + (int64_t)from * a.c.page_bytes;
     uint8_t* dp = base + (int64_t)to * a.c.page_bytes;
-    for (int row = warp; row < part; row += kReorderThreads / 32)
-#pragma unroll 4
-      for (int u = lane; u < per_row; u += 32) {
-        const int h = u / a.units;
-        const int64_t off = (int64_t)row * a.c.row_bytes + (int64_t)h * a.c.head_bytes +
-                            (int64_t)(u - h * a.units) * 16;
-        *(uint4*)(dp + off) = *(const uint4*)(sp + off);
+    for (int u = lane; u < per_row; u += 32) {
+      const int h = u / a.units;
+      const int64_t col = (int64_t)h * a.c.head_bytes + (int64_t)(u - h * a.units) * 16;
+      for (int r0 = warp; r0 < part; r0 += kReorderBatch * kReorderThreads / 32) {
+        uint4 hold[kReorderBatch];
+#pragma unroll
+        for (int i = 0; i < kReorderBatch; ++i)
+          if (r0 + i * kReorderThreads / 32 < part)
+            hold[i] = *(const uint4*)(sp + col + (int64_t)(r0 + i * kReorderThreads / 32) * a.c.row_bytes);
+#pragma unroll
+        for (int i = 0; i < kReorderBatch; ++i)
+          if (r0 + i * kReorderThreads / 32 < part)
+            *(uint4*)(dp + col + (int64_t)(r0 + i * kReorderThreads / 32) * a.c.row_bytes) = hold[i];
       }
+    }
   }
 }
 
@@ -453,7 +460,8 @@ extern "C" pp_status pp_paged_append(const pp_paged_cache* cache, const pp_paged
   const int64_t unit = 16 / e;
   const bool vec = (natural | (uintptr_t)r->q_out) % 16 == 0 && r->k_stride % unit == 0 &&
                    r->v_stride % unit == 0 && (!nh || r->q_stride % unit == 0) &&
-                   a.rot % (a.interleaved ? 8 : 16) == 0;
+                   a.rot % 8 == 0 &&
+                   ((uintptr_t)r->q_norm | (uintptr_t)r->k_norm) % 16 == 0;
   const cudaStream_t st = (cudaStream_t)stream;
   const int rows = (int)batch->rows;
   if (r->dtype == PP_F32) launch_append_to<float>(a, cache->dtype, vec, rows, st, sms);

@@ -11,16 +11,11 @@ using namespace pp;
 
 namespace pp {
 
-// ---- 16-bit caches -------------------------------------------------------------------------
-// CTA of 4 warps: WM warps over the rows (16 each), 4 / WM over the keys of a 64-key tile, each
-// with its own running maximum, sum and output, joined in shared memory when the unit's segment
-// ends. Q stays in registers; K and V tiles come through a ring of NS stages by 16-byte
-// asynchronous copies, each row from wherever its page is. With WM = 1 (up to 16 query vectors, a
-// decoded token or a short chain) a warp fetches and consumes its own 16 keys of every tile and
-// the loop has no CTA barrier.
+// ---- 16-bit caches, few query vectors --------------------------------------------------------
 constexpr int kTreeThreads = 128;
 constexpr int kTreeBN = 64;
-constexpr uint64_t kTreeTcAbove = 32;  // more query vectors of a head than this: pp_tree_tc.cu
+constexpr int kTreeWholeTiles = 4;
+constexpr uint64_t kTreeTcAbove = 8;  // more query vectors of a head than this: pp_tree_tc.cu
 
 template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -50,380 +45,393 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   hi = pack2(ah, bh);
   lo = pack2(Elem<T>::put(a - Elem<T>::get(ah)), Elem<T>::put(b - Elem<T>::get(bh)));
 }
-// Exponent all ones in either half of a register of T.
-template <typename T>
-__device__ __forceinline__ uint32_t nonfinite_halves(uint32_t v) {
-  constexpr uint32_t E = sizeof(T) == 2 && __is_same(T, __half) ? 0x7c00u : 0x7f80u;
-  return ((v & E) == E ? 0xffffu : 0u) | ((v >> 16 & E) == E ? 0xffff0000u : 0u);
+// The narrow kernel's shared memory: a ring of NS stages for each of the four warps, 16 rows of K and
+// of V as 64-dim blocks [16 rows][128 bytes], the 16-byte unit u of row r at u ^ (r & 7).
+template <int DP>
+struct NarrowCfg {
+  static constexpr int BM = 8, KW = 16, NS = DP == 256 ? 2 : 3, kPerSm = DP == 256 ? 1 : 2;
+  static constexpr int kTile = KW * DP * 2, kStage = 2 * kTile, kRing = 4 * NS * kStage;
+  static constexpr int kOPitch = DP + 4;
+  static_assert(4 * BM * (kOPitch * 4 + 8) <= kRing, "the warps' outputs take the ring's place");
+  // Nothing is static, so that the dynamic part starts on the 1024 bytes that the swizzle counts from.
+  static constexpr int kBars = 4 * NS * 8 + 16;
+  static constexpr size_t smem(int batch) { return kRing + kBars + 4 * (size_t)(batch + 1); }
+};
+// Byte offset of 16-byte unit u (dims 8 u ..) of row r in a tile of it.
+__device__ __forceinline__ int narrow_unit(int r, int u) { return (u >> 3) * 2048 + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
+
+// A warp's 16 rows of K and V by 16-byte copies, for pages that boxes do not fit.
+template <int DP>
+__device__ __forceinline__ void narrow_copy(const TreeArgs& a, const RowFetch<16>& f, uint8_t* kd, int lane) {
+  constexpr int UR = DP / 8, RP = 32 / UR;
+  const int u = lane % UR, sub = lane / UR;
+#pragma unroll
+  for (int i = 0; i < 16 / RP; ++i) {
+    const int l = i * RP + sub;
+    const int64_t off = f.row(a, l);
+    const bool read = off >= 0 && 8 * u < a.c.head_dim;
+    const int64_t at = read ? off + 16 * u : 0;
+    cp_async16(kd + narrow_unit(l, u), a.c.k + at, read);
+    cp_async16(kd + NarrowCfg<DP>::kTile + narrow_unit(l, u), a.c.v + at, read);
+  }
 }
 
-template <int DP, int WM>
-struct TreeCfg {
-  static constexpr int WN = 4 / WM, BM = 16 * WM, BN = kTreeBN, KW = BN / WN;
-  static constexpr int NS = DP == 256 ? 2 : 3;
-  static constexpr int kRow = DP * 2, kTile = BN * kRow, kStage = 2 * kTile;
-  static constexpr int kOPitch = DP + 4;
-  static constexpr int kQ = BM * kRow;
-  static constexpr int kOut = 4 * 16 * kOPitch * 4 + 4 * 16 * 8;  // outputs and (max, sum) of 4 warps
-  static constexpr int kRing = NS * kStage > kOut ? NS * kStage : kOut;
-  static constexpr size_t smem(int batch) { return kRing + kQ + 8 * (size_t)(batch + 1); }
-};
-
-template <typename T, int DP, int WM>
-__global__ void __launch_bounds__(kTreeThreads) pp_tree_mma_kernel(const TreeArgs a) {
-  using C = TreeCfg<DP, WM>;
-  constexpr int WN = C::WN, BM = C::BM, BN = C::BN, KW = C::KW, NS = C::NS, RB = C::kRow;
-  constexpr int UR = DP / 8;  // 16-byte units of a row
-  extern __shared__ __align__(128) uint8_t sm[];
-  uint8_t* ring = sm;
-  uint8_t* qs = sm + C::kRing;
-  int64_t* prefix = (int64_t*)(qs + C::kQ);
-  __shared__ int64_t scan[4];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int wm = warp % WM, wn = warp / WM, g4 = lane >> 2, t4 = lane & 3;
+// Up to 8 query vectors of a cached head in a row tile (a decoded token with G <= 8): keys are the
+// products' M dimension and the vectors N, S^T = K Q^T and O^T = V^T P^T on mma.sync, half the
+// products and half the accumulators of a 16-row tile; at 8 rows the cache's bytes bound it, not the
+// tensor cores. A warp fetches (TMA, 16-row boxes) and consumes its own 16 keys of every 64-key
+// tile, so the loop has no CTA barrier. P^T turns from S^T's layout to an operand's by movmatrix.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
+    pp_tree_narrow_kernel(const TreeArgs a, const __grid_constant__ TreeMaps maps) {
+  using C = NarrowCfg<DP>;
+  constexpr int BM = 8, BN = kTreeBN, NS = C::NS, KS = DP / 16, NB = DP / 64;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  uint64_t* full = (uint64_t*)(sm + C::kRing);  // [4][NS]
+  uint32_t* scan = (uint32_t*)(full + 4 * NS);
+  uint32_t* prefix = scan + 4;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
   const int D = a.c.head_dim;
   const float sc = soft_scale<T>(a.scale);
-
+  const bool tma = maps.box != 0;
+  uint8_t* ring = sm + warp * NS * C::kStage;  // the warp's
+  uint64_t* bar = full + warp * NS;
+  if (smem_u32(sm) & 1023u) {  // cannot be: no join, and the caller is told
+    if (tid == 0) write_join<BM>(a, nullptr, 1);
+    if (tid == 0 && a.err) atomicOr(a.err, PAGED_TIMEOUT);
+    return;
+  }
+  if (lane == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(&bar[i], 1);
+    fence_barrier_init();
+  }
   pdl_launch_dependents();
   tile_prefix<BM, BN, kTreeThreads>(a, prefix, scan, blockIdx.x == 0);
-  const int64_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
-  const int64_t begin = blockIdx.x * per, end = min(total, begin + per);
+  const uint32_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
+  uint32_t begin, end;
+  cta_range(per, total, blockIdx.x, begin, end);
+  if (begin >= end && tid == 0) write_join<BM>(a, nullptr, per);
+  uint32_t n = 0;  // tiles that the warp has taken through its ring
+  bool ok = true;
 
-  for (int64_t w = begin; w < end;) {
+  for (uint32_t w = begin; w < end;) {
     const Segment s = segment_at<BM, BN>(a, prefix, w, end);
+    if (w == begin && tid == 0) write_join<BM>(a, &s, per);
     const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
-    const int NR = s.n * a.G;
-
-    // A warp fetches 16 rows of every tile (with WM = 1 those that it consumes). Lane l < 16 looks
-    // row l's page up a tile ahead of the copies, so that no copy waits for the page table.
-    auto look = [&](int t) -> int64_t {
-      const int idx = t * BN + warp * 16 + (lane & 15);
-      if (t >= s.t1 || idx >= s.len) return -1;
-      const int64_t off = paged_offset(a.c, table, a.b.table_stride, idx);
-      if (off < 0) {
-        if (a.err && lane < 16) atomicOr(a.err, PAGED_BAD_PAGE);
-        return -1;
-      }
-      return off + (int64_t)s.h * a.c.head_bytes;
+    RowFetch<16> rows;
+    BoxPlace box;
+    auto look = [&](int t) {
+      const int idx = t * BN + warp * 16;
+      if (tma) box.look(a, s, table, idx, t < s.t1);
+      else rows.look(a, s, table, idx, t < s.t1, lane);
     };
-    auto load_tile = [&](int stage, int64_t mine) {
-      constexpr int RP = 32 / UR;
-      const int u = lane % UR, sub = lane / UR;
-      uint8_t* kd = ring + stage * C::kStage;
-#pragma unroll
-      for (int i = 0; i < 16 / RP; ++i) {
-        const int l = i * RP + sub, r = warp * 16 + l;
-        const int64_t off = __shfl_sync(0xffffffffu, mine, l);
-        const bool read = off >= 0 && 8 * u < D;
-        const int64_t at = read ? off + 16 * u : 0;
-        const int dst = r * RB + ((u ^ (r & 7)) << 4);
-        cp_async16(kd + dst, a.c.k + at, read);
-        cp_async16(kd + C::kTile + dst, a.c.v + at, read);
+    // Tile t, whose place was looked up, into its stage. A stage that ordinary loads have read is
+    // handed to the copy engine by the proxy fence.
+    auto fetch = [&](int t) {
+      const uint32_t stage = (n + (uint32_t)(t - s.t0)) % NS;
+      if (tma) {
+        if (t < s.t1) {
+          if (lane == 0) {
+            fence_async();
+            mbar_arrive_expect_tx(&bar[stage], C::kStage);
+          }
+          __syncwarp();
+          if (lane < 2 * NB)
+            tma_box(ring + stage * C::kStage + lane * 2048, lane < NB ? &maps.k : &maps.v, &bar[stage], maps,
+                    64 * (lane % NB), s.h, box.row, box.page);
+        }
+      } else {
+        if (t < s.t1) narrow_copy<DP>(a, rows, ring + stage * C::kStage, lane);
+        cp_async_commit();
       }
     };
-    auto sync = [&] {
-      if constexpr (WM == 1) __syncwarp();
-      else __syncthreads();
-    };
-
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i) {
-      if (s.t0 + i < s.t1) load_tile(i, look(s.t0 + i));
-      cp_async_commit();
+      look(s.t0 + i);
+      fetch(s.t0 + i);
     }
-    int64_t ahead = look(s.t0 + NS - 1);
-    // Queries: BM rows, zero past the unit's.
-    for (int e = tid; e < BM * UR; e += kTreeThreads) {
-      const int r = e / UR, u = e % UR, R = s.rt * BM + r;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (R < NR && 8 * u < D) {
-        const int i = R / a.G;
-        v = *(const uint4*)((const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride +
-                            (int64_t)(s.h * a.G + R - i * a.G) * D + 8 * u);
-      }
-      *(uint4*)(qs + r * RB + ((u ^ (r & 7)) << 4)) = v;
-    }
-    __syncthreads();
-    constexpr bool kQReg = DP <= 128;
-    uint32_t qa[kQReg ? DP / 16 : 1][4];
-    const int qrow = wm * 16 + (lane & 15);
-    const uint8_t* qp = qs + qrow * RB;
-    if constexpr (kQReg) {
+    look(s.t0 + NS - 1);
+    // Q^T fragments: vector g4, dims 16 ks + 2 t4 and + 8.
+    uint32_t qb[KS][2];
+    {
+      const int R = s.rt * BM + g4, i = R / a.G;
+      const bool in = R < s.n * a.G;
+      const T* q = (const T*)a.q + (int64_t)(s.row0 + (in ? i : 0)) * a.q_stride + (int64_t)(s.h * a.G + (in ? R - i * a.G : 0)) * D;
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks)
-        ldmatrix_x4a(qa[ks], qp + (((2 * ks + (lane >> 4)) ^ (qrow & 7)) << 4));
-    }
-    // The thread's two rows: g4 and g4 + 8 of the warp's 16.
-    const int RA = s.rt * BM + wm * 16 + g4, RBw = RA + 8;
-    const int iA = RA / a.G, iB = RBw / a.G;
-
-    float o[DP / 8][4];
+      for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-    for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    float mrow[2] = {-INFINITY, -INFINITY}, lrow[2] = {0.f, 0.f};
+        for (int e = 0; e < 2; ++e) {
+          const int d = 16 * ks + 8 * e + 2 * t4;
+          qb[ks][e] = in && d < D ? *(const uint32_t*)(q + d) : 0u;
+        }
+    }
+    // The thread's two vectors: 2 t4 and 2 t4 + 1.
+    const int i0 = (s.rt * BM + 2 * t4) / a.G, i1 = (s.rt * BM + 2 * t4 + 1) / a.G;
+    float o[KS][4];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    // ldmatrix rows of the lane: K as [16 keys][16 dims], V the same, transposed.
+    const int kr = lane & 15, ku = lane >> 4, vr = (lane & 7) + ((lane >> 4) << 3), vu = (lane >> 3) & 1;
 
     for (int t = s.t0; t < s.t1; ++t) {
-      const int stage = (t - s.t0) % NS;
-      cp_async_wait<NS - 2>();
-      sync();
-      if (t + NS - 1 < s.t1) load_tile((t - s.t0 + NS - 1) % NS, ahead);
-      cp_async_commit();
-      ahead = look(t + NS);
+      const uint32_t at = n + (uint32_t)(t - s.t0), stage = at % NS;
+      if (tma) {
+        if (!warp_wait(&bar[stage], at / NS & 1u)) {
+          ok = false;
+          // Let the copies in flight land before the shared memory is released.
+          for (int q = t + 1; q < s.t1 && q < t + NS - 1; ++q) {
+            const uint32_t k = n + (uint32_t)(q - s.t0);
+            warp_wait(&bar[k % NS], k / NS & 1u);
+          }
+          break;
+        }
+      } else {
+        cp_async_wait<NS - 2>();
+      }
+      __syncwarp();
+      fetch(t + NS - 1);
+      look(t + NS);
       const uint8_t* kt = ring + stage * C::kStage;
-      const uint8_t* vt = kt + C::kTile;
-      const int kb = wn * KW;
+      uint8_t* vt = ring + stage * C::kStage + C::kTile;
+      const int j0 = t * BN + warp * 16;
 
-      float x[KW / 8][4];
+      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};  // even and odd k steps
 #pragma unroll
-      for (int j = 0; j < KW / 8; ++j) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) {
+      for (int ks = 0; ks < KS; ++ks) {
         if (16 * ks >= D) break;
-        uint32_t qf[4];
-        if constexpr (kQReg) {
+        uint32_t kf[4];
+        ldmatrix_x4a(kf, kt + narrow_unit(kr, 2 * ks + ku));
+        mma16<T>(ks & 1 ? y : x, kf, qb[ks][0], qb[ks][1]);
+      }
+      // Element e: key g4 + 8 (e >> 1), vector 2 t4 + (e & 1).
+      const bool tree = j0 + 16 > s.ctx;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) qf[e] = qa[ks][e];
-        } else {
-          ldmatrix_x4a(qf, qp + (((2 * ks + (lane >> 4)) ^ (qrow & 7)) << 4));
-        }
-#pragma unroll
-        for (int np = 0; np < KW / 16; ++np) {
-          const int r = kb + 16 * np + (lane & 7) + ((lane >> 4) << 3);
-          uint32_t kf[4];
-          ldmatrix_x4a(kf, kt + r * RB + (((2 * ks + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
-          mma16<T>(x[2 * np], qf, kf[0], kf[1]);
-          mma16<T>(x[2 * np + 1], qf, kf[2], kf[3]);
+      for (int e = 0; e < 4; ++e) {
+        x[e] = (x[e] + y[e]) * sc;
+        if (tree) {
+          const int node = j0 + g4 + 8 * (e >> 1) - s.ctx, i = e & 1 ? i1 : i0;
+          if (node >= 0 && (node >= s.n || i >= s.n || !sees_node(a, s.row0 + i, i, node))) x[e] = -INFINITY;
         }
       }
-      // Scale; mask where the tile reaches past the context.
-      const int j0 = t * BN + kb;
-      const bool tree = j0 + KW > s.ctx;
-      float mx[2] = {-INFINITY, -INFINITY};
+      float mx[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
 #pragma unroll
-      for (int j = 0; j < KW / 8; ++j)
+      for (int sh = 4; sh < 32; sh <<= 1)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = x[j][e] * sc;
-          if (tree) {
-            const int node = j0 + 8 * j + 2 * t4 + (e & 1) - s.ctx;
-            const int i = e < 2 ? iA : iB;
-            if (node >= 0 && (node >= s.n || i >= s.n || !sees_node(a, s.row0 + i, i, node))) v = -INFINITY;
+        for (int q = 0; q < 2; ++q) mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], sh));
+      // The old maximum serves until a score passes it by 2^8: P stays small enough, and the output
+      // need not be rescaled at every small step.
+      const bool grown = mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f || (m[0] == -INFINITY && mx[0] > m[0]) ||
+                         (m[1] == -INFINITY && mx[1] > m[1]);
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float mn = fmaxf(m[q], mx[q]);
+          const float alpha = soft_exp<T>(m[q] - (mn == -INFINITY ? 0.f : mn));
+          m[q] = mn;
+          l[q] *= alpha;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            o[k][q] *= alpha;
+            o[k][q + 2] *= alpha;
           }
-          x[j][e] = v;
-          mx[e >> 1] = fmaxf(mx[e >> 1], v);
-        }
-      float base[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-        const float mn = fmaxf(mrow[i], mx[i]);
-        base[i] = mn == -INFINITY ? 0.f : mn;
-        const float alpha = soft_exp<T>(mrow[i] - base[i]);
-        mrow[i] = mn;
-        lrow[i] *= alpha;
-#pragma unroll
-        for (int n = 0; n < DP / 8; ++n) {
-          o[n][2 * i] *= alpha;
-          o[n][2 * i + 1] *= alpha;
         }
       }
+      const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
 #pragma unroll
-      for (int j = 0; j < KW / 8; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[j][e] = soft_exp<T>(x[j][e] - base[e >> 1]);
-          lrow[e >> 1] += x[j][e];
-        }
-      // Hidden nodes: their V must not count even where it is not finite (0 * NaN). Look for such
-      // values only where some row can be blind to a node.
+      for (int e = 0; e < 4; ++e) {
+        x[e] = soft_exp<T>(x[e] - base[e & 1]);
+        l[e & 1] += x[e];
+      }
+      // Positions past the end hold whatever their page did: zeros there. And a V that some row is
+      // blind to must not count even where it is not finite (0 * NaN): then its halves are cleared as
+      // the product reads them, and added below for the rows that see them.
       bool dirty = false;
-      if (tree && (a.mask || s.n > 1)) {
+      const bool blind = tree && (a.mask || s.n > 1);
+      if (blind || j0 + 16 > s.len) {
         uint32_t found = 0;
-        for (int e = lane; e < KW * UR; e += 32) {
-          const uint4 v = *(const uint4*)(vt + kb * RB + e * 16);
-          found |= nonfinite_halves<T>(v.x) | nonfinite_halves<T>(v.y) | nonfinite_halves<T>(v.z) | nonfinite_halves<T>(v.w);
-        }
-        dirty = __any_sync(0xffffffffu, found != 0);
-      }
-      // O += P V. P is carried as hi + lo parts: rounded to T alone it would add as much error as
-      // the rounding of the output.
-#pragma unroll
-      for (int ks = 0; ks < KW / 16; ++ks) {
-        uint32_t ph[4], pl[4];
-        split2<T>(x[2 * ks][0], x[2 * ks][1], ph[0], pl[0]);
-        split2<T>(x[2 * ks][2], x[2 * ks][3], ph[1], pl[1]);
-        split2<T>(x[2 * ks + 1][0], x[2 * ks + 1][1], ph[2], pl[2]);
-        split2<T>(x[2 * ks + 1][2], x[2 * ks + 1][3], ph[3], pl[3]);
-        const int r = kb + 16 * ks + (lane & 7) + (((lane >> 3) & 1) << 3);
-#pragma unroll
-        for (int dp = 0; dp < DP / 16; ++dp) {
-          if (16 * dp >= D) break;
-          uint32_t vf[4];
-          ldmatrix_x4_trans(vf, vt + r * RB + (((2 * dp + (lane >> 4)) ^ (r & 7)) << 4));
-          if (dirty) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) vf[e] &= ~nonfinite_halves<T>(vf[e]);
+        for (int e = lane; e < 16 * (DP / 8); e += 32) {
+          uint4* p = (uint4*)(vt + e * 16);
+          if (j0 + ((e >> 3) & 15) >= s.len) {
+            *p = make_uint4(0u, 0u, 0u, 0u);
+          } else if (blind) {
+            const uint4 v = *p;
+            found |= nonfinite_halves<T>(v.x) | nonfinite_halves<T>(v.y) | nonfinite_halves<T>(v.z) | nonfinite_halves<T>(v.w);
           }
-          mma16<T>(o[2 * dp], ph, vf[0], vf[1]);
-          mma16<T>(o[2 * dp + 1], ph, vf[2], vf[3]);
-          mma16<T>(o[2 * dp], pl, vf[0], vf[1]);
-          mma16<T>(o[2 * dp + 1], pl, vf[2], vf[3]);
         }
+        dirty = __any_sync(0xffffffffu, found != 0);  // and the zeros are seen by every lane
+        __syncwarp();
       }
-      if (dirty) {  // the non-finite values of V, for the rows that see them
+      // P is carried as hi + lo parts: rounded to T alone it would add as much error as the rounding
+      // of the output.
+      uint32_t ph[2], pl[2];
+      split2<T>(x[0], x[1], ph[0], pl[0]);
+      split2<T>(x[2], x[3], ph[1], pl[1]);
 #pragma unroll
-        for (int j = 0; j < KW / 8; ++j)
+      for (int e = 0; e < 2; ++e) {
+        ph[e] = movmatrix(ph[e]);
+        pl[e] = movmatrix(pl[e]);
+      }
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if (16 * k >= D) break;
+        uint32_t vf[4];
+        ldmatrix_x4_trans(vf, vt + narrow_unit(vr, 2 * k + vu));
+        if (dirty) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf[e] &= ~nonfinite_halves<T>(vf[e]);
+        }
+        mma16<T>(o[k], vf, ph[0], ph[1]);
+        mma16<T>(o[k], vf, pl[0], pl[1]);
+      }
+      if (dirty) {  // the non-finite values of V, for the vectors that see them
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh)
           for (int k8 = 0; k8 < 8; ++k8) {
-            const int r = kb + 8 * j + k8, node = t * BN + r - s.ctx;
-            const int from = (lane & ~3) | (k8 >> 1);
-            const float a0 = __shfl_sync(0xffffffffu, x[j][0], from), a1 = __shfl_sync(0xffffffffu, x[j][1], from);
-            const float b0 = __shfl_sync(0xffffffffu, x[j][2], from), b1 = __shfl_sync(0xffffffffu, x[j][3], from);
-            const float p0 = k8 & 1 ? a1 : a0, p1 = k8 & 1 ? b1 : b0;
+            const float p0 = __shfl_sync(0xffffffffu, x[2 * kh], k8 * 4 + t4);
+            const float p1 = __shfl_sync(0xffffffffu, x[2 * kh + 1], k8 * 4 + t4);
+            const int r = 8 * kh + k8, node = j0 + r - s.ctx;
             if (node >= s.n) continue;
-            const bool seeA = node < 0 || (iA < s.n && sees_node(a, s.row0 + iA, iA, node));
-            const bool seeB = node < 0 || (iB < s.n && sees_node(a, s.row0 + iB, iB, node));
+            const bool see0 = node < 0 || (i0 < s.n && sees_node(a, s.row0 + i0, i0, node));
+            const bool see1 = node < 0 || (i1 < s.n && sees_node(a, s.row0 + i1, i1, node));
 #pragma unroll
-            for (int n = 0; n < DP / 8; ++n) {
-              const uint32_t v = *(const uint32_t*)(vt + r * RB + ((n ^ (r & 7)) << 4) + 4 * t4);
-              const uint32_t bad = nonfinite_halves<T>(v);
-              T e2[2];
-              *(uint32_t*)e2 = v;
+            for (int k = 0; k < KS; ++k)
 #pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                if (!(bad >> (16 * q) & 1u)) continue;
-                if (seeA) o[n][q] += p0 * Elem<T>::get(e2[q]);
-                if (seeB) o[n][2 + q] += p1 * Elem<T>::get(e2[q]);
+              for (int dh = 0; dh < 2; ++dh) {
+                const float f = Elem<T>::get(*(const T*)(vt + narrow_unit(r, 2 * k + dh) + 2 * g4));
+                if (isfinite(f)) continue;
+                if (see0) o[k][2 * dh] += p0 * f;
+                if (see1) o[k][2 * dh + 1] += p1 * f;
               }
-            }
           }
       }
     }
-    cp_async_wait<0>();
-    __syncthreads();  // the ring is free
+    n += (uint32_t)(s.t1 - s.t0);
+    if (!tma) cp_async_wait<0>();
+    if (__syncthreads_or(!ok)) break;  // else the rings are free
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      lrow[i] += __shfl_xor_sync(0xffffffffu, lrow[i], 1);
-      lrow[i] += __shfl_xor_sync(0xffffffffu, lrow[i], 2);
-    }
-    // Outputs [wn][BM][DP + 4] and (max, sum) [wn][BM] of the warps.
-    float* os = (float*)ring;
-    float2* ml = (float2*)(ring + 4 * 16 * C::kOPitch * 4);
-    {
-      float* o0 = os + (size_t)(wn * BM + wm * 16 + g4) * C::kOPitch + 2 * t4;
-      float* o1 = o0 + 8 * C::kOPitch;
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        *(float2*)(o0 + 8 * n) = make_float2(o[n][0], o[n][1]);
-        *(float2*)(o1 + 8 * n) = make_float2(o[n][2], o[n][3]);
-      }
-      if (t4 == 0) {
-        ml[wn * BM + wm * 16 + g4] = make_float2(mrow[0], lrow[0]);
-        ml[wn * BM + wm * 16 + g4 + 8] = make_float2(mrow[1], lrow[1]);
-      }
+      for (int sh = 4; sh < 32; sh <<= 1) l[q] += __shfl_xor_sync(0xffffffffu, l[q], sh);
+    // Outputs [warp][8][DP + 4] and (max, sum) [warp][8] of the warps in the rings' place.
+    float* os = (float*)sm;
+    float2* ml = (float2*)(sm + 4 * BM * C::kOPitch * 4);
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        os[(warp * BM + 2 * t4 + (e & 1)) * C::kOPitch + 16 * k + g4 + 8 * (e >> 1)] = o[k][e];
+    if (g4 == 0) {
+      ml[warp * BM + 2 * t4] = make_float2(m[0], l[0]);
+      ml[warp * BM + 2 * t4 + 1] = make_float2(m[1], l[1]);
     }
     __syncthreads();
     const bool whole = s.t0 == 0 && s.t1 == s.tiles;
     const int64_t slot = 2 * (int64_t)blockIdx.x + (w == begin ? 0 : 1);
-    const int rows = min(BM, NR - s.rt * BM);
-    for (int e = tid; e < rows * UR; e += kTreeThreads) {
-      const int r = e / UR, u = e % UR, R = s.rt * BM + r, i = R / a.G;
-      float m = ml[r].x;
+    const int live = min(BM, s.n * a.G - s.rt * BM);
+    for (int e = tid; e < live * (DP / 8); e += kTreeThreads) {
+      const int r = e / (DP / 8), u = e % (DP / 8), R = s.rt * BM + r, i = R / a.G;
+      float top = ml[r].x;
 #pragma unroll
-      for (int k = 1; k < WN; ++k) m = fmaxf(m, ml[k * BM + r].x);
-      const float mb = m == -INFINITY ? 0.f : m;
-      float l = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int k = 1; k < 4; ++k) top = fmaxf(top, ml[k * BM + r].x);
+      const float tb = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < WN; ++k) {
+      for (int k = 0; k < 4; ++k) {
         const float2 v = ml[k * BM + r];
-        const float wgt = WN == 1 ? 1.f : soft_exp<T>(v.x - mb);
-        l += v.y * wgt;
-        const float* src = os + (size_t)(k * BM + r) * C::kOPitch + 8 * u;
+        const float wgt = soft_exp<T>(v.x - tb);
+        sum += v.y * wgt;
+        const float* src = os + (k * BM + r) * C::kOPitch + 8 * u;
 #pragma unroll
         for (int d = 0; d < 8; ++d) f[d] += src[d] * wgt;
       }
       if (whole) {
         const int row = s.row0 + i, head = s.h * a.G + R - i * a.G;
-        const bool empty = l == 0.f && !sees_any(a, row, s.n, s.ctx);
+        const bool empty = sum == 0.f && !sees_any(a, row, s.n, s.ctx);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) f[d] = empty ? 0.f : f[d] / l;
+        for (int d = 0; d < 8; ++d) f[d] = empty ? 0.f : f[d] / sum;
         if (8 * u < D) store8((T*)a.out + ((int64_t)row * a.nh + head) * D + 8 * u, f);
-        if (a.lse && u == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(m, l);
+        if (a.lse && u == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(top, sum);
       } else {
-        float* dst = a.part + (slot * BM + r) * DP + 8 * u;
-        *(float4*)dst = make_float4(f[0], f[1], f[2], f[3]);
-        *(float4*)(dst + 4) = make_float4(f[4], f[5], f[6], f[7]);
-        if (u == 0) ((float2*)(a.part + (int64_t)2 * a.ctas * BM * DP))[slot * BM + r] = make_float2(m, l);
+        store_n<float, 8>(a.part + (slot * BM + r) * DP + 8 * u, f);
+        if (u == 0) a.part_ml[slot * BM + r] = make_float2(top, sum);
       }
     }
-    __syncthreads();  // the ring may be filled again
-    w += s.t1 - s.t0;
+    fence_async();    // the rings go back to the copy engine
+    __syncthreads();
+    w += s.step;
   }
+  if (!ok && lane == 0 && a.err) atomicOr(a.err, PAGED_TIMEOUT);
 }
 
 // ---- F32 caches ----------------------------------------------------------------------------
 // CUDA cores: on these tensor cores three products of split halves would be needed to keep F32,
-// at the rate of an F32 multiply-add and with a worse sum. 16 query vectors, 32-key tiles.
-constexpr int kTreeFBM = 16, kTreeFBN = 32, kTreeFStages = 2;
-template <int DP>
+// at the rate of an F32 multiply-add and with a worse sum. BM query vectors (4 for a decoded token,
+// 16 else), 32-key tiles, four warps. Scores: warp w the rows w BM / 4 .., lane = key, so the softmax
+// of a row stays in its warp; output: thread = dim, all rows.
+constexpr int kTreeFBN = 32, kTreeFStages = 2;
+template <int DP, int BM>
 struct TreeFCfg {
   static constexpr int P = DP + 4;  // row pitch: 16-byte columns of consecutive rows in other banks
+  static constexpr int PP = BM + 4;  // pitch of the probabilities' rows
   static constexpr int kTile = kTreeFBN * P * 4, kStage = 2 * kTile;
-  static constexpr int kQ = kTreeFBM * P * 4;
-  static constexpr int kS = kTreeFBM * 33 * 4, kP = kTreeFBN * kTreeFBM * 4, kRows = 5 * kTreeFBM * 4;
+  static constexpr int kQ = BM * P * 4, kP = kTreeFBN * PP * 4, kRows = 2 * BM * 4;
+  static constexpr int kPerSm = DP <= 64 ? 5 : DP <= 128 ? 3 : 1;
   static constexpr size_t smem(int batch) {
-    return kTreeFStages * kStage + kQ + kP + kS + kRows + 8 * (size_t)(batch + 1) + 16;
+    return kTreeFStages * kStage + kQ + kP + kRows + 4 * (size_t)(batch + 1);
   }
 };
 
-template <int DP>
+template <int DP, int BM>
 __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArgs a) {
-  using C = TreeFCfg<DP>;
-  constexpr int BM = kTreeFBM, BN = kTreeFBN, NS = kTreeFStages, P = C::P, UR = DP / 4;
+  using C = TreeFCfg<DP, BM>;
+  constexpr int BN = kTreeFBN, NS = kTreeFStages, P = C::P, PP = C::PP, UR = DP / 4, RW = BM / 4;
   constexpr int DT = DP <= 128 ? 1 : DP / 128;  // dims of a thread: tid, tid + 128
   extern __shared__ __align__(128) uint8_t sm[];
   uint8_t* ring = sm;
   float* qs = (float*)(sm + NS * C::kStage);
-  float* pt = qs + BM * P;        // [key][row]
-  float* ss = pt + BN * BM;       // [row][33]
-  float* m_s = ss + BM * 33;
-  float* l_s = m_s + BM;
-  float* al_s = l_s + BM;
-  float* base_s = al_s + BM;
-  uint32_t* vis_s = (uint32_t*)(base_s + BM);
-  int64_t* prefix = (int64_t*)(((uintptr_t)(vis_s + BM) + 7) & ~(uintptr_t)7);
-  __shared__ int64_t scan[4];
+  float* pt = qs + BM * P;  // [key][PP]
+  float* al_s = pt + BN * PP;
+  uint32_t* vis_s = (uint32_t*)(al_s + BM);
+  uint32_t* prefix = vis_s + BM;
+  __shared__ uint32_t scan[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.c.head_dim;
 
   pdl_launch_dependents();
   tile_prefix<BM, BN, kTreeThreads>(a, prefix, scan, blockIdx.x == 0);
-  const int64_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
-  const int64_t begin = blockIdx.x * per, end = min(total, begin + per);
+  const uint32_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
+  uint32_t begin, end;
+  cta_range(per, total, blockIdx.x, begin, end);
+  if (begin >= end && tid == 0) write_join<BM>(a, nullptr, per);
 
-  for (int64_t w = begin; w < end;) {
+  for (uint32_t w = begin; w < end;) {
     const Segment s = segment_at<BM, BN>(a, prefix, w, end);
+    if (w == begin && tid == 0) write_join<BM>(a, &s, per);
     const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
     const int NR = s.n * a.G;
-    auto load_tile = [&](int t, int stage) {
-      constexpr int RP = kTreeThreads / UR;
-      const int u = tid % UR;
+    RowFetch<8> ahead;  // a warp fetches 8 rows of every tile
+    auto look = [&](int t) { ahead.look(a, s, table, t * BN + warp * 8, t < s.t1, lane); };
+    auto fetch = [&](int stage) {
       uint8_t* kd = ring + stage * C::kStage;
 #pragma unroll
-      for (int i = 0; i < BN / RP; ++i) {
-        const int r = i * RP + tid / UR, idx = t * BN + r;
-        int64_t off = -1;
-        if (idx < s.len) {
-          off = paged_offset(a.c, table, a.b.table_stride, idx);
-          if (off < 0 && a.err && u == 0) atomicOr(a.err, PAGED_BAD_PAGE);
-        }
+      for (int i = 0; i < 8 * UR / 32; ++i) {
+        const int e = lane + 32 * i, l = e / UR, u = e % UR, r = warp * 8 + l;
+        const int64_t off = ahead.row(a, l);
         const bool read = off >= 0 && 4 * u < D;
-        const int64_t at = read ? off + (int64_t)s.h * a.c.head_bytes + 16 * u : 0;
+        const int64_t at = read ? off + 16 * u : 0;
         cp_async16(kd + (r * P + 4 * u) * 4, a.c.k + at, read);
         cp_async16(kd + C::kTile + (r * P + 4 * u) * 4, a.c.v + at, read);
       }
     };
-    load_tile(s.t0, 0);
+    look(s.t0);
+    fetch(0);
     cp_async_commit();
+    look(s.t0 + 1);
     for (int e = tid; e < BM * UR; e += kTreeThreads) {
       const int r = e / UR, u = e % UR, R = s.rt * BM + r;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -434,9 +442,11 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
       }
       *(float4*)(qs + r * P + 4 * u) = v;
     }
-    if (tid < BM) {
-      m_s[tid] = -INFINITY;
-      l_s[tid] = 0.f;
+    float m[RW], l[RW];  // of the warp's rows
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
     }
     float acc[DT][BM];
 #pragma unroll
@@ -446,84 +456,104 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
 
     for (int t = s.t0; t < s.t1; ++t) {
       const int stage = (t - s.t0) % NS;
-      if (t + 1 < s.t1) load_tile(t + 1, (t + 1 - s.t0) % NS);
+      if (t + 1 < s.t1) fetch((t + 1 - s.t0) % NS);
       cp_async_commit();
+      look(t + 2);
       cp_async_wait<1>();
       __syncthreads();
-      const float* kt = (const float*)(ring + stage * C::kStage);
+      const float* kt = (const float*)(ring + stage * C::kStage) + lane * P;
       const float* vt = (const float*)(ring + stage * C::kStage + C::kTile);
-      {  // scores: keys kk, kk + 16 by rows rr, rr + 8
-        const int kk = tid & 15, rr = tid >> 4;
-        float x[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+      const float* qw = qs + warp * RW * P;
+      float x[RW][2];
+#pragma unroll
+      for (int r = 0; r < RW; ++r) x[r][0] = x[r][1] = 0.f;
 #pragma unroll 4
-        for (int d = 0; d < D; d += 4) {
-          const float4 k0 = *(const float4*)(kt + kk * P + d), k1 = *(const float4*)(kt + (kk + 16) * P + d);
-          const float4 q0 = *(const float4*)(qs + rr * P + d), q1 = *(const float4*)(qs + (rr + 8) * P + d);
-          x[0][0] += q0.x * k0.x + q0.y * k0.y + q0.z * k0.z + q0.w * k0.w;
-          x[0][1] += q0.x * k1.x + q0.y * k1.y + q0.z * k1.z + q0.w * k1.w;
-          x[1][0] += q1.x * k0.x + q1.y * k0.y + q1.z * k0.z + q1.w * k0.w;
-          x[1][1] += q1.x * k1.x + q1.y * k1.y + q1.z * k1.z + q1.w * k1.w;
+      for (int d = 0; d < D; d += 4) {
+        const float4 k = *(const float4*)(kt + d);
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+          const float4 q = *(const float4*)(qw + r * P + d);
+          x[r][0] += q.x * k.x;
+          x[r][1] += q.y * k.y;
+          x[r][0] += q.z * k.z;
+          x[r][1] += q.w * k.w;
         }
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) ss[(rr + 8 * i) * 33 + kk + 16 * k] = x[i][k];
       }
-      __syncthreads();
-      // Softmax: warp w the rows 4 w .. 4 w + 3, lane = key.
       const int node = t * BN + lane - s.ctx;
+      const bool tree = (t + 1) * BN > s.ctx;
+      float v[RW], mn[RW];
+      uint32_t seen[RW];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = 4 * warp + q, i = (s.rt * BM + r) / a.G;
-        const bool see = node < 0 || (node < s.n && i < s.n && sees_node(a, s.row0 + i, i, node));
-        const float v = see ? ss[r * 33 + lane] * a.scale : -INFINITY;
-        const float mo = m_s[r], mn = fmaxf(mo, warp_max(v)), base = mn == -INFINITY ? 0.f : mn;
-        const float p = expf(v - base);
-        const float sum = warp_sum(p);
-        const uint32_t seen = __ballot_sync(0xffffffffu, see);
-        pt[lane * BM + r] = p;
+      for (int r = 0; r < RW; ++r) {
+        bool see = true;
+        if (tree && node >= 0) {
+          const int i = (s.rt * BM + warp * RW + r) / a.G;
+          see = node < s.n && i < s.n && sees_node(a, s.row0 + i, i, node);
+        }
+        v[r] = see ? (x[r][0] + x[r][1]) * a.scale : -INFINITY;
+        mn[r] = v[r];
+        seen[r] = tree ? __ballot_sync(0xffffffffu, see) : 0u;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int r = 0; r < RW; ++r) mn[r] = fmaxf(mn[r], __shfl_xor_sync(0xffffffffu, mn[r], o));
+      float p[RW];
+#pragma unroll
+      for (int r = 0; r < RW; ++r) {
+        mn[r] = fmaxf(mn[r], m[r]);
+        const float base = mn[r] == -INFINITY ? 0.f : mn[r];
+        p[r] = expf(v[r] - base);
+        const float alpha = expf(m[r] - base);
+        m[r] = mn[r];
+        l[r] = l[r] * alpha + p[r];  // this lane's keys
         if (lane == 0) {
-          const float alpha = expf(mo - base);
-          m_s[r] = mn;
-          l_s[r] = l_s[r] * alpha + sum;
-          al_s[r] = alpha;
-          vis_s[r] = seen;
+          al_s[warp * RW + r] = alpha;
+          vis_s[warp * RW + r] = seen[r];
         }
       }
+      if constexpr (RW == 4) *(float4*)(pt + lane * PP + 4 * warp) = make_float4(p[0], p[1], p[2], p[3]);
+      else pt[lane * PP + warp] = p[0];
       __syncthreads();
-      const bool tree = (t + 1) * BN > s.ctx;
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         const int dim = tid + 128 * d;
         if (dim >= D) break;
 #pragma unroll
         for (int r = 0; r < BM; ++r) acc[d][r] *= al_s[r];
-        if (!tree) {
-#pragma unroll 4
-          for (int k = 0; k < BN; ++k) {
-            const float v = vt[k * P + dim];
+#pragma unroll 8
+        for (int k = 0; k < BN; ++k) {
+          const float v1 = vt[k * P + dim];
+          if (tree && !isfinite(v1)) {  // it must not count for the rows that do not see it (0 * NaN)
+            for (int r = 0; r < BM; ++r) {
+              const float add = vis_s[r] >> k & 1u ? pt[k * PP + r] * v1 : 0.f;
 #pragma unroll
-            for (int r = 0; r < BM; r += 4) {
-              const float4 p = *(const float4*)(pt + k * BM + r);
-              acc[d][r] += p.x * v;
-              acc[d][r + 1] += p.y * v;
-              acc[d][r + 2] += p.z * v;
-              acc[d][r + 3] += p.w * v;
+              for (int q = 0; q < BM; ++q)
+                if (q == r) acc[d][q] += add;
             }
+            continue;
           }
-        } else {  // an unseen V must not count even where it is not finite
-          const int keys = min(BN, s.len - t * BN);
-          for (int k = 0; k < keys; ++k) {
-            const float v = vt[k * P + dim];
 #pragma unroll
-            for (int r = 0; r < BM; ++r)
-              if (vis_s[r] >> k & 1u) acc[d][r] += pt[k * BM + r] * v;
+          for (int r = 0; r < BM; r += 4) {
+            const float4 pr = *(const float4*)(pt + k * PP + r);
+            acc[d][r] += pr.x * v1;
+            acc[d][r + 1] += pr.y * v1;
+            acc[d][r + 2] += pr.z * v1;
+            acc[d][r + 3] += pr.w * v1;
           }
         }
       }
-      __syncthreads();  // the stage, scores and probabilities are free
+      __syncthreads();  // the stage and the probabilities are free
     }
     cp_async_wait<0>();
+    // (max, sum) of every row, through the probabilities' space.
+    float2* ml = (float2*)pt;
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+      l[r] = warp_sum(l[r]);
+      if (lane == 0) ml[warp * RW + r] = make_float2(m[r], l[r]);
+    }
+    __syncthreads();
     const bool whole = s.t0 == 0 && s.t1 == s.tiles;
     const int64_t slot = 2 * (int64_t)blockIdx.x + (w == begin ? 0 : 1);
 #pragma unroll
@@ -531,23 +561,23 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
       const int R = s.rt * BM + r;
       if (R >= NR) break;
       const int i = R / a.G, row = s.row0 + i, head = s.h * a.G + R - i * a.G;
-      const float m = m_s[r], l = l_s[r];
+      const float2 v = ml[r];
       if (whole) {
-        const bool empty = l == 0.f && !sees_any(a, row, s.n, s.ctx);
+        const bool empty = v.y == 0.f && !sees_any(a, row, s.n, s.ctx);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
           if (tid + 128 * d < D)
-            ((float*)a.out)[((int64_t)row * a.nh + head) * D + tid + 128 * d] = empty ? 0.f : acc[d][r] / l;
-        if (a.lse && tid == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<float>(m, l);
+            ((float*)a.out)[((int64_t)row * a.nh + head) * D + tid + 128 * d] = empty ? 0.f : acc[d][r] / v.y;
+        if (a.lse && tid == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<float>(v.x, v.y);
       } else {
 #pragma unroll
         for (int d = 0; d < DT; ++d)
           if (tid + 128 * d < DP) a.part[(slot * BM + r) * DP + tid + 128 * d] = acc[d][r];
-        if (tid == 0) ((float2*)(a.part + (int64_t)2 * a.ctas * BM * DP))[slot * BM + r] = make_float2(m, l);
+        if (tid == 0) a.part_ml[slot * BM + r] = v;
       }
     }
     __syncthreads();
-    w += s.t1 - s.t0;
+    w += s.step;
   }
 }
 
@@ -555,53 +585,108 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
 // Which kernel and how many CTAs, by the query vectors that share a cached head.
 struct TreePlan {
   int dp, bm, bn, ctas;
-  bool tc;
+  bool tc, whole;
   uint64_t work;
 };
-inline TreePlan tree_plan(const pp_paged_cache& c, const pp_paged_batch& b, uint32_t n_heads, int sms, bool tc_ok) {
+inline TreePlan tree_plan(const pp_paged_cache& c, const pp_paged_batch& b, uint32_t n_heads, int sms) {
   TreePlan p;
   p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   const uint64_t G = n_heads / c.n_kv_heads, vectors = (uint64_t)(b.max_rows ? b.max_rows : 1) * G;
-  p.tc = tc_ok && c.dtype != PP_F32 && vectors > kTreeTcAbove;
+  p.tc = c.dtype != PP_F32 && vectors > kTreeTcAbove;
+  uint64_t per_sm = 2;
   if (c.dtype == PP_F32) {
-    p.bm = kTreeFBM;
+    p.bm = vectors <= 4 ? 4 : 16;
     p.bn = kTreeFBN;
+    per_sm = p.dp == 64 ? 5 : p.dp == 128 ? 3 : 1;
   } else {
-    p.bm = p.tc ? 128 : vectors <= 16 ? 16 : vectors <= 32 ? 32 : 64;
+    p.bm = p.tc ? 128 : 8;
     p.bn = kTreeBN;
+    if (p.dp == 256) per_sm = 1;
   }
   const uint64_t units = ((uint64_t)b.rows * G / p.bm + b.batch) * c.n_kv_heads;
-  const uint64_t tiles = units * (((uint64_t)b.max_len + p.bn - 1) / p.bn + 1);
-  const uint64_t most = (uint64_t)sms * (p.dp == 256 ? 1 : 2);
+  // A cache of a few tiles is not worth the second kernel.
+  p.whole = b.max_len <= (uint32_t)kTreeWholeTiles * p.bn;
+  const uint64_t tiles = units * (p.whole ? 1 : ((uint64_t)b.max_len + p.bn - 1) / p.bn + 1);
+  const uint64_t most = (uint64_t)sms * per_sm;
   p.ctas = (int)(tiles < most ? (tiles ? tiles : 1) : most);
-  p.work = 2ull * p.ctas * p.bm * (p.dp + 2) * 4;
+  p.work = 2ull * p.ctas * p.bm * (p.dp + 2) * 4 + (uint64_t)p.ctas * sizeof(JoinRec);
   return p;
 }
 
-template <typename T, int DP, int WM>
-pp_status run_tree_mma(const TreeArgs& a, cudaStream_t st) {
-  using C = TreeCfg<DP, WM>;
-  const pp_status r = launch_tree(pp_tree_mma_kernel<T, DP, WM>, a, kTreeThreads, C::smem(a.b.batch), st);
-  if (r != PP_OK || a.ctas == 1) return r;
-  return launch_join(pp_tree_join_kernel<T, DP, C::BM, C::BN>, a, C::BM, st);
+// Tensor maps of the layer's K and V; box 0 (16-byte copies then) where they do not fit.
+inline TreeMaps tree_maps(const pp_paged_cache& c, const PagedView& v, int most) noexcept {
+  TreeMaps m = {};
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return (Encode)p;
+  }();
+  if (!encode || c.dtype == PP_F32 || c.page_size % 16) return m;
+  int box = most;
+  while (c.page_size % box) box >>= 1;
+  // Heads, rows and pages by ascending stride; a dimension of one element takes any stride.
+  struct Dim {
+    uint64_t size, stride;
+    int what;
+  } d[3] = {{c.n_kv_heads, (uint64_t)v.head_bytes, 0}, {c.page_size, (uint64_t)v.row_bytes, 1},
+            {c.n_pages, (uint64_t)v.page_bytes, 2}};
+  for (Dim& x : d) {
+    if (x.size == 1) x.stride = (uint64_t)c.head_dim * 2;
+    if (x.stride >= (1ull << 40)) return m;
+  }
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (d[j].stride > d[j + 1].stride) {
+        const Dim t = d[j];
+        d[j] = d[j + 1];
+        d[j + 1] = t;
+      }
+  cuuint64_t size[4] = {c.head_dim}, stride[3];
+  cuuint32_t box_dim[4] = {64, 1, 1, 1}, one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 3; ++i) {
+    size[i + 1] = d[i].size;
+    stride[i] = d[i].stride;
+    if (d[i].what == 0) m.at_head = i + 1;
+    else if (d[i].what == 1) m.at_row = i + 1, box_dim[i + 1] = box;
+    else m.at_page = i + 1;
+  }
+  const CUtensorMapDataType t = c.dtype == PP_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  for (int i = 0; i < 2; ++i)
+    if (encode(i ? &m.v : &m.k, t, 4, i ? v.v : v.k, size, stride, box_dim, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return m;
+  m.box = box;
+  return m;
 }
+
 template <typename T, int DP>
-pp_status run_tree_rows(const TreeArgs& a, int bm, cudaStream_t st) {
-  if (bm == 16) return run_tree_mma<T, DP, 1>(a, st);
-  if (bm == 32) return run_tree_mma<T, DP, 2>(a, st);
-  return run_tree_mma<T, DP, 4>(a, st);
+pp_status run_tree_narrow(const TreeArgs& a, const TreeMaps& m, cudaStream_t st) {
+  const pp_status r = launch_tree<pp_tree_narrow_kernel<T, DP>>(a, kTreeThreads, NarrowCfg<DP>::smem(a.b.batch), st, m);
+  if (r != PP_OK || a.whole) return r;
+  return launch_join<T, DP>(a, st);
 }
 template <typename T>
-pp_status run_tree_16(const TreeArgs& a, int dp, int bm, cudaStream_t st) {
-  if (dp == 64) return run_tree_rows<T, 64>(a, bm, st);
-  if (dp == 128) return run_tree_rows<T, 128>(a, bm, st);
-  return run_tree_rows<T, 256>(a, bm, st);
+pp_status run_tree_16(const TreeArgs& a, const TreeMaps& m, int dp, cudaStream_t st) {
+  if (dp == 64) return run_tree_narrow<T, 64>(a, m, st);
+  if (dp == 128) return run_tree_narrow<T, 128>(a, m, st);
+  return run_tree_narrow<T, 256>(a, m, st);
+}
+template <int DP, int BM>
+pp_status run_tree_f32_rows(const TreeArgs& a, cudaStream_t st) {
+  const pp_status r = launch_tree<pp_tree_f32_kernel<DP, BM>>(a, kTreeThreads, TreeFCfg<DP, BM>::smem(a.b.batch), st);
+  if (r != PP_OK || a.whole) return r;
+  return launch_join<float, DP>(a, st);
 }
 template <int DP>
 pp_status run_tree_f32(const TreeArgs& a, cudaStream_t st) {
-  const pp_status r = launch_tree(pp_tree_f32_kernel<DP>, a, kTreeThreads, TreeFCfg<DP>::smem(a.b.batch), st);
-  if (r != PP_OK || a.ctas == 1) return r;
-  return launch_join(pp_tree_join_kernel<float, DP, kTreeFBM, kTreeFBN>, a, kTreeFBM, st);
+  return a.bm == 4 ? run_tree_f32_rows<DP, 4>(a, st) : run_tree_f32_rows<DP, 16>(a, st);
 }
 
 inline const char* tree_problem(const pp_paged_cache* c, const pp_paged_batch* b, uint32_t n_heads) {
@@ -610,6 +695,12 @@ inline const char* tree_problem(const pp_paged_cache* c, const pp_paged_batch* b
   if (n_heads == 0 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > 1024)
     return "n_heads must be a multiple of n_kv_heads, at most 1024 times it";
   if (b->max_rows > (1u << 20)) return "max_rows out of range";
+  // The line of tiles is counted in 32 bits, whatever the device's lengths turn out to be.
+  const uint64_t G = n_heads / c->n_kv_heads;
+  const uint64_t units = ((uint64_t)b->rows * G / 4 + b->batch) * c->n_kv_heads;
+  const uint64_t longest = (uint64_t)b->table_stride * c->page_size;
+  if (longest > 0x7fffffffull) return "a page table of more than 2^31 positions";
+  if (units * (longest / 32 + 1) > 0x7fffffffull) return "rows times positions out of range";
   return nullptr;
 }
 
@@ -622,10 +713,7 @@ extern "C" uint64_t pp_tree_attention_work_bytes(const pp_paged_cache* cache, co
     return 0;
   }
   const int found = sm_count(cache->cuda_device), sms = found ? found : 148;
-  // Enough for either kernel: which one runs also depends on the query.
-  const uint64_t x = tree_plan(*cache, *batch, n_heads, sms, true).work;
-  const uint64_t y = tree_plan(*cache, *batch, n_heads, sms, false).work;
-  return x > y ? x : y;
+  return tree_plan(*cache, *batch, n_heads, sms).work;
 }
 
 extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_paged_batch* batch,
@@ -646,8 +734,7 @@ extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_pag
   DeviceScope dev(cache->cuda_device);
   const int sms = dev.ok ? sm_count(cache->cuda_device) : 0;
   if (!sms) return paged_fail(PP_E_CUDA, "cannot use the cache's device");
-  // The tcgen05 kernel takes the maximum before the scale.
-  const TreePlan p = tree_plan(*cache, *batch, q->n_heads, sms, q->scale > 0.f);
+  const TreePlan p = tree_plan(*cache, *batch, q->n_heads, sms);
   if ((uintptr_t)work % 16 || work_bytes < p.work)
     return paged_fail(PP_E_INVALID, "work must be 16-byte aligned and pp_tree_attention_work_bytes long");
   if (batch->rows == 0) return PP_OK;
@@ -663,9 +750,13 @@ extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_pag
   a.nh = (int32_t)q->n_heads;
   a.G = (int32_t)(q->n_heads / cache->n_kv_heads);
   a.scale = q->scale;
+  a.bm = p.bm;
   a.part = (float*)work;
+  a.part_ml = (float2*)(a.part + 2ll * p.ctas * p.bm * p.dp);
+  a.recs = (JoinRec*)(a.part_ml + 2ll * p.ctas * p.bm);
   a.ctas = p.ctas;
-  a.min_per = 1;
+  a.whole = p.whole;
+  a.dev = cache->cuda_device;
   a.err = err;
   const cudaStream_t st = (cudaStream_t)stream;
   if (cache->dtype == PP_F32) {
@@ -673,7 +764,8 @@ extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_pag
     if (p.dp == 128) return run_tree_f32<128>(a, st);
     return run_tree_f32<256>(a, st);
   }
-  if (p.tc) return run_tree_tc(a, cache->dtype, p.dp, st);
-  if (cache->dtype == PP_BF16) return run_tree_16<__nv_bfloat16>(a, p.dp, p.bm, st);
-  return run_tree_16<__half>(a, p.dp, p.bm, st);
+  const TreeMaps m = tree_maps(*cache, a.c, p.tc ? 64 : 16);
+  if (p.tc) return run_tree_tc(a, m, cache->dtype, p.dp, st);
+  if (cache->dtype == PP_BF16) return run_tree_16<__nv_bfloat16>(a, m, p.dp, st);
+  return run_tree_16<__half>(a, m, p.dp, st);
 }

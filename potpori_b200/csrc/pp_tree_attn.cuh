@@ -16,6 +16,8 @@
 
 namespace pp {
 
+struct JoinRec;
+
 struct TreeArgs {
   PagedView c;  // the layer
   BatchView b;
@@ -26,9 +28,13 @@ struct TreeArgs {
   const uint32_t* mask;
   int32_t mask_words, nh, G;
   float scale;
-  float* part;      // [2 * ctas][BM][DP] outputs, then [2 * ctas][BM] (max, sum)
+  float* part;      // [2 * ctas][BM][DP] outputs
+  float2* part_ml;  // [2 * ctas][BM] (max, sum)
+  JoinRec* recs;  // [ctas]
   int32_t ctas;     // CTAs that the line of tiles is cut over
-  int32_t min_per;  // least tiles of a CTA
+  int32_t bm;       // rows of a tile
+  int32_t whole;    // units are not cut (short caches): no partials, no join
+  int32_t dev;
   uint32_t* err;
 };
 
@@ -37,33 +43,34 @@ __device__ __forceinline__ bool bad_sequence(const TreeArgs& a, int n, int len) 
   return n < 0 || len < n || (int64_t)len > (int64_t)a.b.table_stride * a.c.page.d;
 }
 
-// prefix[b] = tiles before sequence b on the line; prefix[batch] = all. By the whole CTA
+// prefix[b] = tiles (units, where they are not cut) before sequence b on the line; prefix[batch] =
+// all. By the whole CTA
 // (NT threads), scan: NT / 32 words of shared memory.
 template <int BM, int BN, int NT>
-__device__ __forceinline__ void tile_prefix(const TreeArgs& a, int64_t* prefix, int64_t* scan,
+__device__ __forceinline__ void tile_prefix(const TreeArgs& a, uint32_t* prefix, uint32_t* scan,
                                             bool report) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.b.batch;
-  const int each = (B + NT - 1) / NT, b0 = tid * each, b1 = min(B, b0 + each);
-  int64_t sum = 0;
+  const int each = (B + NT - 1) / NT, b0 = min(B, tid * each), b1 = min(B, b0 + each);
+  uint32_t sum = 0;
   for (int b = b0; b < b1; ++b) {
     const int n = a.b.cu_rows[b + 1] - a.b.cu_rows[b], len = a.b.kv_len[b];
     prefix[b] = sum;  // inside this thread's share
     if (bad_sequence(a, n, len)) {
       if (report && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
     } else if (n > 0) {
-      const int64_t rts = ((int64_t)n * a.G + BM - 1) / BM;
-      sum += rts * a.c.n_kv * ((len + BN - 1) / BN);
+      const uint32_t rts = ((uint32_t)n * a.G + BM - 1) / BM;
+      sum += rts * a.c.n_kv * (a.whole ? 1 : (len + BN - 1) / BN);
     }
   }
-  int64_t inc = sum;
+  uint32_t inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += v;
   }
   if (lane == 31) scan[warp] = inc;
   __syncthreads();
-  int64_t before = inc - sum;
+  uint32_t before = inc - sum;
   for (int w = 0; w < warp; ++w) before += scan[w];
   for (int b = b0; b < b1; ++b) prefix[b] += before;
   if (tid == NT - 1) prefix[B] = before + sum;
@@ -75,11 +82,12 @@ struct Segment {
   int32_t b, h, rt;           // unit
   int32_t t0, t1, tiles;      // key tiles [t0, t1) of `tiles`
   int32_t row0, n, len, ctx;  // first row of the sequence, nodes, positions, context positions
-  int64_t unit0;              // place of the unit's first tile on the line
+  uint32_t unit0;             // place of the unit's first tile on the line
+  uint32_t step;              // places on the line that the segment takes
 };
 template <int BM, int BN>
-__device__ __forceinline__ Segment segment_at(const TreeArgs& a, const int64_t* prefix, int64_t w,
-                                              int64_t end) {
+__device__ __forceinline__ Segment segment_at(const TreeArgs& a, const uint32_t* prefix, uint32_t w,
+                                              uint32_t end) {
   int lo = 0, hi = a.b.batch;  // last b with prefix[b] <= w: the one with tiles, as w < prefix[b + 1]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -93,17 +101,49 @@ __device__ __forceinline__ Segment segment_at(const TreeArgs& a, const int64_t* 
   s.len = a.b.kv_len[lo];
   s.ctx = s.len - s.n;
   s.tiles = (s.len + BN - 1) / BN;
-  const int64_t off = w - prefix[lo], unit = off / s.tiles;
-  s.t0 = (int)(off - unit * s.tiles);
-  s.rt = (int)(unit / a.c.n_kv);
-  s.h = (int)(unit - (int64_t)s.rt * a.c.n_kv);
-  s.t1 = (int)min((int64_t)s.tiles, s.t0 + (end - w));
+  const uint32_t line = a.whole ? 1 : s.tiles;
+  const uint32_t off = w - prefix[lo], unit = off / line;
+  s.t0 = (int)(off - unit * line);
+  s.rt = (int)(unit / (uint32_t)a.c.n_kv);
+  s.h = (int)(unit - (uint32_t)s.rt * a.c.n_kv);
+  s.t1 = a.whole ? s.tiles : (int)min((uint32_t)s.tiles, s.t0 + (end - w));
   s.unit0 = w - s.t0;
+  s.step = a.whole ? 1 : s.t1 - s.t0;
   return s;
 }
-__device__ __forceinline__ int64_t tiles_per_cta(const TreeArgs& a, int64_t total) {
-  const int64_t even = (total + a.ctas - 1) / a.ctas;
-  return even > a.min_per ? even : a.min_per;
+__device__ __forceinline__ uint32_t tiles_per_cta(const TreeArgs& a, uint32_t total) {
+  return max((total + a.ctas - 1) / a.ctas, 1u);
+}
+// Range of the line that CTA `cta` takes.
+__device__ __forceinline__ void cta_range(uint32_t per, uint32_t total, uint32_t cta, uint32_t& begin,
+                                          uint32_t& end) {
+  begin = min((uint64_t)cta * per, (uint64_t)total);
+  end = min(begin + per, total);
+}
+
+// What the join has to know of a unit whose last tile this CTA took and whose first one it did
+// not; parts = 0 for a CTA without such a unit. Only a CTA's first segment can be one.
+struct JoinRec {
+  int32_t parts, rows;      // partials, rows of the tile
+  int32_t first_slot, cta;  // slot of the first partial; the others are 2 * (cta + p)
+  int32_t row0, vec0, head0, see;  // first array row, vector of row 0, first head; n << 1 | (ctx > 0)
+};
+template <int BM>
+__device__ __forceinline__ void write_join(const TreeArgs& a, const Segment* s, uint32_t per) {
+  if (a.whole) return;
+  JoinRec r = {};
+  if (s && s->t0 > 0 && s->t1 == s->tiles) {
+    const uint32_t c0 = s->unit0 / per;
+    r.parts = (int)(blockIdx.x - c0) + 1;
+    r.rows = min(BM, s->n * a.G - s->rt * BM);
+    r.first_slot = (int)(c0 * per == s->unit0 ? 2 * c0 : 2 * c0 + 1);
+    r.cta = (int)c0;
+    r.row0 = s->row0;
+    r.vec0 = s->rt * BM;
+    r.head0 = s->h * a.G;
+    r.see = s->n << 1 | (s->ctx > 0);
+  }
+  a.recs[blockIdx.x] = r;
 }
 
 // Whether row (sequence row i) sees node j (0 <= j < n).
@@ -123,6 +163,91 @@ __device__ __forceinline__ bool sees_any(const TreeArgs& a, int row, int n, int 
   }
   return false;
 }
+
+// K and V of the layer as tensor maps (TMA), for 16-bit caches with pages of a multiple of 16
+// positions: 64-dim boxes of `box` rows of one page, 128-byte swizzled. Dimension 0 is the head's dim;
+// heads, rows and pages are the dimensions at_head, at_row and at_page in order of their strides.
+// A box at page n_pages is out of range and reads zeros: so do absent pages.
+struct TreeMaps {
+  CUtensorMap k, v;
+  int32_t box;  // rows of a box; 0: no maps, 16-byte copies instead
+  int32_t at_head, at_row, at_page;
+};
+__device__ __forceinline__ void tma_box(void* dst, const CUtensorMap* map, uint64_t* bar, const TreeMaps& m,
+                                        int32_t x, int32_t head, int32_t row, int32_t page) {
+  const int32_t c1 = m.at_head == 1 ? head : m.at_row == 1 ? row : page;
+  const int32_t c2 = m.at_head == 2 ? head : m.at_row == 2 ? row : page;
+  const int32_t c3 = m.at_head == 3 ? head : m.at_row == 3 ? row : page;
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+// Page and row in it of position idx (a multiple of the box's rows); page n_pages where there is
+// nothing to read.
+struct BoxPlace {
+  int32_t page, row;
+  __device__ __forceinline__ void look(const TreeArgs& a, const Segment& s, const int32_t* table, int idx, bool in_range) {
+    page = a.c.n_pages;
+    row = 0;
+    if (!in_range || idx >= s.len) return;
+    const uint32_t p = a.c.page.div((uint32_t)idx);
+    const int32_t id = __ldg(table + p);  // p is within the table: idx < len
+    if ((uint32_t)id < (uint32_t)a.c.n_pages) {
+      page = id;
+      row = idx - (int)(p * a.c.page.d);
+    } else if (a.err) {
+      atomicOr(a.err, PAGED_BAD_PAGE);
+    }
+  }
+};
+
+// Exponent all ones in either half of a register of T.
+template <typename T>
+__device__ __forceinline__ uint32_t nonfinite_halves(uint32_t v) {
+  constexpr uint32_t E = __is_same(T, __half) ? 0x7c00u : 0x7f80u;
+  return ((v & E) == E ? 0xffffu : 0u) | ((v >> 16 & E) == E ? 0xffff0000u : 0u);
+}
+// One arrival for the warp, after all its lanes' work.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+// Bounded wait of a whole warp: the same answer in every lane, so that a warp leaves together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A warp's fetch of ROWS consecutive positions of a tile (one K and V row of the head each): where
+// the rows are is looked up a tile ahead of the copies. With pages of a multiple of ROWS positions
+// they are evenly spaced in one page and one lookup serves all; else lane l looks row l up.
+template <int ROWS>
+struct RowFetch {
+  int64_t off;  // of row 0, or of row `lane`; -1: none
+  int left;     // rows before the sequence's end
+  __device__ __forceinline__ void look(const TreeArgs& a, const Segment& s, const int32_t* table, int idx0,
+                                       bool in_range, int lane) {
+    off = -1;
+    left = in_range ? s.len - idx0 : 0;
+    if (left <= 0) return;
+    const bool even = a.c.page.d % ROWS == 0;
+    const int idx = even ? idx0 : idx0 + lane % ROWS;
+    if (idx >= s.len) return;
+    off = paged_offset(a.c, table, a.b.table_stride, idx);
+    if (off < 0) {
+      if (a.err) atomicOr(a.err, PAGED_BAD_PAGE);
+      return;
+    }
+    off += (int64_t)s.h * a.c.head_bytes;
+  }
+  // Offset of row l (warp-collective), -1 where there is nothing to read.
+  __device__ __forceinline__ int64_t row(const TreeArgs& a, int l) const {
+    if (a.c.page.d % ROWS == 0) return off >= 0 && l < left ? off + l * a.c.row_bytes : -1;
+    return __shfl_sync(0xffffffffu, off, l);
+  }
+};
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool read) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
@@ -153,77 +278,162 @@ __device__ __forceinline__ float soft_lse(float m, float l) {
   return (sizeof(T) == 4 ? m : m * 0.69314718055994531f) + logf(l);
 }
 
-// Joins the partials of a unit: CTA (c, y) of the grid looks at the unit whose last tile CTA c of
-// the line held, if others held its earlier ones, and joins rows y * 4 + warp, + 4 * gridDim.y, ...
-// of it, a warp per row, lane l the dims l * 4 .. (float4), partial after partial.
-template <typename T, int DP, int BM, int BN>
+// Joins the partials of the units that the line was cut in. Items are spread over a grid of any
+// size: of a unit with few partials 16 rows, four a warp with all their loads in flight together; of
+// one with many a row, its partials over the four warps. Lane l of a warp holds dims 4 l .. of every
+// 128 (2 l .. of 64).
+constexpr int kJoinMany = 8, kJoinRows = 4;
+template <typename T, int DP>
+__device__ __forceinline__ void join_add(float (&acc)[DP / 32], const float* o, float f, int lane) {
+  if constexpr (DP >= 128) {
+#pragma unroll
+    for (int q = 0; q < DP / 128; ++q) {
+      const float4 v = __ldcg((const float4*)(o + q * 128 + 4 * lane));
+      acc[4 * q] += v.x * f;
+      acc[4 * q + 1] += v.y * f;
+      acc[4 * q + 2] += v.z * f;
+      acc[4 * q + 3] += v.w * f;
+    }
+  } else {
+    const float2 v = __ldcg((const float2*)(o + 2 * lane));
+    acc[0] += v.x * f;
+    acc[1] += v.y * f;
+  }
+}
+template <typename T, int DP>
+__device__ __forceinline__ void join_write(const TreeArgs& a, const JoinRec& rec, int r, const float (&acc)[DP / 32],
+                                           float l, float mx, int lane) {
+  const int R = rec.vec0 + r, i = R / a.G, row = rec.row0 + i, head = rec.head0 + (R - i * a.G), D = a.c.head_dim;
+  const bool empty = l == 0.f && !sees_any(a, row, rec.see >> 1, rec.see & 1);
+  T* out = (T*)a.out + ((int64_t)row * a.nh + head) * D;
+  constexpr int V = DP >= 128 ? 4 : 2;
+#pragma unroll
+  for (int q = 0; q < DP / 32; q += V) {
+    const int d = q / V * 32 * V + V * lane;
+    if (d >= D) continue;
+    float f[4];
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = empty ? 0.f : acc[q + e] / l;
+    if constexpr (V * sizeof(T) >= 8) {
+      store_n<T, V>(out + d, f);
+    } else {
+      out[d] = Elem<T>::put(f[0]);
+      out[d + 1] = Elem<T>::put(f[1]);
+    }
+  }
+  if (a.lse && lane == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(mx, l);
+}
+template <typename T, int DP>
 __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
-  extern __shared__ int64_t s_prefix[];
-  __shared__ int64_t scan[4];
+  extern __shared__ uint32_t s_items[];  // [ctas + 1] prefix of items
+  __shared__ uint32_t scan[4];
+  __shared__ float s_acc[3][DP];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
-  tile_prefix<BM, BN, 128>(a, s_prefix, scan, false);
-  const int64_t total = s_prefix[a.b.batch], per = tiles_per_cta(a, total);
-  const int64_t c = blockIdx.x, w = c * per, end = min(total, w + per);
-  if (w >= total) return;
-  const Segment s = segment_at<BM, BN>(a, s_prefix, w, end);
-  if (s.t0 == 0 || s.t1 != s.tiles) return;
-  const int64_t c0 = s.unit0 / per;
-  const int64_t first = c0 * per == s.unit0 ? 2 * c0 : 2 * c0 + 1;
-  const int parts = (int)(c - c0) + 1;
-  const float2* ml = (const float2*)(a.part + (int64_t)2 * a.ctas * BM * DP);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rows = min(BM, s.n * a.G - s.rt * BM);
-  const int D = a.c.head_dim;
-  for (int r = blockIdx.y * 4 + warp; r < rows; r += 4 * gridDim.y) {
-    const int R = s.rt * BM + r, i = R / a.G, row = s.row0 + i;
-    const int head = s.h * a.G + (R - i * a.G);
-    auto slot = [&](int p) { return p == 0 ? first : 2 * (c0 + p); };
-    float mx = -INFINITY;
-    for (int p = lane; p < parts; p += 32) mx = fmaxf(mx, ml[slot(p) * BM + r].x);
-    mx = warp_max(mx);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float acc[DP / 32];
+  {
+    constexpr int kMost = 8;  // CTAs on the line per thread: up to 1024
+    const int each = (a.ctas + 127) / 128, c0 = min(a.ctas, tid * each), c1 = min(a.ctas, c0 + each);
+    int2 pr[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+      pr[i] = c0 + i < c1 ? __ldcg((const int2*)&a.recs[c0 + i]) : make_int2(0, 0);  // parts, rows
+    uint32_t sum = 0, mine[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      mine[i] = sum;
+      if (pr[i].x > 0) sum += pr[i].x > kJoinMany ? pr[i].y : (pr[i].y + 4 * kJoinRows - 1) / (4 * kJoinRows);
+    }
+    uint32_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    uint32_t before = inc - sum;
+    for (int w = 0; w < warp; ++w) before += scan[w];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i)
+      if (c0 + i < c1) s_items[c0 + i] = before + mine[i];
+    if (tid == 127) s_items[a.ctas] = before + sum;
+    __syncthreads();
+  }
+  const uint32_t total = s_items[a.ctas];
+  for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
+    int lo = 0, hi = a.ctas;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_items[mid] <= item) lo = mid;
+      else hi = mid;
+    }
+    const JoinRec rec = a.recs[lo];
+    const int at = (int)(item - s_items[lo]);
+    auto slot = [&](int p, int r) { return (int64_t)(p == 0 ? rec.first_slot : 2 * (rec.cta + p)) * a.bm + r; };
+    if (rec.parts <= kJoinMany) {
+      // Lane 8 i + p: partial p of the warp's row i.
+      const int r0 = (at * 4 + warp) * kJoinRows, p = lane & 7, i = lane >> 3;
+      const bool has = p < rec.parts && r0 + i < rec.rows;
+      const float2 ml = has ? __ldcg(&a.part_ml[slot(p, r0 + i)]) : make_float2(-INFINITY, 0.f);
+      float mx = ml.x;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      const float wgt = soft_exp<T>(ml.x - (mx == -INFINITY ? 0.f : mx));
+      float l = has ? ml.y * wgt : 0.f;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      float acc[kJoinRows][DP / 32];
+#pragma unroll
+      for (int k = 0; k < kJoinRows; ++k)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[k][d] = 0.f;
+      for (int q = 0; q < rec.parts; ++q)
+#pragma unroll
+        for (int k = 0; k < kJoinRows; ++k) {
+          const float f = __shfl_sync(0xffffffffu, wgt, 8 * k + q);
+          if (r0 + k < rec.rows) join_add<T, DP>(acc[k], a.part + slot(q, r0 + k) * DP, f, lane);
+        }
+#pragma unroll
+      for (int k = 0; k < kJoinRows; ++k) {
+        const float lk = __shfl_sync(0xffffffffu, l, 8 * k), mk = __shfl_sync(0xffffffffu, mx, 8 * k);
+        if (r0 + k < rec.rows) join_write<T, DP>(a, rec, r0 + k, acc[k], lk, mk, lane);
+      }
+      continue;
+    }
+    float mx = -INFINITY, l = 0.f, acc[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) acc[d] = 0.f;
-    float l = 0.f;
-    for (int p0 = 0; p0 < parts; p0 += 32) {
+    for (int p = lane; p < rec.parts; p += 32) mx = fmaxf(mx, __ldcg(&a.part_ml[slot(p, at)]).x);
+    mx = warp_max(mx);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    for (int p0 = 0; p0 < rec.parts; p0 += 32) {
       float wgt = 0.f;
-      if (p0 + lane < parts) {
-        const float2 v = ml[slot(p0 + lane) * BM + r];
+      if (p0 + lane < rec.parts) {
+        const float2 v = __ldcg(&a.part_ml[slot(p0 + lane, at)]);
         wgt = soft_exp<T>(v.x - base);
         l += v.y * wgt;
       }
-      const int m = min(32, parts - p0);
-#pragma unroll 4
-      for (int p = 0; p < m; ++p) {
-        const float f = __shfl_sync(0xffffffffu, wgt, p);
-        const float* o = a.part + (slot(p0 + p) * BM + r) * DP;
-        if constexpr (DP >= 128) {
 #pragma unroll
-          for (int q = 0; q < DP / 128; ++q) {
-            const float4 v = __ldcg((const float4*)(o + q * 128 + 4 * lane));
-            acc[4 * q] += v.x * f;
-            acc[4 * q + 1] += v.y * f;
-            acc[4 * q + 2] += v.z * f;
-            acc[4 * q + 3] += v.w * f;
-          }
-        } else {
-          const float2 v = __ldcg((const float2*)(o + 2 * lane));
-          acc[0] += v.x * f;
-          acc[1] += v.y * f;
-        }
+      for (int k = 0; k < 8; ++k) {
+        const int p = 4 * k + warp;
+        const float f = __shfl_sync(0xffffffffu, wgt, p);
+        if (p0 + p < rec.parts) join_add<T, DP>(acc, a.part + slot(p0 + p, at) * DP, f, lane);
       }
     }
     l = warp_sum(l);
-    const bool empty = l == 0.f && !sees_any(a, row, s.n, s.ctx);
-    T* out = (T*)a.out + ((int64_t)row * a.nh + head) * D;
-    constexpr int V = DP >= 128 ? 4 : 2;
+    // The warps' shares, in order.
+    if (warp > 0)
 #pragma unroll
-    for (int q = 0; q < DP / 32; ++q) {
-      const int d = (q / V) * 32 * V + V * lane + q % V;
-      if (d < D) out[d] = Elem<T>::put(empty ? 0.f : acc[q] / l);
+      for (int q = 0; q < DP / 32; ++q) s_acc[warp - 1][q * 32 + lane] = acc[q];
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int w = 0; w < 3; ++w)
+#pragma unroll
+        for (int q = 0; q < DP / 32; ++q) acc[q] += s_acc[w][q * 32 + lane];
+      join_write<T, DP>(a, rec, at, acc, l, mx, lane);
     }
-    if (a.lse && lane == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(mx, l);
+    __syncthreads();
   }
 }
 

@@ -4,36 +4,36 @@
 
 namespace pp {
 
-template <typename K, typename... Extra>
-pp_status launch_tree(K kernel, const TreeArgs& a, int threads, size_t smem, cudaStream_t st, Extra... extra) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+template <auto kernel, typename... Extra>
+pp_status launch_tree(const TreeArgs& a, int threads, size_t smem, cudaStream_t st, Extra... extra) {
+  static bool done[64] = {};
+  // Less the static shared memory of any of the kernels.
+  if (!reserve_smem(kernel, kMaxSmem - 512, a.dev, done))
     return paged_fail(PP_E_CUDA, "cannot reserve the attention's shared memory");
   kernel<<<a.ctas, threads, smem, st>>>(a, extra...);
   return launch_status("pp_tree_attention");
 }
 
 // The join starts while the last CTAs of the attention still run and waits for them on the device.
-// Rows over gridDim.y, as far as one wave of CTAs goes.
-template <typename K>
-pp_status launch_join(K kernel, const TreeArgs& a, int bm, cudaStream_t st) {
-  int y = bm / 4;
-  while (y > 1 && (int64_t)y * a.ctas > 148 * 16) y >>= 1;
+template <typename T, int DP>
+pp_status launch_join(const TreeArgs& a, cudaStream_t st) {
+  const int items = a.ctas * a.bm;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(a.ctas, y);
+  cfg.gridDim = dim3(items < 148 * 8 ? items : 148 * 8);
   cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = 8 * (size_t)(a.b.batch + 1);
+  cfg.dynamicSmemBytes = 4 * (size_t)(a.ctas + 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, (const TreeArgs)a) != cudaSuccess)
+  if (cudaLaunchKernelEx(&cfg, pp_tree_join_kernel<T, DP>, (const TreeArgs)a) != cudaSuccess)
     return launch_status("pp_tree_attention join");
   return PP_OK;
 }
 
 // pp_tree_tc.cu
-pp_status run_tree_tc(const TreeArgs& a, uint32_t dtype, int dp, cudaStream_t st);
+pp_status run_tree_tc(const TreeArgs& a, const TreeMaps& m, uint32_t dtype, int dp, cudaStream_t st);
 
 }  // namespace pp

@@ -5,11 +5,11 @@
 //
 // One CTA, 224 threads, two CTAs on an SM (one at head_dim 256), so that one's softmax runs under
 // the other's products:
-//  * warps 4 and 5, producers: the K and V rows of every key tile, each from wherever its page is, by
-//    16-byte asynchronous copies into a ring of tile-sized slots, in the order in which the
-//    products need them (K0, K1, V0, K2, V1, ...). A slot holds 64-dim blocks of 64 rows x 128
-//    bytes, the 16-byte unit u of row r at u ^ (r & 7): read K-major it is the B operand of
-//    Q K^T, read MN-major the B operand of P V.
+//  * warp 4, producer: the K and V tiles by TMA, in boxes of 16, 32 or 64 rows of one page, into a
+//    ring of tile-sized slots, in the order in which the products need them (K0, K1, V0, K2, V1, ...).
+//    A slot holds 64-dim blocks of 64 rows x 128 bytes, the 16-byte unit u of row r at u ^ (r & 7):
+//    read K-major it is the B operand of Q K^T, read MN-major the B operand of P V. Where pages are
+//    not multiples of 16 positions, warps 4 and 5 fetch row by row with 16-byte asynchronous copies.
 //  * warp 6, one thread: S = Q K^T (128 x 64, both operands in shared memory) and O += P V (P in
 //    TMEM), each returned by a commit on an mbarrier. S of the next tile is issued as soon as the
 //    softmax has taken S of this one.
@@ -43,26 +43,24 @@ struct TcCfg {
   static constexpr int kPerSm = DP == 256 ? 1 : 2;
   static constexpr int kCols = DP == 256 ? 512 : 256;  // TMEM: O [DP], S [64], P hi [32], P lo [32]
   static constexpr int kBars = 256;
-  // Two CTAs share 228 KB less 1 KB each: with 5 slots, 1 KB is left for barriers and up to 95
+  // Two CTAs share 228 KB less 1 KB each: with 5 slots, 1 KB is left for barriers and up to 180
   // sequences' prefix; larger batches give up a slot.
-  static int slots(int batch) { return DP == 128 && batch > 88 ? 4 : kSlots; }
+  static int slots(int batch) { return DP == 128 && batch > 180 ? 4 : kSlots; }
   static size_t smem(int batch) {
-    return kQ + (size_t)slots(batch) * kItem + kBars + 8 * (size_t)(batch + 1);
+    return kQ + (size_t)slots(batch) * kItem + kBars + 4 * (size_t)(batch + 1);
   }
 };
 
 struct TcBars {
   uint64_t full[8], free[8];
   uint64_t q_full, s_full, s_free, p_full, pv_done, end;
-  int64_t scan[8];
-  uint64_t pad;
+  uint32_t scan[8];
   uint32_t tmem, dirty;
 };
 static_assert(sizeof(TcBars) <= 256, "barriers");
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
@@ -119,11 +117,6 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) 
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Bounded wait of a whole warp: the same answer in every lane, so that a warp leaves together.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
-}
-
 // 64 bits: which of the positions j0 .. j0 + 63 row i (array row `row`) sees.
 __device__ __forceinline__ uint64_t seen64(const TreeArgs& a, const Segment& s, int row, int i, int j0) {
   const int node0 = j0 - s.ctx;  // may be negative: context
@@ -148,11 +141,6 @@ __device__ __forceinline__ uint64_t seen64(const TreeArgs& a, const Segment& s, 
   return skip ? m << skip | ((1ull << skip) - 1) : m;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t tc_nonfinite(uint32_t v) {
-  constexpr uint32_t E = __is_same(T, __half) ? 0x7c00u : 0x7f80u;
-  return ((v & E) == E ? 0xffffu : 0u) | ((v >> 16 & E) == E ? 0xffff0000u : 0u);
-}
 __device__ __forceinline__ uint32_t tc_pack(float a, float b, __nv_bfloat16*) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *(const uint32_t*)&v;
@@ -165,30 +153,31 @@ __device__ __forceinline__ float2 tc_unpack(uint32_t v, __nv_bfloat16*) { return
 __device__ __forceinline__ float2 tc_unpack(uint32_t v, __half*) { return __half22float2(*(const __half2*)&v); }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kernel(const TreeArgs a, const int slots) {
+__global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kernel(const TreeArgs a, const __grid_constant__ TreeMaps maps, const int slots) {
   using C = TcCfg<DP>;
   constexpr int BM = kTcBM, BN = kTcBN, UR = DP / 8;
   extern __shared__ __align__(1024) uint8_t sm[];
   uint8_t* qs = sm;
   uint8_t* ring = sm + C::kQ;
   TcBars* bars = (TcBars*)(ring + (size_t)slots * C::kItem);
-  int64_t* prefix = (int64_t*)((uint8_t*)bars + C::kBars);
+  uint32_t* prefix = (uint32_t*)((uint8_t*)bars + C::kBars);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int D = a.c.head_dim;
-  if (smem_u32(sm) & 1023u) {  // the swizzle counts from 1024-byte boundaries
+  if (smem_u32(sm) & 1023u) {  // cannot be (nothing is static): no join, and the caller is told
+    if (tid == 0) write_join<BM>(a, nullptr, 1);
     if (tid == 0 && a.err) atomicOr(a.err, PAGED_TIMEOUT);
     return;
   }
 
   if (tid == 0) {
     for (int i = 0; i < slots; ++i) {
-      mbar_init(&bars->full[i], 64);
+      mbar_init(&bars->full[i], maps.box ? 1 : 2);
       mbar_init(&bars->free[i], 1);
     }
-    mbar_init(&bars->q_full, 128);
+    mbar_init(&bars->q_full, 4);
     mbar_init(&bars->s_full, 1);
-    mbar_init(&bars->s_free, 128);
-    mbar_init(&bars->p_full, 128);
+    mbar_init(&bars->s_free, 4);
+    mbar_init(&bars->p_full, 4);
     mbar_init(&bars->pv_done, 1);
     mbar_init(&bars->end, 1);
     bars->dirty = 0;
@@ -205,33 +194,64 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
   const uint32_t tO = tmem, tS = tmem + DP, tP = tmem + DP + 64;
-  const int64_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
-  const int64_t begin = blockIdx.x * per, end = min(total, begin + per);
+  const uint32_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
+  uint32_t begin, end;
+  cta_range(per, total, blockIdx.x, begin, end);
   bool ok = true;
 
-  if (warp == 4 || warp == 5) {
+  if (warp == 4 && maps.box) {
+    // ---- producer, by TMA: lane (g, b) of a tile its row group g and 64-dim block b
+    constexpr int NB = DP / 64;
+    const int boxes = BN / maps.box * NB, grp = lane / NB, blk = lane % NB;
+    int n = 0;
+    for (uint32_t w = begin; w < end && ok;) {
+      const Segment s = segment_at<BM, BN>(a, prefix, w, end);
+      const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
+      const int cnt = s.t1 - s.t0;
+      // Places of tile i (V's turn), i + 1 (K's) and i + 2, looked up ahead of their copies.
+      BoxPlace prev, cur, next;
+      auto look = [&](BoxPlace& f, int i) { f.look(a, s, table, (s.t0 + i) * BN + grp * maps.box, i < cnt && lane < boxes); };
+      look(cur, 0);
+      look(next, 1);
+      prev = cur;
+      for (int j = 0; j < 2 * cnt; ++j, ++n) {
+        const bool isv = j == 2 * cnt - 1 || (j > 0 && !(j & 1));
+        const int slot = n % slots;
+        if (n >= slots && !warp_wait(&bars->free[slot], (uint32_t)(n / slots - 1) & 1u)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], C::kItem);
+        __syncwarp();
+        if (lane < boxes)
+          tma_box(ring + (size_t)slot * C::kItem + blk * (BN * 128) + grp * maps.box * 128, isv ? &maps.v : &maps.k,
+                  &bars->full[slot], maps, 64 * blk, s.h, isv ? prev.row : cur.row, isv ? prev.page : cur.page);
+        if (j == 0 || isv) {
+          prev = cur;
+          cur = next;
+          look(next, j / 2 + 2);
+        }
+      }
+      w += s.step;
+    }
+    if (!ok)  // let the copies in flight land
+      for (int i = n > slots ? n - slots : 0; i < n; ++i) warp_wait(&bars->full[i % slots], (uint32_t)(i / slots) & 1u);
+  } else if ((warp == 4 || warp == 5) && !maps.box) {
     // ---- producers: warp pw the rows 32 pw .. + 31 of every tile
     const int pw = warp - 4;
     constexpr int RPP = 32 / UR;  // rows of one pass of a warp
     const int u = lane % UR, sub = lane / UR;
     int n = 0;
-    for (int64_t w = begin; w < end && ok;) {
+    for (uint32_t w = begin; w < end && ok;) {
       const Segment s = segment_at<BM, BN>(a, prefix, w, end);
       const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
       const int cnt = s.t1 - s.t0;
-      // Lane l looks the tile's row l of the warp up, a tile ahead of its copies.
-      auto look = [&](int i) -> int64_t {
-        const int idx = (s.t0 + i) * BN + pw * 32 + lane;
-        if (i >= cnt || idx >= s.len) return -1;
-        const int64_t off = paged_offset(a.c, table, a.b.table_stride, idx);
-        if (off < 0) {
-          if (a.err) atomicOr(a.err, PAGED_BAD_PAGE);
-          return -1;
-        }
-        return off + (int64_t)s.h * a.c.head_bytes;
-      };
-      // Rows of tile i (V's turn), i + 1 (K's) and i + 2.
-      int64_t prev = -1, cur = look(0), next = look(1);
+      // Rows of tile i (V's turn), i + 1 (K's) and i + 2, looked up ahead of their copies.
+      RowFetch<32> prev, cur, next;
+      auto look = [&](RowFetch<32>& f, int i) { f.look(a, s, table, (s.t0 + i) * BN + pw * 32, i < cnt, lane); };
+      look(cur, 0);
+      look(next, 1);
+      prev = cur;
       for (int j = 0; j < 2 * cnt; ++j, ++n) {
         const bool isv = j == 2 * cnt - 1 || (j > 0 && !(j & 1));
         const int slot = n % slots;
@@ -241,11 +261,10 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         }
         uint8_t* dst = ring + (size_t)slot * C::kItem;
         const uint8_t* base = isv ? a.c.v : a.c.k;
-        const int64_t mine = isv ? prev : cur;
 #pragma unroll
         for (int q = 0; q < 32 / RPP; ++q) {
           const int l = q * RPP + sub, r = pw * 32 + l;
-          const int64_t off = __shfl_sync(0xffffffffu, mine, l);
+          const int64_t off = isv ? prev.row(a, l) : cur.row(a, l);
           const bool read = off >= 0 && 8 * u < D;
           cp_async16(dst + (u >> 3) * (BN * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4), base + (read ? off + 16 * u : 0), read);
         }
@@ -253,19 +272,19 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         if (j == 0 || isv) {
           prev = cur;
           cur = next;
-          next = look(j / 2 + 2);
+          look(next, j / 2 + 2);
         }
         if (n >= kTcLag) {
           cp_async_wait<kTcLag>();
           fence_async();
-          mbar_arrive(&bars->full[(n - kTcLag) % slots]);
+          warp_arrive(&bars->full[(n - kTcLag) % slots], lane);
         }
       }
-      w += cnt;
+      w += s.step;
     }
     cp_async_wait<0>();
     fence_async();
-    for (int i = n > kTcLag ? n - kTcLag : 0; i < n; ++i) mbar_arrive(&bars->full[i % slots]);
+    for (int i = n > kTcLag ? n - kTcLag : 0; i < n; ++i) warp_arrive(&bars->full[i % slots], lane);
   } else if (warp == 6) {
     // ---- products
     if (lane == 0) {
@@ -284,7 +303,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         tc_commit(&bars->s_full);
         ++n;
       };
-      for (int64_t w = begin; w < end && ok;) {
+      for (uint32_t w = begin; w < end && ok;) {
         const Segment s = segment_at<BM, BN>(a, prefix, w, end);
         const int cnt = s.t1 - s.t0;
         ok = mbar_wait(&bars->q_full, (uint32_t)seg & 1u) && take() && (g == 0 || mbar_wait(&bars->s_free, (uint32_t)(g - 1) & 1u));
@@ -313,20 +332,25 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           ++n;
         }
         ++seg;
-        w += cnt;
+        w += s.step;
       }
       tc_commit(&bars->end);
       mbar_wait(&bars->end, 0);  // no product of this CTA runs when TMEM is freed
     }
-  } else {
+  } else if (warp < 4) {
     // ---- softmax
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const float sc = soft_scale<T>(a.scale);
+    // The maximum is taken before the scale, so the scale must be positive: its sign goes into Q, and
+    // a scale of zero makes Q zero.
+    const float sc = a.scale == 0.f ? 1.f : soft_scale<T>(fabsf(a.scale));
+    const uint32_t keep = a.scale == 0.f ? 0u : ~0u, flip = a.scale < 0.f ? 0x80008000u : 0u;
     int n0 = 0, g = 0;  // items before this segment, tiles so far
     uint32_t seg = 0;
-    for (int64_t w = begin; w < end && ok;) {
+    if (begin >= end && tid == 0) write_join<BM>(a, nullptr, per);
+    for (uint32_t w = begin; w < end && ok;) {
       const Segment s = segment_at<BM, BN>(a, prefix, w, end);
       const int cnt = s.t1 - s.t0, NR = s.n * a.G;
+      if (w == begin && tid == 0) write_join<BM>(a, &s, per);
       // The previous segment's products with Q are complete (its last S was taken).
       for (int e = tid; e < BM * UR; e += 128) {
         const int r = e / UR, u = e % UR, R = s.rt * BM + r;
@@ -334,11 +358,12 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         if (R < NR && 8 * u < D) {
           const int i = R / a.G;
           v = *(const uint4*)((const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(s.h * a.G + R - i * a.G) * D + 8 * u);
+          v = make_uint4((v.x & keep) ^ flip, (v.y & keep) ^ flip, (v.z & keep) ^ flip, (v.w & keep) ^ flip);
         }
         *(uint4*)(qs + (u >> 3) * (BM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = v;
       }
       fence_async();
-      mbar_arrive(&bars->q_full);
+      warp_arrive(&bars->q_full, lane);
 
       const int R = s.rt * BM + tid, i = R / a.G, row = s.row0 + i;
       float m = -INFINITY, l = 0.f;
@@ -353,7 +378,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         tc_ld32(tS + lanes + 32, x[1]);
         tc_wait_ld();
         tc_fence_before();
-        mbar_arrive(&bars->s_free);
+        warp_arrive(&bars->s_free, lane);
         const int j0 = (s.t0 + t) * BN;
         const bool tree = j0 + BN > s.ctx;
         if (tree) {
@@ -362,10 +387,10 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           for (int k = 0; k < 64; ++k)
             if (!(see >> k & 1u)) x[k >> 5][k & 31] = -INFINITY;
         }
-        float mx = -INFINITY;
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int k = 0; k < 64; ++k) mx = fmaxf(mx, x[k >> 5][k & 31]);
-        mx *= sc;  // scale > 0
+        for (int k = 0; k < 64; ++k) top[k & 3] = fmaxf(top[k & 3], x[k >> 5][k & 31]);
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;  // scale > 0
         const bool grown = mx > m + 8.f || (m == -INFINITY && mx > m);
         float alpha = 1.f;
         const bool rescale = __any_sync(0xffffffffu, grown);
@@ -384,10 +409,12 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           sum[k & 3] += v;
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (tree && (a.mask || s.n > 1)) {
-          // A V that some row is blind to must not count even where it is not finite (0 * NaN):
-          // such values leave the tile here and come back, for the rows that see them, with the
-          // output. The slot stays until this tile's product, which waits for p_full.
+        const bool blind = tree && (a.mask || s.n > 1);
+        if (blind || j0 + BN > s.len) {
+          // Positions past the end hold whatever their page did: zeros there. And a V that some row
+          // is blind to must not count even where it is not finite (0 * NaN): such values leave the
+          // tile here and come back, for the rows that see them, with the output. The slot stays
+          // until this tile's product, which waits for p_full.
           const int item = n0 + (t == cnt - 1 ? 2 * cnt - 1 : 2 * t + 2), slot = item % slots;
           if (!warp_wait(&bars->full[slot], (uint32_t)(item / slots) & 1u)) {
             ok = false;
@@ -396,11 +423,15 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           uint32_t found = 0;
           for (int e = tid; e < BN * UR; e += 128) {
             uint4* p = (uint4*)(ring + (size_t)slot * C::kItem + e * 16);
-            uint4 v = *p;
-            const uint32_t b0 = tc_nonfinite<T>(v.x), b1 = tc_nonfinite<T>(v.y), b2 = tc_nonfinite<T>(v.z), b3 = tc_nonfinite<T>(v.w);
-            if (b0 | b1 | b2 | b3) {
-              found = 1;
-              *p = make_uint4(v.x & ~b0, v.y & ~b1, v.z & ~b2, v.w & ~b3);
+            if (j0 + ((e >> 3) & (BN - 1)) >= s.len) {
+              *p = make_uint4(0u, 0u, 0u, 0u);
+            } else if (blind) {
+              const uint4 v = *p;
+              const uint32_t b0 = nonfinite_halves<T>(v.x), b1 = nonfinite_halves<T>(v.y), b2 = nonfinite_halves<T>(v.z), b3 = nonfinite_halves<T>(v.w);
+              if (b0 | b1 | b2 | b3) {
+                found = 1;
+                *p = make_uint4(v.x & ~b0, v.y & ~b1, v.z & ~b2, v.w & ~b3);
+              }
             }
           }
           if (found) bars->dirty = seg + 1;
@@ -438,7 +469,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         tc_st32(tP + lanes + 32, p);
         tc_wait_st();
         tc_fence_before();
-        mbar_arrive(&bars->p_full);
+        warp_arrive(&bars->p_full, lane);
       }
       if (!ok || !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
         ok = false;
@@ -473,7 +504,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               if (c + 2 * k >= D) break;
-              const uint32_t v = src[k], bad = tc_nonfinite<T>(v);
+              const uint32_t v = src[k], bad = nonfinite_halves<T>(v);
               const float2 f = tc_unpack(v, (T*)nullptr);
               if (bad & 1u) o[2 * k] += f.x;
               if (bad >> 16) o[2 * k + 1] += f.y;
@@ -496,11 +527,11 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         }
       }
       if (live && whole && a.lse) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(m, l);
-      if (live && !whole) ((float2*)(a.part + (int64_t)2 * a.ctas * BM * DP))[slot * BM + tid] = make_float2(m, l);
+      if (live && !whole) a.part_ml[slot * BM + tid] = make_float2(m, l);
       tc_fence_before();  // O may be overwritten after the next p_full
       ++seg;
       n0 += 2 * cnt;
-      w += cnt;
+      w += s.step;
     }
   }
   if (!ok && a.err) atomicOr(a.err, PAGED_TIMEOUT);
@@ -513,21 +544,21 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
 }
 
 template <typename T, int DP>
-static pp_status run_tc(const TreeArgs& a, cudaStream_t st) {
+static pp_status run_tc(const TreeArgs& a, const TreeMaps& m, cudaStream_t st) {
   using C = TcCfg<DP>;
   const int B = a.b.batch;
-  const pp_status r = launch_tree(pp_tree_tc_kernel<T, DP>, a, kTcThreads, C::smem(B), st, C::slots(B));
-  if (r != PP_OK || a.ctas == 1) return r;
-  return launch_join(pp_tree_join_kernel<T, DP, kTcBM, kTcBN>, a, kTcBM, st);
+  const pp_status r = launch_tree<pp_tree_tc_kernel<T, DP>>(a, kTcThreads, C::smem(B), st, m, C::slots(B));
+  if (r != PP_OK || a.whole) return r;
+  return launch_join<T, DP>(a, st);
 }
 template <typename T>
-static pp_status run_tc_dim(const TreeArgs& a, int dp, cudaStream_t st) {
-  if (dp == 64) return run_tc<T, 64>(a, st);
-  if (dp == 128) return run_tc<T, 128>(a, st);
-  return run_tc<T, 256>(a, st);
+static pp_status run_tc_dim(const TreeArgs& a, const TreeMaps& m, int dp, cudaStream_t st) {
+  if (dp == 64) return run_tc<T, 64>(a, m, st);
+  if (dp == 128) return run_tc<T, 128>(a, m, st);
+  return run_tc<T, 256>(a, m, st);
 }
-pp_status run_tree_tc(const TreeArgs& a, uint32_t dtype, int dp, cudaStream_t st) {
-  return dtype == PP_BF16 ? run_tc_dim<__nv_bfloat16>(a, dp, st) : run_tc_dim<__half>(a, dp, st);
+pp_status run_tree_tc(const TreeArgs& a, const TreeMaps& m, uint32_t dtype, int dp, cudaStream_t st) {
+  return dtype == PP_BF16 ? run_tc_dim<__nv_bfloat16>(a, m, dp, st) : run_tc_dim<__half>(a, m, dp, st);
 }
 
 }  // namespace pp
