@@ -438,7 +438,7 @@ extern "C" pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t 
   const size_t smem = base + (a.staged ? warps * copy : 0);
   static bool done[64] = {};
   if (!reserve_smem(pp_beam_merge_kernel, (int)kMergeSmem, cuda_device, done))
-    return paged_fail(PP_E_CUDA, "cannot reserve the merge's shared memory");
+    return PP_E_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(groups);
   cfg.blockDim = dim3(32 * warps);

@@ -63,7 +63,13 @@ template <typename K>
 inline bool reserve_smem(K kernel, int bytes, int dev, bool (&done)[64]) noexcept {
   if (dev < 0 || dev >= 64) return false;
   if (!done[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) {
+      char msg[160];
+      snprintf(msg, sizeof msg, "cannot reserve a kernel's shared memory: %s", cudaGetErrorString(e));
+      paged_fail(PP_E_CUDA, msg);
+      return false;
+    }
     done[dev] = true;
   }
   return true;

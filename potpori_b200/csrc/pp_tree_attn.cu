@@ -65,7 +65,7 @@ template <int DP>
 __device__ __forceinline__ void narrow_copy(const TreeArgs& a, const RowFetch<16>& f, uint8_t* kd, int lane) {
   constexpr int UR = DP / 8, RP = 32 / UR;
   const int u = lane % UR, sub = lane / UR;
-#pragma unroll
+#pragma unroll 4
   for (int i = 0; i < 16 / RP; ++i) {
     const int l = i * RP + sub;
     const int64_t off = f.row(a, l);
@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
     pp_tree_narrow_kernel(const TreeArgs a, const __grid_constant__ TreeMaps maps) {
   using C = NarrowCfg<DP>;
   constexpr int BM = 8, BN = kTreeBN, NS = C::NS, KS = DP / 16, NB = DP / 64;
-  extern __shared__ __align__(1024) uint8_t sm[];
+  extern __shared__ __align__(1024) uint8_t narrow_smem[];
+  uint8_t* sm = narrow_smem;
   uint64_t* full = (uint64_t*)(sm + C::kRing);  // [4][NS]
   uint32_t* scan = (uint32_t*)(full + 4 * NS);
   uint32_t* prefix = scan + 4;
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
   uint32_t begin, end;
   cta_range(per, total, blockIdx.x, begin, end);
   if (begin >= end && tid == 0) write_join<BM>(a, nullptr, per);
-  uint32_t n = 0;  // tiles that the warp has taken through its ring
+  RingCursor use;  // the stage of the next tile to consume
   bool ok = true;
 
   for (uint32_t w = begin; w < end;) {
@@ -125,86 +126,80 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
     const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
     RowFetch<16> rows;
     BoxPlace box;
+    // Where tile t's rows are, a tile ahead of their copies.
     auto look = [&](int t) {
       const int idx = t * BN + warp * 16;
       if (tma) box.look(a, s, table, idx, t < s.t1);
       else rows.look(a, s, table, idx, t < s.t1, lane);
     };
-    // Tile t, whose place was looked up, into its stage. A stage that ordinary loads have read is
-    // handed to the copy engine by the proxy fence.
-    auto fetch = [&](int t) {
-      const uint32_t stage = (n + (uint32_t)(t - s.t0)) % NS;
-      if (tma) {
-        if (t < s.t1) {
-          if (lane == 0) {
-            fence_async();
-            mbar_arrive_expect_tx(&bar[stage], C::kStage);
-          }
-          __syncwarp();
-          if (lane < 2 * NB)
-            tma_box(ring + stage * C::kStage + lane * 2048, lane < NB ? &maps.k : &maps.v, &bar[stage], maps,
-                    64 * (lane % NB), s.h, box.row, box.page);
-        }
-      } else {
-        if (t < s.t1) narrow_copy<DP>(a, rows, ring + stage * C::kStage, lane);
-        cp_async_commit();
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i) {
-      look(s.t0 + i);
-      fetch(s.t0 + i);
-    }
-    look(s.t0 + NS - 1);
+    look(s.t0);
     // Q^T fragments: vector g4, dims 16 ks + 2 t4 and + 8.
     uint32_t qb[KS][2];
     {
-      const int R = s.rt * BM + g4, i = R / a.G;
+      const int R = s.rt * BM + g4, i = (int)a.by_g.div((uint32_t)R);
       const bool in = R < s.n * a.G;
-      const T* q = (const T*)a.q + (int64_t)(s.row0 + (in ? i : 0)) * a.q_stride + (int64_t)(s.h * a.G + (in ? R - i * a.G : 0)) * D;
+      const T* q = (const T*)a.q + (int64_t)(s.row0 + (in ? i : 0)) * a.q_stride + (int64_t)(s.h * a.G + (in ? R - i * a.G : 0)) * D + 2 * t4;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = 16 * ks + 8 * e + 2 * t4;
-          qb[ks][e] = in && d < D ? *(const uint32_t*)(q + d) : 0u;
-        }
+        for (int e = 0; e < 2; ++e)
+          qb[ks][e] = in && 16 * ks + 8 * e < D ? *(const uint32_t*)(q + 16 * ks + 8 * e) : 0u;
     }
     // The thread's two vectors: 2 t4 and 2 t4 + 1.
-    const int i0 = (s.rt * BM + 2 * t4) / a.G, i1 = (s.rt * BM + 2 * t4 + 1) / a.G;
+    const int i0 = (int)a.by_g.div((uint32_t)(s.rt * BM + 2 * t4)), i1 = (int)a.by_g.div((uint32_t)(s.rt * BM + 2 * t4 + 1));
     float o[KS][4];
 #pragma unroll
     for (int k = 0; k < KS; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     // ldmatrix rows of the lane: K as [16 keys][16 dims], V the same, transposed.
     const int kr = lane & 15, ku = lane >> 4, vr = (lane & 7) + ((lane >> 4) << 3), vu = (lane >> 3) & 1;
+    uint32_t found = 0;  // non-finite values of V were taken out of the products
 
-    for (int t = s.t0; t < s.t1; ++t) {
-      const uint32_t at = n + (uint32_t)(t - s.t0), stage = at % NS;
-      if (tma) {
-        if (!warp_wait(&bar[stage], at / NS & 1u)) {
-          ok = false;
-          // Let the copies in flight land before the shared memory is released.
-          for (int q = t + 1; q < s.t1 && q < t + NS - 1; ++q) {
-            const uint32_t k = n + (uint32_t)(q - s.t0);
-            warp_wait(&bar[k % NS], k / NS & 1u);
+    uint32_t into = use.slot;  // the stage that the next fetched tile takes
+    for (int t = s.t0 - (NS - 1); t < s.t1; ++t) {
+      if (t >= s.t0) {
+        if (tma) {
+          if (!warp_wait(&bar[use.slot], use.phase)) {
+            ok = false;
+            break;
           }
-          break;
+        } else {
+          cp_async_wait<NS - 2>();
         }
-      } else {
-        cp_async_wait<NS - 2>();
       }
       __syncwarp();
-      fetch(t + NS - 1);
-      look(t + NS);
-      const uint8_t* kt = ring + stage * C::kStage;
-      uint8_t* vt = ring + stage * C::kStage + C::kTile;
+      // Tile t + NS - 1 into the stage that tile t - 1 has left. A stage that ordinary loads have read
+      // is handed to the copy engine by the proxy fence.
+      const bool more = t + NS - 1 < s.t1;
+      if (tma) {
+        if (more) {
+          if (elect_one()) {
+            fence_async();
+            mbar_arrive_expect_tx(&bar[into], C::kStage);
+#pragma unroll
+            for (int i = 0; i < 2 * NB; ++i)
+              tma_box(ring + into * C::kStage + i * 2048, i < NB ? &maps.k : &maps.v, &bar[into], maps, 64 * (i % NB),
+                      s.h, box.row, box.page);
+          }
+          __syncwarp();
+        }
+      } else {
+        if (more) narrow_copy<DP>(a, rows, ring + into * C::kStage, lane);
+        cp_async_commit();
+      }
+      if (more) {
+        into = into + 1 == NS ? 0 : into + 1;
+        look(t + NS);
+      }
+      if (t < s.t0) continue;
+      const uint8_t* kt = ring + use.slot * C::kStage;
+      uint8_t* vt = ring + use.slot * C::kStage + C::kTile;
       const int j0 = t * BN + warp * 16;
+      use.next(NS);
 
       float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};  // even and odd k steps
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        if (16 * ks >= D) break;
+      for (int ks = 0; ks < KS; ++ks) {  // dims past the head's are zero in Q
         uint32_t kf[4];
         ldmatrix_x4a(kf, kt + narrow_unit(kr, 2 * ks + ku));
         mma16<T>(ks & 1 ? y : x, kf, qb[ks][0], qb[ks][1]);
@@ -212,9 +207,10 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
       // Element e: key g4 + 8 (e >> 1), vector 2 t4 + (e & 1).
       const bool tree = j0 + 16 > s.ctx;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = (x[e] + y[e]) * sc;
-        if (tree) {
+      for (int e = 0; e < 4; ++e) x[e] = (x[e] + y[e]) * sc;
+      if (tree) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
           const int node = j0 + g4 + 8 * (e >> 1) - s.ctx, i = e & 1 ? i1 : i0;
           if (node >= 0 && (node >= s.n || i >= s.n || !sees_node(a, s.row0 + i, i, node))) x[e] = -INFINITY;
         }
@@ -249,22 +245,25 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
         l[e & 1] += x[e];
       }
       // Positions past the end hold whatever their page did: zeros there. And a V that some row is
-      // blind to must not count even where it is not finite (0 * NaN): then its halves are cleared as
-      // the product reads them, and added below for the rows that see them.
-      bool dirty = false;
+      // blind to must not count even where it is not finite (0 * NaN): such values leave the tile
+      // here and come back, for the rows that see them, with the output.
       const bool blind = tree && (a.mask || s.n > 1);
       if (blind || j0 + 16 > s.len) {
-        uint32_t found = 0;
+#pragma unroll 1
         for (int e = lane; e < 16 * (DP / 8); e += 32) {
           uint4* p = (uint4*)(vt + e * 16);
-          if (j0 + ((e >> 3) & 15) >= s.len) {
-            *p = make_uint4(0u, 0u, 0u, 0u);
-          } else if (blind) {
-            const uint4 v = *p;
-            found |= nonfinite_halves<T>(v.x) | nonfinite_halves<T>(v.y) | nonfinite_halves<T>(v.z) | nonfinite_halves<T>(v.w);
+          uint4 v = *p;
+          uint32_t bad[4] = {~0u, ~0u, ~0u, ~0u};
+          if (j0 + ((e >> 3) & 15) < s.len) {
+            bad[0] = nonfinite_halves<T>(v.x);
+            bad[1] = nonfinite_halves<T>(v.y);
+            bad[2] = nonfinite_halves<T>(v.z);
+            bad[3] = nonfinite_halves<T>(v.w);
+            if (!blind || !(bad[0] | bad[1] | bad[2] | bad[3])) continue;
+            found = 1;
           }
+          *p = make_uint4(v.x & ~bad[0], v.y & ~bad[1], v.z & ~bad[2], v.w & ~bad[3]);
         }
-        dirty = __any_sync(0xffffffffu, found != 0);  // and the zeros are seen by every lane
         __syncwarp();
       }
       // P is carried as hi + lo parts: rounded to T alone it would add as much error as the rounding
@@ -279,40 +278,14 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
       }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        if (16 * k >= D) break;
         uint32_t vf[4];
         ldmatrix_x4_trans(vf, vt + narrow_unit(vr, 2 * k + vu));
-        if (dirty) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vf[e] &= ~nonfinite_halves<T>(vf[e]);
-        }
         mma16<T>(o[k], vf, ph[0], ph[1]);
         mma16<T>(o[k], vf, pl[0], pl[1]);
       }
-      if (dirty) {  // the non-finite values of V, for the vectors that see them
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh)
-          for (int k8 = 0; k8 < 8; ++k8) {
-            const float p0 = __shfl_sync(0xffffffffu, x[2 * kh], k8 * 4 + t4);
-            const float p1 = __shfl_sync(0xffffffffu, x[2 * kh + 1], k8 * 4 + t4);
-            const int r = 8 * kh + k8, node = j0 + r - s.ctx;
-            if (node >= s.n) continue;
-            const bool see0 = node < 0 || (i0 < s.n && sees_node(a, s.row0 + i0, i0, node));
-            const bool see1 = node < 0 || (i1 < s.n && sees_node(a, s.row0 + i1, i1, node));
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-              for (int dh = 0; dh < 2; ++dh) {
-                const float f = Elem<T>::get(*(const T*)(vt + narrow_unit(r, 2 * k + dh) + 2 * g4));
-                if (isfinite(f)) continue;
-                if (see0) o[k][2 * dh] += p0 * f;
-                if (see1) o[k][2 * dh + 1] += p1 * f;
-              }
-          }
-      }
     }
-    n += (uint32_t)(s.t1 - s.t0);
     if (!tma) cp_async_wait<0>();
+    const bool dirty = __syncthreads_or(found != 0);
     if (__syncthreads_or(!ok)) break;  // else the rings are free
 #pragma unroll
     for (int q = 0; q < 2; ++q)
@@ -334,8 +307,14 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
     const bool whole = s.t0 == 0 && s.t1 == s.tiles;
     const int64_t slot = 2 * (int64_t)blockIdx.x + (w == begin ? 0 : 1);
     const int live = min(BM, s.n * a.G - s.rt * BM);
+    if (dirty) {
+      add_nonfinite<T>(a, s, live, max(s.ctx, s.t0 * BN), min(s.len, s.t1 * BN), tid, kTreeThreads,
+                       [&](int r, int d) -> float& { return os[r * C::kOPitch + d]; });
+      __syncthreads();
+    }
+#pragma unroll 1
     for (int e = tid; e < live * (DP / 8); e += kTreeThreads) {
-      const int r = e / (DP / 8), u = e % (DP / 8), R = s.rt * BM + r, i = R / a.G;
+      const int r = e / (DP / 8), u = e % (DP / 8), R = s.rt * BM + r, i = (int)a.by_g.div((uint32_t)R);
       float top = ml[r].x;
 #pragma unroll
       for (int k = 1; k < 4; ++k) top = fmaxf(top, ml[k * BM + r].x);
@@ -353,8 +332,9 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
       if (whole) {
         const int row = s.row0 + i, head = s.h * a.G + R - i * a.G;
         const bool empty = sum == 0.f && !sees_any(a, row, s.n, s.ctx);
+        const float inv = 1.f / sum;
 #pragma unroll
-        for (int d = 0; d < 8; ++d) f[d] = empty ? 0.f : f[d] / sum;
+        for (int d = 0; d < 8; ++d) f[d] = empty ? 0.f : f[d] * inv;
         if (8 * u < D) store8((T*)a.out + ((int64_t)row * a.nh + head) * D + 8 * u, f);
         if (a.lse && u == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(top, sum);
       } else {
@@ -366,7 +346,12 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
     __syncthreads();
     w += s.step;
   }
-  if (!ok && lane == 0 && a.err) atomicOr(a.err, PAGED_TIMEOUT);
+  if (!ok) {
+    // Let the copies in flight land before the shared memory is released: at most one a stage.
+    if (tma)
+      for (int i = 0; i < NS; ++i) warp_wait(&bar[use.slot], use.phase), use.next(NS);
+    if (lane == 0 && a.err) atomicOr(a.err, PAGED_TIMEOUT);
+  }
 }
 
 // ---- F32 caches ----------------------------------------------------------------------------
@@ -383,7 +368,7 @@ struct TreeFCfg {
   static constexpr int kQ = BM * P * 4, kP = kTreeFBN * PP * 4, kRows = 2 * BM * 4;
   static constexpr int kPerSm = DP <= 64 ? 5 : DP <= 128 ? 3 : 1;
   static constexpr size_t smem(int batch) {
-    return kTreeFStages * kStage + kQ + kP + kRows + 4 * (size_t)(batch + 1);
+    return kTreeFStages * kStage + kQ + kP + kRows + 16 + 4 * (size_t)(batch + 1);
   }
 };
 
@@ -392,14 +377,15 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
   using C = TreeFCfg<DP, BM>;
   constexpr int BN = kTreeFBN, NS = kTreeFStages, P = C::P, PP = C::PP, UR = DP / 4, RW = BM / 4;
   constexpr int DT = DP <= 128 ? 1 : DP / 128;  // dims of a thread: tid, tid + 128
-  extern __shared__ __align__(128) uint8_t sm[];
+  extern __shared__ __align__(128) uint8_t f32_smem[];
+  uint8_t* sm = f32_smem;
   uint8_t* ring = sm;
   float* qs = (float*)(sm + NS * C::kStage);
   float* pt = qs + BM * P;  // [key][PP]
   float* al_s = pt + BN * PP;
   uint32_t* vis_s = (uint32_t*)(al_s + BM);
-  uint32_t* prefix = vis_s + BM;
-  __shared__ uint32_t scan[4];
+  uint32_t* scan = vis_s + BM;
+  uint32_t* prefix = scan + 4;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.c.head_dim;
 
   pdl_launch_dependents();
@@ -418,7 +404,7 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
     auto look = [&](int t) { ahead.look(a, s, table, t * BN + warp * 8, t < s.t1, lane); };
     auto fetch = [&](int stage) {
       uint8_t* kd = ring + stage * C::kStage;
-#pragma unroll
+#pragma unroll 4
       for (int i = 0; i < 8 * UR / 32; ++i) {
         const int e = lane + 32 * i, l = e / UR, u = e % UR, r = warp * 8 + l;
         const int64_t off = ahead.row(a, l);
@@ -432,11 +418,12 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
     fetch(0);
     cp_async_commit();
     look(s.t0 + 1);
+#pragma unroll 2
     for (int e = tid; e < BM * UR; e += kTreeThreads) {
       const int r = e / UR, u = e % UR, R = s.rt * BM + r;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       if (R < NR && 4 * u < D) {
-        const int i = R / a.G;
+        const int i = (int)a.by_g.div((uint32_t)R);
         v = *(const float4*)((const float*)a.q + (int64_t)(s.row0 + i) * a.q_stride +
                              (int64_t)(s.h * a.G + R - i * a.G) * D + 4 * u);
       }
@@ -487,7 +474,7 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
       for (int r = 0; r < RW; ++r) {
         bool see = true;
         if (tree && node >= 0) {
-          const int i = (s.rt * BM + warp * RW + r) / a.G;
+          const int i = (int)a.by_g.div((uint32_t)(s.rt * BM + warp * RW + r));
           see = node < s.n && i < s.n && sees_node(a, s.row0 + i, i, node);
         }
         v[r] = see ? (x[r][0] + x[r][1]) * a.scale : -INFINITY;
@@ -521,18 +508,22 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
         if (dim >= D) break;
 #pragma unroll
         for (int r = 0; r < BM; ++r) acc[d][r] *= al_s[r];
+        // A V that a row does not see must not count for it even where it is not finite (0 * NaN):
+        // such a value is added for the rows that see it and leaves the tile.
+        if (tree)
+#pragma unroll 1
+          for (int k = 0; k < BN; ++k) {
+            float* at = (float*)vt + k * P + dim;
+            const float odd = *at;
+            if (isfinite(odd)) continue;
+#pragma unroll
+            for (int r = 0; r < BM; ++r)
+              if (vis_s[r] >> k & 1u) acc[d][r] += pt[k * PP + r] * odd;
+            *at = 0.f;
+          }
 #pragma unroll 8
         for (int k = 0; k < BN; ++k) {
           const float v1 = vt[k * P + dim];
-          if (tree && !isfinite(v1)) {  // it must not count for the rows that do not see it (0 * NaN)
-            for (int r = 0; r < BM; ++r) {
-              const float add = vis_s[r] >> k & 1u ? pt[k * PP + r] * v1 : 0.f;
-#pragma unroll
-              for (int q = 0; q < BM; ++q)
-                if (q == r) acc[d][q] += add;
-            }
-            continue;
-          }
 #pragma unroll
           for (int r = 0; r < BM; r += 4) {
             const float4 pr = *(const float4*)(pt + k * PP + r);
@@ -560,7 +551,7 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
     for (int r = 0; r < BM; ++r) {
       const int R = s.rt * BM + r;
       if (R >= NR) break;
-      const int i = R / a.G, row = s.row0 + i, head = s.h * a.G + R - i * a.G;
+      const int i = (int)a.by_g.div((uint32_t)R), row = s.row0 + i, head = s.h * a.G + R - i * a.G;
       const float2 v = ml[r];
       if (whole) {
         const bool empty = v.y == 0.f && !sees_any(a, row, s.n, s.ctx);
@@ -750,6 +741,8 @@ extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_pag
   a.nh = (int32_t)q->n_heads;
   a.G = (int32_t)(q->n_heads / cache->n_kv_heads);
   a.scale = q->scale;
+  a.by_g = FastDiv((uint32_t)a.G);
+  a.by_kv = FastDiv(cache->n_kv_heads);
   a.bm = p.bm;
   a.part = (float*)work;
   a.part_ml = (float2*)(a.part + 2ll * p.ctas * p.bm * p.dp);

@@ -27,6 +27,7 @@ struct TreeArgs {
   int64_t q_stride;  // elements
   const uint32_t* mask;
   int32_t mask_words, nh, G;
+  FastDiv by_g, by_kv;  // by G, by the cached heads
   float scale;
   float* part;      // [2 * ctas][BM][DP] outputs
   float2* part_ml;  // [2 * ctas][BM] (max, sum)
@@ -58,7 +59,7 @@ __device__ __forceinline__ void tile_prefix(const TreeArgs& a, uint32_t* prefix,
     if (bad_sequence(a, n, len)) {
       if (report && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
     } else if (n > 0) {
-      const uint32_t rts = ((uint32_t)n * a.G + BM - 1) / BM;
+      const uint32_t rts = ((uint32_t)n * a.G + BM - 1) / BM;  // BM is a power of two
       sum += rts * a.c.n_kv * (a.whole ? 1 : (len + BN - 1) / BN);
     }
   }
@@ -101,10 +102,9 @@ __device__ __forceinline__ Segment segment_at(const TreeArgs& a, const uint32_t*
   s.len = a.b.kv_len[lo];
   s.ctx = s.len - s.n;
   s.tiles = (s.len + BN - 1) / BN;
-  const uint32_t line = a.whole ? 1 : s.tiles;
-  const uint32_t off = w - prefix[lo], unit = off / line;
-  s.t0 = (int)(off - unit * line);
-  s.rt = (int)(unit / (uint32_t)a.c.n_kv);
+  const uint32_t off = w - prefix[lo], unit = a.whole ? off : off / (uint32_t)s.tiles;
+  s.t0 = a.whole ? 0 : (int)(off - unit * s.tiles);
+  s.rt = (int)a.by_kv.div(unit);
   s.h = (int)(unit - (uint32_t)s.rt * a.c.n_kv);
   s.t1 = a.whole ? s.tiles : (int)min((uint32_t)s.tiles, s.t0 + (end - w));
   s.unit0 = w - s.t0;
@@ -164,6 +164,19 @@ __device__ __forceinline__ bool sees_any(const TreeArgs& a, int row, int n, int 
   return false;
 }
 
+// Place in a ring of item after item: slot and the parity of its use (a division by a run-time slot
+// count would cost more than a product's issue).
+struct RingCursor {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int slots) {
+    if (++slot == slots) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
+
 // K and V of the layer as tensor maps (TMA), for 16-bit caches with pages of a multiple of 16
 // positions: 64-dim boxes of `box` rows of one page, 128-byte swizzled. Dimension 0 is the head's dim;
 // heads, rows and pages are the dimensions at_head, at_row and at_page in order of their strides.
@@ -208,6 +221,14 @@ template <typename T>
 __device__ __forceinline__ uint32_t nonfinite_halves(uint32_t v) {
   constexpr uint32_t E = __is_same(T, __half) ? 0x7c00u : 0x7f80u;
   return ((v & E) == E ? 0xffffu : 0u) | ((v >> 16 & E) == E ? 0xffff0000u : 0u);
+}
+// True in one lane of the (converged) warp. Products and TMA copies take their operands from uniform
+// registers: behind this branch, of values that the whole warp holds alike, the compiler needs no
+// loop over the lanes to get them there.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
 }
 // One arrival for the warp, after all its lanes' work.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
@@ -278,70 +299,52 @@ __device__ __forceinline__ float soft_lse(float m, float l) {
   return (sizeof(T) == 4 ? m : m * 0.69314718055994531f) + logf(l);
 }
 
+// Adds the non-finite values of a tree's V rows [j0, j1) (positions) to the outputs that see them: the
+// kernels' products saw zeros in their place. o(r, d) is the output of vector r of the tile, dim d; a
+// weight is positive, so the sum is what the value is. By NT threads over (vector, dim); kept small,
+// it hardly ever runs.
+template <typename T, typename O>
+__device__ __forceinline__ void add_nonfinite(const TreeArgs& a, const Segment& s, int rows, int j0, int j1, int tid, int nt, O o) {
+  const int D = a.c.head_dim;
+  const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
+#pragma unroll 1
+  for (int j = j0; j < j1; ++j) {
+    const int64_t off = paged_offset(a.c, table, a.b.table_stride, j);
+    if (off < 0) continue;
+    const T* v = (const T*)(a.c.v + off + (int64_t)s.h * a.c.head_bytes);
+#pragma unroll 1
+    for (int e = tid; e < rows * D; e += nt) {
+      const int r = e / D, d = e - r * D;
+      const float f = Elem<T>::get(v[d]);
+      if (isfinite(f)) continue;
+      const int i = (int)a.by_g.div((uint32_t)(s.rt * a.bm + r));
+      if (sees_node(a, s.row0 + i, i, j - s.ctx)) o(r, d) += f;
+    }
+  }
+}
+
 // Joins the partials of the units that the line was cut in. Items are spread over a grid of any
-// size: of a unit with few partials 16 rows, four a warp with all their loads in flight together; of
-// one with many a row, its partials over the four warps. Lane l of a warp holds dims 4 l .. of every
-// 128 (2 l .. of 64).
-constexpr int kJoinMany = 8, kJoinRows = 4;
-template <typename T, int DP>
-__device__ __forceinline__ void join_add(float (&acc)[DP / 32], const float* o, float f, int lane) {
-  if constexpr (DP >= 128) {
-#pragma unroll
-    for (int q = 0; q < DP / 128; ++q) {
-      const float4 v = __ldcg((const float4*)(o + q * 128 + 4 * lane));
-      acc[4 * q] += v.x * f;
-      acc[4 * q + 1] += v.y * f;
-      acc[4 * q + 2] += v.z * f;
-      acc[4 * q + 3] += v.w * f;
-    }
-  } else {
-    const float2 v = __ldcg((const float2*)(o + 2 * lane));
-    acc[0] += v.x * f;
-    acc[1] += v.y * f;
-  }
-}
-template <typename T, int DP>
-__device__ __forceinline__ void join_write(const TreeArgs& a, const JoinRec& rec, int r, const float (&acc)[DP / 32],
-                                           float l, float mx, int lane) {
-  const int R = rec.vec0 + r, i = R / a.G, row = rec.row0 + i, head = rec.head0 + (R - i * a.G), D = a.c.head_dim;
-  const bool empty = l == 0.f && !sees_any(a, row, rec.see >> 1, rec.see & 1);
-  T* out = (T*)a.out + ((int64_t)row * a.nh + head) * D;
-  constexpr int V = DP >= 128 ? 4 : 2;
-#pragma unroll
-  for (int q = 0; q < DP / 32; q += V) {
-    const int d = q / V * 32 * V + V * lane;
-    if (d >= D) continue;
-    float f[4];
-#pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = empty ? 0.f : acc[q + e] / l;
-    if constexpr (V * sizeof(T) >= 8) {
-      store_n<T, V>(out + d, f);
-    } else {
-      out[d] = Elem<T>::put(f[0]);
-      out[d + 1] = Elem<T>::put(f[1]);
-    }
-  }
-  if (a.lse && lane == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(mx, l);
-}
+// size; 16 lanes take a row, DP / 16 dims each: of a unit with few partials an item is 8 rows, of one
+// with many a row, its partials dealt to the 8 groups. The kernel runs once through its code, which
+// therefore is kept short: fetching instructions is most of its time.
+constexpr int kJoinMany = 8;
 template <typename T, int DP>
 __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
   extern __shared__ uint32_t s_items[];  // [ctas + 1] prefix of items
   __shared__ uint32_t scan[4];
-  __shared__ float s_acc[3][DP];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ float s_acc[8][DP];
+  __shared__ float s_l[8];
+  constexpr int V = DP / 16;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = tid >> 4, l16 = tid & 15;
+  const int each = (a.ctas + 127) / 128, c0 = min(a.ctas, tid * each), c1 = min(a.ctas, c0 + each);
   pdl_wait();
   {
-    constexpr int kMost = 8;  // CTAs on the line per thread: up to 1024
-    const int each = (a.ctas + 127) / 128, c0 = min(a.ctas, tid * each), c1 = min(a.ctas, c0 + each);
-    int2 pr[kMost];
-#pragma unroll
-    for (int i = 0; i < kMost; ++i)
-      pr[i] = c0 + i < c1 ? __ldcg((const int2*)&a.recs[c0 + i]) : make_int2(0, 0);  // parts, rows
-    uint32_t sum = 0, mine[kMost];
-#pragma unroll
-    for (int i = 0; i < kMost; ++i) {
-      mine[i] = sum;
-      if (pr[i].x > 0) sum += pr[i].x > kJoinMany ? pr[i].y : (pr[i].y + 4 * kJoinRows - 1) / (4 * kJoinRows);
+    uint32_t sum = 0;
+#pragma unroll 1
+    for (int c = c0; c < c1; ++c) {
+      const int2 pr = __ldcg((const int2*)&a.recs[c]);  // parts, rows
+      s_items[c] = sum;
+      if (pr.x > 0) sum += pr.x > kJoinMany ? pr.y : (pr.y + 7) / 8;
     }
     uint32_t inc = sum;
 #pragma unroll
@@ -352,88 +355,86 @@ __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
     if (lane == 31) scan[warp] = inc;
     __syncthreads();
     uint32_t before = inc - sum;
+#pragma unroll 1
     for (int w = 0; w < warp; ++w) before += scan[w];
-#pragma unroll
-    for (int i = 0; i < kMost; ++i)
-      if (c0 + i < c1) s_items[c0 + i] = before + mine[i];
+#pragma unroll 1
+    for (int c = c0; c < c1; ++c) s_items[c] += before;
     if (tid == 127) s_items[a.ctas] = before + sum;
     __syncthreads();
   }
   const uint32_t total = s_items[a.ctas];
+#pragma unroll 1
   for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
     int lo = 0, hi = a.ctas;
+#pragma unroll 1
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (s_items[mid] <= item) lo = mid;
       else hi = mid;
     }
     const JoinRec rec = a.recs[lo];
-    const int at = (int)(item - s_items[lo]);
-    auto slot = [&](int p, int r) { return (int64_t)(p == 0 ? rec.first_slot : 2 * (rec.cta + p)) * a.bm + r; };
-    if (rec.parts <= kJoinMany) {
-      // Lane 8 i + p: partial p of the warp's row i.
-      const int r0 = (at * 4 + warp) * kJoinRows, p = lane & 7, i = lane >> 3;
-      const bool has = p < rec.parts && r0 + i < rec.rows;
-      const float2 ml = has ? __ldcg(&a.part_ml[slot(p, r0 + i)]) : make_float2(-INFINITY, 0.f);
-      float mx = ml.x;
+    const bool many = rec.parts > kJoinMany;
+    const int at = (int)(item - s_items[lo]), r = many ? at : at * 8 + grp;
+    const bool live = r < rec.rows;
+    const int parts = live ? rec.parts : 0;
+    auto slot = [&](int p) { return (int64_t)(p == 0 ? rec.first_slot : 2 * (rec.cta + p)) * a.bm + r; };
+    float mx = -INFINITY;
+#pragma unroll 2
+    for (int p = l16; p < parts; p += 16) mx = fmaxf(mx, __ldcg(&a.part_ml[slot(p)]).x);
 #pragma unroll
-      for (int o = 1; o < 8; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      const float wgt = soft_exp<T>(ml.x - (mx == -INFINITY ? 0.f : mx));
-      float l = has ? ml.y * wgt : 0.f;
-#pragma unroll
-      for (int o = 1; o < 8; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      float acc[kJoinRows][DP / 32];
-#pragma unroll
-      for (int k = 0; k < kJoinRows; ++k)
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) acc[k][d] = 0.f;
-      for (int q = 0; q < rec.parts; ++q)
-#pragma unroll
-        for (int k = 0; k < kJoinRows; ++k) {
-          const float f = __shfl_sync(0xffffffffu, wgt, 8 * k + q);
-          if (r0 + k < rec.rows) join_add<T, DP>(acc[k], a.part + slot(q, r0 + k) * DP, f, lane);
-        }
-#pragma unroll
-      for (int k = 0; k < kJoinRows; ++k) {
-        const float lk = __shfl_sync(0xffffffffu, l, 8 * k), mk = __shfl_sync(0xffffffffu, mx, 8 * k);
-        if (r0 + k < rec.rows) join_write<T, DP>(a, rec, r0 + k, acc[k], lk, mk, lane);
-      }
-      continue;
-    }
-    float mx = -INFINITY, l = 0.f, acc[DP / 32];
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d) acc[d] = 0.f;
-    for (int p = lane; p < rec.parts; p += 32) mx = fmaxf(mx, __ldcg(&a.part_ml[slot(p, at)]).x);
-    mx = warp_max(mx);
+    for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     const float base = mx == -INFINITY ? 0.f : mx;
-    for (int p0 = 0; p0 < rec.parts; p0 += 32) {
-      float wgt = 0.f;
-      if (p0 + lane < rec.parts) {
-        const float2 v = __ldcg(&a.part_ml[slot(p0 + lane, at)]);
-        wgt = soft_exp<T>(v.x - base);
-        l += v.y * wgt;
+    float acc[V], l = 0.f;
+#pragma unroll
+    for (int d = 0; d < V; ++d) acc[d] = 0.f;
+#pragma unroll 4
+    for (int p = many ? grp : 0; p < parts; p += many ? 8 : 1) {
+      const float2 ml = __ldcg(&a.part_ml[slot(p)]);
+      const float* o = a.part + slot(p) * DP + V * l16;
+      float x[V];
+#pragma unroll
+      for (int d = 0; d < V; d += 4) {
+        const float4 v = __ldcg((const float4*)(o + d));
+        x[d] = v.x;
+        x[d + 1] = v.y;
+        x[d + 2] = v.z;
+        x[d + 3] = v.w;
       }
+      const float f = soft_exp<T>(ml.x - base);
+      l += ml.y * f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int p = 4 * k + warp;
-        const float f = __shfl_sync(0xffffffffu, wgt, p);
-        if (p0 + p < rec.parts) join_add<T, DP>(acc, a.part + slot(p0 + p, at) * DP, f, lane);
+      for (int d = 0; d < V; ++d) acc[d] += x[d] * f;
+    }
+    if (many) {  // the groups' shares, in order
+#pragma unroll
+      for (int d = 0; d < V; ++d) s_acc[grp][V * l16 + d] = acc[d];
+      if (l16 == 0) s_l[grp] = l;
+      __syncthreads();
+      if (grp == 0) {
+#pragma unroll 1
+        for (int g = 1; g < 8; ++g) {
+          l += s_l[g];
+#pragma unroll
+          for (int d = 0; d < V; ++d) acc[d] += s_acc[g][V * l16 + d];
+        }
       }
+      __syncthreads();
     }
-    l = warp_sum(l);
-    // The warps' shares, in order.
-    if (warp > 0)
+    if (!live || (many && grp > 0)) continue;
+    const int R = rec.vec0 + r, i = (int)a.by_g.div((uint32_t)R), row = rec.row0 + i, head = rec.head0 + (R - i * a.G);
+    const bool empty = l == 0.f && !sees_any(a, row, rec.see >> 1, rec.see & 1);
+    const float inv = 1.f / l;
 #pragma unroll
-      for (int q = 0; q < DP / 32; ++q) s_acc[warp - 1][q * 32 + lane] = acc[q];
-    __syncthreads();
-    if (warp == 0) {
+    for (int d = 0; d < V; ++d) acc[d] = empty ? 0.f : acc[d] * inv;
+    T* out = (T*)a.out + ((int64_t)row * a.nh + head) * a.c.head_dim + V * l16;
+    if constexpr (V == 4) {
+      if (4 * l16 < a.c.head_dim) store_n<T, 4>(out, acc);
+    } else {
 #pragma unroll
-      for (int w = 0; w < 3; ++w)
-#pragma unroll
-        for (int q = 0; q < DP / 32; ++q) acc[q] += s_acc[w][q * 32 + lane];
-      join_write<T, DP>(a, rec, at, acc, l, mx, lane);
+      for (int d = 0; d < V; d += 8)
+        if (V * l16 + d < a.c.head_dim) store_n<T, 8>(out + d, acc + d);
     }
-    __syncthreads();
+    if (a.lse && l16 == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(mx, l);
   }
 }
 

@@ -7,9 +7,8 @@ namespace pp {
 template <auto kernel, typename... Extra>
 pp_status launch_tree(const TreeArgs& a, int threads, size_t smem, cudaStream_t st, Extra... extra) {
   static bool done[64] = {};
-  // Less the static shared memory of any of the kernels.
-  if (!reserve_smem(kernel, kMaxSmem - 512, a.dev, done))
-    return paged_fail(PP_E_CUDA, "cannot reserve the attention's shared memory");
+  if (!reserve_smem(kernel, kMaxSmem, a.dev, done))
+    return PP_E_CUDA;
   kernel<<<a.ctas, threads, smem, st>>>(a, extra...);
   return launch_status("pp_tree_attention");
 }

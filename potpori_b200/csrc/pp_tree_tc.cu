@@ -65,30 +65,30 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                : "memory");
 }
-// SWIZZLE_128B operand at byte address saddr: `lead` bytes between 64-element blocks of a
-// MN-major operand (unused K-major), 1024 between 8-row atoms.
-__device__ __forceinline__ uint64_t tc_desc(uint32_t saddr, uint32_t lead) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) | ((uint64_t)64 << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// Descriptor of a SWIZZLE_128B operand: the low word holds its address / 16 and, MN-major, the bytes
+// / 16 between its 64-element blocks; the high word 1024 bytes between 8-row atoms, version, swizzle.
+// One thread issues every product, so what it computes per product counts: the words are kept and
+// stepped by constants.
+constexpr uint32_t kTcDescHi = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ constexpr uint32_t tc_lead(uint32_t bytes) { return (bytes >> 4) << 16; }
 // kind::f16, F32 accumulator, A and B both of T, M = 128, N = n, B MN-major when mn.
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t tc_idesc(int n, bool mn) {
   constexpr uint32_t t = __is_same(T, __half) ? 0u : 1u;
   return (1u << 4) | (t << 7) | (t << 10) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kTcDescHi)
       : "memory");
 }
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kTcDescHi)
       : "memory");
 }
 // 32 columns of the thread's lane.
@@ -156,7 +156,8 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kernel(const TreeArgs a, const __grid_constant__ TreeMaps maps, const int slots) {
   using C = TcCfg<DP>;
   constexpr int BM = kTcBM, BN = kTcBN, UR = DP / 8;
-  extern __shared__ __align__(1024) uint8_t sm[];
+  extern __shared__ __align__(1024) uint8_t tc_smem[];
+  uint8_t* sm = tc_smem;
   uint8_t* qs = sm;
   uint8_t* ring = sm + C::kQ;
   TcBars* bars = (TcBars*)(ring + (size_t)slots * C::kItem);
@@ -200,32 +201,43 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
   bool ok = true;
 
   if (warp == 4 && maps.box) {
-    // ---- producer, by TMA: lane (g, b) of a tile its row group g and 64-dim block b
+    // ---- producer, by TMA: lane g looks row group g of a tile up (box rows, one page)
     constexpr int NB = DP / 64;
-    const int boxes = BN / maps.box * NB, grp = lane / NB, blk = lane % NB;
+    const int groups = BN / maps.box;
     int n = 0;
+    RingCursor rc;
     for (uint32_t w = begin; w < end && ok;) {
       const Segment s = segment_at<BM, BN>(a, prefix, w, end);
       const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
       const int cnt = s.t1 - s.t0;
       // Places of tile i (V's turn), i + 1 (K's) and i + 2, looked up ahead of their copies.
       BoxPlace prev, cur, next;
-      auto look = [&](BoxPlace& f, int i) { f.look(a, s, table, (s.t0 + i) * BN + grp * maps.box, i < cnt && lane < boxes); };
+      auto look = [&](BoxPlace& f, int i) { f.look(a, s, table, (s.t0 + i) * BN + lane * maps.box, i < cnt && lane < groups); };
       look(cur, 0);
       look(next, 1);
       prev = cur;
       for (int j = 0; j < 2 * cnt; ++j, ++n) {
         const bool isv = j == 2 * cnt - 1 || (j > 0 && !(j & 1));
-        const int slot = n % slots;
-        if (n >= slots && !warp_wait(&bars->free[slot], (uint32_t)(n / slots - 1) & 1u)) {
+        const int slot = rc.slot;
+        if (n >= slots && !warp_wait(&bars->free[slot], rc.phase ^ 1u)) {
           ok = false;
           break;
         }
-        if (lane == 0) mbar_arrive_expect_tx(&bars->full[slot], C::kItem);
+        uint8_t* dst = ring + (size_t)slot * C::kItem;
+        if (elect_one()) mbar_arrive_expect_tx(&bars->full[slot], C::kItem);
         __syncwarp();
-        if (lane < boxes)
-          tma_box(ring + (size_t)slot * C::kItem + blk * (BN * 128) + grp * maps.box * 128, isv ? &maps.v : &maps.k,
-                  &bars->full[slot], maps, 64 * blk, s.h, isv ? prev.row : cur.row, isv ? prev.page : cur.page);
+#pragma unroll 1
+        for (int g = 0; g < groups; ++g) {
+          const int page = __shfl_sync(0xffffffffu, isv ? prev.page : cur.page, g);
+          const int row = __shfl_sync(0xffffffffu, isv ? prev.row : cur.row, g);
+          if (elect_one())
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+              tma_box(dst + i * (BN * 128) + g * maps.box * 128, isv ? &maps.v : &maps.k, &bars->full[slot], maps, 64 * i,
+                      s.h, row, page);
+          __syncwarp();
+        }
+        rc.next(slots);
         if (j == 0 || isv) {
           prev = cur;
           cur = next;
@@ -242,6 +254,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
     constexpr int RPP = 32 / UR;  // rows of one pass of a warp
     const int u = lane % UR, sub = lane / UR;
     int n = 0;
+    RingCursor rc, done;
     for (uint32_t w = begin; w < end && ok;) {
       const Segment s = segment_at<BM, BN>(a, prefix, w, end);
       const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
@@ -254,14 +267,14 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       prev = cur;
       for (int j = 0; j < 2 * cnt; ++j, ++n) {
         const bool isv = j == 2 * cnt - 1 || (j > 0 && !(j & 1));
-        const int slot = n % slots;
-        if (n >= slots && !warp_wait(&bars->free[slot], (uint32_t)(n / slots - 1) & 1u)) {
+        const int slot = rc.slot;
+        if (n >= slots && !warp_wait(&bars->free[slot], rc.phase ^ 1u)) {
           ok = false;
           break;
         }
         uint8_t* dst = ring + (size_t)slot * C::kItem;
         const uint8_t* base = isv ? a.c.v : a.c.k;
-#pragma unroll
+#pragma unroll 4
         for (int q = 0; q < 32 / RPP; ++q) {
           const int l = q * RPP + sub, r = pw * 32 + l;
           const int64_t off = isv ? prev.row(a, l) : cur.row(a, l);
@@ -269,6 +282,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           cp_async16(dst + (u >> 3) * (BN * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4), base + (read ? off + 16 * u : 0), read);
         }
         cp_async_commit();
+        rc.next(slots);
         if (j == 0 || isv) {
           prev = cur;
           cur = next;
@@ -277,65 +291,85 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         if (n >= kTcLag) {
           cp_async_wait<kTcLag>();
           fence_async();
-          warp_arrive(&bars->full[(n - kTcLag) % slots], lane);
+          warp_arrive(&bars->full[done.slot], lane);
+          done.next(slots);
         }
       }
       w += s.step;
     }
     cp_async_wait<0>();
     fence_async();
-    for (int i = n > kTcLag ? n - kTcLag : 0; i < n; ++i) warp_arrive(&bars->full[i % slots], lane);
+    for (int i = n > kTcLag ? n - kTcLag : 0; i < n; ++i) {
+      warp_arrive(&bars->full[done.slot], lane);
+      done.next(slots);
+    }
   } else if (warp == 6) {
-    // ---- products
-    if (lane == 0) {
+    // ---- products: the warp waits together, one lane issues
+    {
       constexpr uint32_t iqk = tc_idesc<T>(BN, false), ipv = tc_idesc<T>(DP, true);
-      const uint32_t qb = smem_u32(qs), rb = smem_u32(ring);
-      int n = 0, g = 0, seg = 0;  // items, tiles, segments so far
-      auto take = [&]() -> bool { return mbar_wait(&bars->full[n % slots], (uint32_t)(n / slots) & 1u); };
-      auto qk = [&]() {  // S = Q K^T from the ring's next item
-        const uint32_t kb = rb + (uint32_t)(n % slots) * C::kItem;
+      const uint32_t qa = (smem_u32(qs) >> 4) | tc_lead(16), ring_a = smem_u32(ring) >> 4;
+      RingCursor rc;
+      uint32_t tile = 0;  // parity of the tile whose S comes next
+      uint32_t seg = 0;
+      bool first = true;
+      auto take = [&]() -> bool { return warp_wait(&bars->full[rc.slot], rc.phase); };
+      auto qk = [&]() {  // S = Q K^T from the ring's next item; dims past the head's are zero
+        const uint32_t ka = (ring_a + rc.slot * (C::kItem >> 4)) | tc_lead(16);
+        if (elect_one()) {
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks)
-          if (16 * ks < D)
-            tc_mma_ss(tS, tc_desc(qb + (ks >> 2) * (BM * 128) + (ks & 3) * 32, 16),
-                      tc_desc(kb + (ks >> 2) * (BN * 128) + (ks & 3) * 32, 16), iqk, ks != 0);
-        tc_commit(&bars->free[n % slots]);
-        tc_commit(&bars->s_full);
-        ++n;
+          for (int ks = 0; ks < DP / 16; ++ks)
+            tc_mma_ss(tS, qa + (ks >> 2) * (BM * 8) + (ks & 3) * 2, ka + (ks >> 2) * (BN * 8) + (ks & 3) * 2, iqk, ks != 0);
+          tc_commit(&bars->s_full);
+          tc_commit(&bars->free[rc.slot]);
+        }
+        __syncwarp();
+        rc.next(slots);
       };
       for (uint32_t w = begin; w < end && ok;) {
         const Segment s = segment_at<BM, BN>(a, prefix, w, end);
         const int cnt = s.t1 - s.t0;
-        ok = mbar_wait(&bars->q_full, (uint32_t)seg & 1u) && take() && (g == 0 || mbar_wait(&bars->s_free, (uint32_t)(g - 1) & 1u));
-        if (!ok) break;
-        tc_fence_after();
-        qk();
-        for (int i = 0; i < cnt; ++i, ++g) {
+        if (!warp_wait(&bars->q_full, seg)) {
+          ok = false;
+          break;
+        }
+        // Step i issues S of tile i + 1, then O of tile i.
+        for (int i = -1; i < cnt; ++i) {
           if (i + 1 < cnt) {
-            ok = take() && mbar_wait(&bars->s_free, (uint32_t)g & 1u);
-            if (!ok) break;
+            if (!take() || !(first || warp_wait(&bars->s_free, tile ^ 1u))) {
+              ok = false;
+              break;
+            }
+            first = false;
+            tile ^= 1u;
             tc_fence_after();
             qk();
           }
-          ok = take() && mbar_wait(&bars->p_full, (uint32_t)g & 1u);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t vb = rb + (uint32_t)(n % slots) * C::kItem;
-#pragma unroll
-          for (int ks = 0; ks < BN / 16; ++ks) {
-            const uint64_t vd = tc_desc(vb + ks * 2048, BN * 128);
-            tc_mma_ts(tO, tP + 8 * ks, vd, ipv, (i | ks) != 0);
-            tc_mma_ts(tO, tP + 32 + 8 * ks, vd, ipv, 1u);
+          if (i < 0) continue;
+          // P of tile i: where S of tile i + 1 went out above, `tile` is already the next one's.
+          if (!take() || !warp_wait(&bars->p_full, i + 1 < cnt ? tile : tile ^ 1u)) {
+            ok = false;
+            break;
           }
-          tc_commit(&bars->free[n % slots]);
-          tc_commit(&bars->pv_done);
-          ++n;
+          tc_fence_after();
+          const uint32_t va = (ring_a + rc.slot * (C::kItem >> 4)) | tc_lead(BN * 128);
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks) {
+              tc_mma_ts(tO, tP + 8 * ks, va + ks * 128, ipv, ks == 0 ? i : 1u);
+              tc_mma_ts(tO, tP + 32 + 8 * ks, va + ks * 128, ipv, 1u);
+            }
+            tc_commit(&bars->pv_done);
+            tc_commit(&bars->free[rc.slot]);
+          }
+          __syncwarp();
+          rc.next(slots);
         }
-        ++seg;
+        seg ^= 1u;
         w += s.step;
       }
-      tc_commit(&bars->end);
-      mbar_wait(&bars->end, 0);  // no product of this CTA runs when TMEM is freed
+      if (elect_one()) tc_commit(&bars->end);
+      __syncwarp();
+      warp_wait(&bars->end, 0);  // no product of this CTA runs when TMEM is freed
     }
   } else if (warp < 4) {
     // ---- softmax
@@ -352,11 +386,12 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       const int cnt = s.t1 - s.t0, NR = s.n * a.G;
       if (w == begin && tid == 0) write_join<BM>(a, &s, per);
       // The previous segment's products with Q are complete (its last S was taken).
+#pragma unroll 4
       for (int e = tid; e < BM * UR; e += 128) {
         const int r = e / UR, u = e % UR, R = s.rt * BM + r;
         uint4 v = make_uint4(0u, 0u, 0u, 0u);
         if (R < NR && 8 * u < D) {
-          const int i = R / a.G;
+          const int i = (int)a.by_g.div((uint32_t)R);
           v = *(const uint4*)((const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(s.h * a.G + R - i * a.G) * D + 8 * u);
           v = make_uint4((v.x & keep) ^ flip, (v.y & keep) ^ flip, (v.z & keep) ^ flip, (v.w & keep) ^ flip);
         }
@@ -365,7 +400,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       fence_async();
       warp_arrive(&bars->q_full, lane);
 
-      const int R = s.rt * BM + tid, i = R / a.G, row = s.row0 + i;
+      const int R = s.rt * BM + tid, i = (int)a.by_g.div((uint32_t)R), row = s.row0 + i;
       float m = -INFINITY, l = 0.f;
       for (int t = 0; t < cnt; ++t, ++g) {
         if (!warp_wait(&bars->s_full, (uint32_t)g & 1u)) {
@@ -421,6 +456,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
             break;
           }
           uint32_t found = 0;
+#pragma unroll 4
           for (int e = tid; e < BN * UR; e += 128) {
             uint4* p = (uint4*)(ring + (size_t)slot * C::kItem + e * 16);
             if (j0 + ((e >> 3) & (BN - 1)) >= s.len) {
@@ -488,43 +524,66 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       const int head = s.h * a.G + R - i * a.G;
       const bool empty = live && l == 0.f && !sees_any(a, row, s.n, s.ctx);
       const float inv = 1.f / l;
+      if (dirty) {  // column after column in TMEM: a value is the same for every lane of the warp
+#pragma unroll 1
+        for (int j = max(s.ctx, s.t0 * BN); j < min(s.len, s.t1 * BN); ++j) {
+          const int64_t off = paged_offset(a.c, a.b.table + (int64_t)s.b * a.b.table_stride, a.b.table_stride, j);
+          if (off < 0) continue;
+          const bool see = live && sees_node(a, row, i, j - s.ctx);
+          const T* src = (const T*)(a.c.v + off + (int64_t)s.h * a.c.head_bytes);
+#pragma unroll 1
+          for (int d = 0; d < D; ++d) {
+            const float f = Elem<T>::get(src[d]);
+            if (isfinite(f)) continue;
+            uint32_t col;
+            asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(col) : "r"(tO + lanes + d) : "memory");
+            tc_wait_ld();
+            col = __float_as_uint(__uint_as_float(col) + (see ? f : 0.f));
+            asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(tO + lanes + d), "r"(col) : "memory");
+            tc_wait_st();
+          }
+        }
+      }
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
-        if (c >= D && whole) break;
         float o[32];
         tc_ld32(tO + lanes + c, o);
         tc_wait_ld();
-        if (dirty && live) {
-          const int last = min(s.len, s.t1 * BN);
-          for (int j = max(s.ctx, s.t0 * BN); j < last; ++j) {
-            if (!sees_node(a, row, i, j - s.ctx)) continue;
-            const int64_t off = paged_offset(a.c, a.b.table + (int64_t)s.b * a.b.table_stride, a.b.table_stride, j);
-            if (off < 0) continue;
-            const uint32_t* src = (const uint32_t*)(a.c.v + off + (int64_t)s.h * a.c.head_bytes + 2 * c);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              if (c + 2 * k >= D) break;
-              const uint32_t v = src[k], bad = nonfinite_halves<T>(v);
-              const float2 f = tc_unpack(v, (T*)nullptr);
-              if (bad & 1u) o[2 * k] += f.x;
-              if (bad >> 16) o[2 * k + 1] += f.y;
-            }
-          }
-        }
-        if (live && whole) {
+        // A lane holds a row, so its stores would scatter over 32 rows: the warp's rows pass through
+        // its share of Q's space (every product with Q is complete) and leave 128 bytes of a row at a
+        // time. Unit v of row r sits at v ^ (r & 7).
+        uint8_t* turn = qs + warp * 4096;
+        if (whole) {
+          const uint32_t half = (c >> 5 & 1) * 4;  // 64 dims of T fill the 128 bytes
 #pragma unroll
           for (int k = 0; k < 32; k += 8) {
-            if (c + k >= D) break;
             float f[8];
 #pragma unroll
             for (int q = 0; q < 8; ++q) f[q] = empty ? 0.f : o[k + q] * inv;
-            store8((T*)a.out + ((int64_t)row * a.nh + head) * D + c + k, f);
+            store8((T*)(turn + lane * 128 + (((half + k / 8) ^ (lane & 7)) << 4)), f);
           }
-        } else if (live) {
-          float4* dst = (float4*)(a.part + (slot * BM + tid) * DP + c);
+          if (!half && c + 32 < DP) continue;
+        } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          for (int k = 0; k < 8; ++k)
+            *(float4*)(turn + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         }
+        __syncwarp();
+        const int v = lane & 7;
+#pragma unroll 4
+        for (int k = 0; k < 8; ++k) {
+          const int r = 4 * k + (lane >> 3), Rr = s.rt * BM + warp * 32 + r;
+          const uint4 x = *(const uint4*)(turn + r * 128 + ((v ^ (r & 7)) << 4));
+          if (Rr >= NR) continue;
+          if (whole) {
+            const int d = (c & ~63) + 8 * v, ir = (int)a.by_g.div((uint32_t)Rr);
+            if (d < D)
+              *(uint4*)((T*)a.out + ((int64_t)(s.row0 + ir) * a.nh + s.h * a.G + Rr - ir * a.G) * D + d) = x;
+          } else {
+            *(uint4*)(a.part + (slot * BM + warp * 32 + r) * DP + c + 4 * v) = x;
+          }
+        }
+        __syncwarp();
       }
       if (live && whole && a.lse) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(m, l);
       if (live && !whole) a.part_ml[slot * BM + tid] = make_float2(m, l);
