@@ -39,16 +39,16 @@ template <int DP>
 struct TcCfg {
   static constexpr int kQ = kTcBM * DP * 2;
   static constexpr int kItem = kTcBN * DP * 2;  // a K or V tile
-  static constexpr int kSlots = DP == 256 ? 4 : DP == 128 ? 5 : 8;
+  static constexpr int kTurn = 4 * 4096;        // rows on their way out, 4 KB a softmax warp
+  static constexpr int kSlots = DP == 64 ? 8 : 4;
   static constexpr int kPerSm = DP == 256 ? 1 : 2;
   static constexpr int kCols = DP == 256 ? 512 : 256;  // TMEM: O [DP], S [64], P hi [32], P lo [32]
   static constexpr int kBars = 256;
-  // Two CTAs share 228 KB less 1 KB each: with 5 slots, 1 KB is left for barriers and up to 180
-  // sequences' prefix; larger batches give up a slot.
-  static int slots(int batch) { return DP == 128 && batch > 180 ? 4 : kSlots; }
-  static size_t smem(int batch) {
-    return kQ + (size_t)slots(batch) * kItem + kBars + 4 * (size_t)(batch + 1);
-  }
+  // Two CTAs share 228 KB less 1 KB each: at head_dim 128 that leaves 1 KB beside Q, four slots and
+  // the turn buffer, for the barriers and the prefix of up to 180 sequences. (More slots than four
+  // only lengthen every other load's way through memory: at the card's rate 148 x 2 x 64 KB in flight
+  // are 3 us already.)
+  static size_t smem(int batch) { return kQ + kTurn + kSlots * (size_t)kItem + kBars + 4 * (size_t)(batch + 1); }
 };
 
 struct TcBars {
@@ -153,13 +153,13 @@ __device__ __forceinline__ float2 tc_unpack(uint32_t v, __nv_bfloat16*) { return
 __device__ __forceinline__ float2 tc_unpack(uint32_t v, __half*) { return __half22float2(*(const __half2*)&v); }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kernel(const TreeArgs a, const __grid_constant__ TreeMaps maps, const int slots) {
+__global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kernel(const TreeArgs a, const __grid_constant__ TreeMaps maps) {
   using C = TcCfg<DP>;
-  constexpr int BM = kTcBM, BN = kTcBN, UR = DP / 8;
+  constexpr int BM = kTcBM, BN = kTcBN, UR = DP / 8, slots = C::kSlots;
   extern __shared__ __align__(1024) uint8_t tc_smem[];
   uint8_t* sm = tc_smem;
   uint8_t* qs = sm;
-  uint8_t* ring = sm + C::kQ;
+  uint8_t* ring = sm + C::kQ + C::kTurn;
   TcBars* bars = (TcBars*)(ring + (size_t)slots * C::kItem);
   uint32_t* prefix = (uint32_t*)((uint8_t*)bars + C::kBars);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -374,33 +374,40 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
   } else if (warp < 4) {
     // ---- softmax
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    // The maximum is taken before the scale, so the scale must be positive: its sign goes into Q, and
-    // a scale of zero makes Q zero.
+    // The maximum is taken before the scale, so the scale must be positive: another sign, or zero,
+    // goes into the scores.
     const float sc = a.scale == 0.f ? 1.f : soft_scale<T>(fabsf(a.scale));
-    const uint32_t keep = a.scale == 0.f ? 0u : ~0u, flip = a.scale < 0.f ? 0x80008000u : 0u;
+    // A segment's queries into Q's space, zero past the unit's: asynchronous copies, the next
+    // segment's on their way while this one's rows leave.
+    auto fetch_q = [&](const Segment& f) {
+      const int nr = f.n * a.G;
+#pragma unroll 4
+      for (int e = tid; e < BM * UR; e += 128) {
+        const int r = e / UR, u = e % UR, Rq = f.rt * BM + r;
+        const bool read = Rq < nr && 8 * u < D;
+        const int iq = (int)a.by_g.div((uint32_t)(read ? Rq : 0));
+        const T* src = (const T*)a.q + (read ? (int64_t)(f.row0 + iq) * a.q_stride + (int64_t)(f.h * a.G + Rq - iq * a.G) * D + 8 * u : 0);
+        cp_async16(qs + (u >> 3) * (BM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4), src, read);
+      }
+      cp_async_commit();
+    };
+    Segment s;
+    if (begin < end) {
+      s = segment_at<BM, BN>(a, prefix, begin, end);
+      fetch_q(s);
+    }
     int n0 = 0, g = 0;  // items before this segment, tiles so far
     uint32_t seg = 0;
     if (begin >= end && tid == 0) write_join<BM>(a, nullptr, per);
     for (uint32_t w = begin; w < end && ok;) {
-      const Segment s = segment_at<BM, BN>(a, prefix, w, end);
       const int cnt = s.t1 - s.t0, NR = s.n * a.G;
       if (w == begin && tid == 0) write_join<BM>(a, &s, per);
-      // The previous segment's products with Q are complete (its last S was taken).
-#pragma unroll 4
-      for (int e = tid; e < BM * UR; e += 128) {
-        const int r = e / UR, u = e % UR, R = s.rt * BM + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (R < NR && 8 * u < D) {
-          const int i = (int)a.by_g.div((uint32_t)R);
-          v = *(const uint4*)((const T*)a.q + (int64_t)(s.row0 + i) * a.q_stride + (int64_t)(s.h * a.G + R - i * a.G) * D + 8 * u);
-          v = make_uint4((v.x & keep) ^ flip, (v.y & keep) ^ flip, (v.z & keep) ^ flip, (v.w & keep) ^ flip);
-        }
-        *(uint4*)(qs + (u >> 3) * (BM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = v;
-      }
+      cp_async_wait<0>();
       fence_async();
       warp_arrive(&bars->q_full, lane);
 
       const int R = s.rt * BM + tid, i = (int)a.by_g.div((uint32_t)R), row = s.row0 + i;
+      const bool idle = s.rt * BM + warp * 32 >= NR;
       float m = -INFINITY, l = 0.f;
       for (int t = 0; t < cnt; ++t, ++g) {
         if (!warp_wait(&bars->s_full, (uint32_t)g & 1u)) {
@@ -416,34 +423,6 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         warp_arrive(&bars->s_free, lane);
         const int j0 = (s.t0 + t) * BN;
         const bool tree = j0 + BN > s.ctx;
-        if (tree) {
-          const uint64_t see = seen64(a, s, row, i, j0);
-#pragma unroll
-          for (int k = 0; k < 64; ++k)
-            if (!(see >> k & 1u)) x[k >> 5][k & 31] = -INFINITY;
-        }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int k = 0; k < 64; ++k) top[k & 3] = fmaxf(top[k & 3], x[k >> 5][k & 31]);
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;  // scale > 0
-        const bool grown = mx > m + 8.f || (m == -INFINITY && mx > m);
-        float alpha = 1.f;
-        const bool rescale = __any_sync(0xffffffffu, grown);
-        if (rescale) {
-          const float mn = fmaxf(m, mx);
-          alpha = soft_exp<T>(m - (mn == -INFINITY ? 0.f : mn));
-          m = mn;
-          l *= alpha;
-        }
-        const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < 64; ++k) {
-          float& v = x[k >> 5][k & 31];
-          v = soft_exp<T>(fmaf(v, sc, -base));
-          sum[k & 3] += v;
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         const bool blind = tree && (a.mask || s.n > 1);
         if (blind || j0 + BN > s.len) {
           // Positions past the end hold whatever their page did: zeros there. And a V that some row
@@ -473,6 +452,51 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           if (found) bars->dirty = seg + 1;
           fence_async();
         }
+        if (idle) {  // no row of the warp is in the unit: its P may be anything
+          if (g > 0 && !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
+            ok = false;
+            break;
+          }
+          warp_arrive(&bars->p_full, lane);
+          continue;
+        }
+        if (a.scale <= 0.f) {
+          const float by = a.scale < 0.f ? -1.f : 0.f;
+#pragma unroll
+          for (int k = 0; k < 64; ++k) x[k >> 5][k & 31] *= by;
+        }
+        if (tree) {
+          const uint64_t see = seen64(a, s, row, i, j0);
+#pragma unroll
+          for (int k = 0; k < 64; ++k)
+            if (!(see >> k & 1u)) x[k >> 5][k & 31] = -INFINITY;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < 64; ++k) top[k & 3] = fmaxf(top[k & 3], x[k >> 5][k & 31]);
+        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;  // scale > 0
+        const bool grown = mx > m + 8.f || (m == -INFINITY && mx > m);
+        float alpha = 1.f;
+        const bool rescale = __any_sync(0xffffffffu, grown);
+        if (rescale) {
+          const float mn = fmaxf(m, mx);
+          alpha = soft_exp<T>(m - (mn == -INFINITY ? 0.f : mn));
+          m = mn;
+          l *= alpha;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        // Two elements an instruction where there is one for F32 pairs.
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          float& v0 = x[k >> 4][(2 * k) & 31];
+          float& v1 = x[k >> 4][(2 * k + 1) & 31];
+          const float2 y = __ffma2_rn(make_float2(v0, v1), make_float2(sc, sc), make_float2(-base, -base));
+          v0 = soft_exp<T>(y.x);
+          v1 = soft_exp<T>(y.y);
+          sum[k & 1] = __fadd2_rn(sum[k & 1], make_float2(v0, v1));
+        }
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         if (g > 0 && !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
           ok = false;
           break;
@@ -496,8 +520,9 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           float& v1 = x[k >> 4][(2 * k + 1) & 31];
           p[k] = tc_pack(v0, v1, (T*)nullptr);
           const float2 h = tc_unpack(p[k], (T*)nullptr);
-          v0 -= h.x;
-          v1 -= h.y;
+          const float2 rest = __fadd2_rn(make_float2(v0, v1), make_float2(-h.x, -h.y));
+          v0 = rest.x;
+          v1 = rest.y;
         }
         tc_st32(tP + lanes, p);
 #pragma unroll
@@ -517,6 +542,12 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       if (!warp_wait(&bars->p_full, (uint32_t)(g - 1) & 1u)) {
         ok = false;
         break;
+      }
+      // The last S is taken, so every product with Q is complete: the next segment's queries may come.
+      Segment following = s;
+      if (w + s.step < end) {
+        following = segment_at<BM, BN>(a, prefix, w + s.step, end);
+        fetch_q(following);
       }
       const bool dirty = *(volatile uint32_t*)&bars->dirty == seg + 1;
       const bool whole = s.t0 == 0 && s.t1 == s.tiles, live = R < NR;
@@ -550,9 +581,8 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         tc_ld32(tO + lanes + c, o);
         tc_wait_ld();
         // A lane holds a row, so its stores would scatter over 32 rows: the warp's rows pass through
-        // its share of Q's space (every product with Q is complete) and leave 128 bytes of a row at a
-        // time. Unit v of row r sits at v ^ (r & 7).
-        uint8_t* turn = qs + warp * 4096;
+        // shared memory and leave 128 bytes of a row at a time. Unit v of row r sits at v ^ (r & 7).
+        uint8_t* turn = sm + C::kQ + warp * 4096;
         if (whole) {
           const uint32_t half = (c >> 5 & 1) * 4;  // 64 dims of T fill the 128 bytes
 #pragma unroll
@@ -591,6 +621,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       ++seg;
       n0 += 2 * cnt;
       w += s.step;
+      s = following;
     }
   }
   if (!ok && a.err) atomicOr(a.err, PAGED_TIMEOUT);
@@ -606,7 +637,7 @@ template <typename T, int DP>
 static pp_status run_tc(const TreeArgs& a, const TreeMaps& m, cudaStream_t st) {
   using C = TcCfg<DP>;
   const int B = a.b.batch;
-  const pp_status r = launch_tree<pp_tree_tc_kernel<T, DP>>(a, kTcThreads, C::smem(B), st, m, C::slots(B));
+  const pp_status r = launch_tree<pp_tree_tc_kernel<T, DP>>(a, kTcThreads, C::smem(B), st, m);
   if (r != PP_OK || a.whole) return r;
   return launch_join<T, DP>(a, st);
 }
