@@ -114,14 +114,17 @@ __global__ void __launch_bounds__(kBeamThreads) pp_beam_rows_kernel(const BeamAr
   // among the logits make it NaN.
   const uint32_t wt = __reduce_max_sync(0xffffffffu, top);
   const float wm = wt ? from_ordered(wt) : 0.f;
-  float sums[4] = {0.f, 0.f, 0.f, 0.f};
+  float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"((x[i] - wm) * 1.44269504088896341f));
-    sums[i & 3] += y;
+  for (int i = 0; i < PER; i += 2) {
+    const float2 d = __fadd2_rn(make_float2(x[i], x[i + 1]), make_float2(-wm, -wm));
+    const float2 e = __fmul2_rn(d, make_float2(1.44269504088896341f, 1.44269504088896341f));
+    float2 y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(e.y));
+    sums[i >> 1 & 1] = __fadd2_rn(sums[i >> 1 & 1], y);
   }
-  const float ws = warp_sum((sums[0] + sums[1]) + (sums[2] + sums[3]));
+  const float ws = warp_sum((sums[0].x + sums[0].y) + (sums[1].x + sums[1].y));
   if (lane == 0) s_part[warp] = SliceSum{wt ? wm : -INFINITY, ws};
   __syncthreads();
   if (tid == 0) {
@@ -166,11 +169,21 @@ __global__ void __launch_bounds__(kBeamThreads) pp_beam_rows_kernel(const BeamAr
     }
   }
   if (top && top >= bound) {
+    // Few threads come here, each for few of its logits: those are read again rather than picked out
+    // of the registers, which keeps the code short.
+    const float at_least = bound ? from_ordered(bound) : -INFINITY;
+    uint32_t mask = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (x[i] == -INFINITY || ordered(x[i]) < bound) continue;
+    for (int i = 0; i < PER; ++i) mask |= (uint32_t)(x[i] >= at_least) << i;
+    while (mask) {
+      const int i = __ffs(mask) - 1;
+      mask &= mask - 1;
+      const uint32_t tok = token(i);
+      if (tok >= (uint32_t)(first + n)) continue;  // past the row: -inf in the register
+      const uint64_t key = beam_key(Elem<T>::get(src[tok - first]), tok);
+      if (!key) continue;
       const int at = atomicAdd(&s_n, 1);
-      if (at < kBeamList) s_keys[at] = beam_key(x[i], token(i));
+      if (at < kBeamList) s_keys[at] = key;
     }
   }
   __syncthreads();
@@ -186,11 +199,12 @@ __global__ void __launch_bounds__(kBeamThreads) pp_beam_rows_kernel(const BeamAr
     for (int i = cnt + tid; i < a.k; i += kBeamThreads) out[i] = 0;
   } else {
     uint64_t last = ~0ull;
+#pragma unroll 1
     for (int r = 0; r < a.k; ++r) {
       uint64_t best = 0;
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const uint64_t key = beam_key(x[i], token(i));
+#pragma unroll 1
+      for (int e = tid; e < n; e += kBeamThreads) {
+        const uint64_t key = beam_key(Elem<T>::get(src[e]), (uint32_t)(first + e));
         if (key < last && key > best) best = key;
       }
       best = warp_max_u64(best);

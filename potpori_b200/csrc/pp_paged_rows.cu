@@ -43,109 +43,126 @@ __device__ __forceinline__ float2 rotation(int32_t pos, double inv_freq) {
   return make_float2(c, s);
 }
 
-// Where row t goes: its sequence, cache index and page. By warp 0 into shared memory; index -1
-// marks a row of no sequence.
+// (a, b) turned by the angle of r = (cos, sin).
+__device__ __forceinline__ void turn(float& a, float& b, float2 r) {
+  const float a0 = a, b0 = b;
+  a = a0 * r.x - b0 * r.y;
+  b = b0 * r.x + a0 * r.y;
+}
+
+// Where row t goes: its sequence, cache index and page, by a warp. `report`: this warp marks a bad one.
 struct RowPlace {
   int64_t offset;  // -1: no valid page
   int32_t in_batch, pos;
 };
-__device__ __forceinline__ void place_row(const AppendArgs& a, int t, int lane, RowPlace* out) {
+__device__ __forceinline__ RowPlace place_row(const AppendArgs& a, int t, int lane, bool report) {
+  const int given = a.positions ? a.positions[t] : 0;
   const int b = find_sequence(a.b.cu_rows, a.b.batch, t, lane);
-  if (lane != 0) return;
   RowPlace r = {-1, 0, 0};
   if (b >= 0) {
     const int first = a.b.cu_rows[b], n = a.b.cu_rows[b + 1] - first, len = a.b.kv_len[b];
-    const int32_t given = a.positions ? a.positions[t] : 0;
     const int index = len - n + (t - first);
     r.in_batch = 1;
     r.pos = a.positions ? given : index;
     const int64_t room = (int64_t)a.b.table_stride * a.c.page.d;
     if (len >= n && len <= room)
       r.offset = paged_offset(a.c, a.b.table + (int64_t)b * a.b.table_stride, a.b.table_stride, index);
-    if (r.offset < 0 && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
+    if (r.offset < 0 && report && lane == 0 && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
   }
-  *out = r;
+  return r;
 }
 
-// One CTA per row and share of its heads. tph lanes take a head, 8 dims each, as two runs of 4: of
-// the rotated dims lane j holds both halves' run j, so that a pair never leaves its lane, of the
-// others 8 in a row. (Interleaved pairs: all dims 8 in a row.) The row's rotary_dim / 2 angles are
-// formed once, in shared memory, and a lane keeps its own for all heads; its first head is fetched
-// while the row's place and angles are found.
+// A warp per row and share of its heads; nothing is shared between warps, so that the row's chain of
+// dependent loads (sequence, length, page) of one hides behind the copies of others. The warp forms
+// the row's rotary_dim / 2 angles once. tph lanes take a head, 8 dims each, as two runs of 4: of the
+// rotated dims lane j holds both halves' run j, so that a pair never leaves its lane, of the others 8
+// in a row (interleaved pairs: all dims 8 in a row). kAppendAhead heads a lane are in flight at once,
+// the first of them before the row's place is known.
+constexpr int kAppendAhead = 4;
 template <typename TI, typename TC>
 __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendArgs a) {
-  __shared__ float2 cs[128];
-  __shared__ RowPlace place;
-  const int t = blockIdx.x, tid = threadIdx.x;
+  __shared__ float2 cs_all[kAppendThreads / 32][128];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * (kAppendThreads / 32) + warp;
+  if (t >= a.b.rows) return;
+  float2* cs = cs_all[warp];
   const int D = a.c.head_dim, K = a.c.n_kv, heads = a.nh + 2 * K;
-  const int per = kAppendThreads / a.tph, grp = tid / a.tph, j = tid % a.tph;
+  const int per = 32 / a.tph, j = lane % a.tph;
   const bool dims = 8 * j < D, turns = 8 * j < a.rot;
   const int d0 = turns && !a.interleaved ? 4 * j : 8 * j;
   const int d1 = turns && !a.interleaved ? a.rot / 2 + 4 * j : 8 * j + 4;
-  auto fetch = [&](int slot, float (&x)[8]) {
-    const TI* src;
-    if (slot < a.nh) src = (const TI*)a.q + (int64_t)t * a.q_stride + slot * D;
-    else if (slot < a.nh + K) src = (const TI*)a.k + (int64_t)t * a.k_stride + (slot - a.nh) * D;
-    else src = (const TI*)a.v + (int64_t)t * a.v_stride + (slot - a.nh - K) * D;
-    load_n<TI, 4>(src + d0, x);
-    load_n<TI, 4>(src + d1, x + 4);
-  };
-  float next[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int step = per * gridDim.y;
-  int slot = blockIdx.y * per + grp;
-  if (slot < heads && dims) fetch(slot, next);
-
-  if (tid < 32) place_row(a, t, tid, &place);
-  __syncthreads();
+  int slot = blockIdx.y * per + lane / a.tph;
+  float x[kAppendAhead][8];
+  auto fetch = [&](int first) {
+#pragma unroll
+    for (int u = 0; u < kAppendAhead; ++u) {
+      const int h = first + u * step;
+      if (h >= heads || !dims) continue;
+      const TI* src;
+      if (h < a.nh) src = (const TI*)a.q + (int64_t)t * a.q_stride + h * D;
+      else if (h < a.nh + K) src = (const TI*)a.k + (int64_t)t * a.k_stride + (h - a.nh) * D;
+      else src = (const TI*)a.v + (int64_t)t * a.v_stride + (h - a.nh - K) * D;
+      load_n<TI, 4>(src + d0, x[u]);
+      load_n<TI, 4>(src + d1, x[u] + 4);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < kAppendAhead; ++u)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+  fetch(slot);
+  const RowPlace place = place_row(a, t, lane, blockIdx.y == 0);
   if (!place.in_batch) return;
-  if (tid < a.rot / 2) cs[tid] = rotation(place.pos, a.inv_freq[tid]);
-  __syncthreads();
+  for (int i = lane; i < a.rot / 2; i += 32) cs[i] = rotation(place.pos, a.inv_freq[i]);
+  __syncwarp();
   float2 r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) r[i] = turns ? cs[4 * j + i] : make_float2(1.f, 0.f);
 
-  for (int s0 = blockIdx.y * per; s0 < heads; s0 += step, slot += step) {
-    const bool live = slot < heads && dims;
-    float x[8];
+#pragma unroll 1
+  for (int s0 = blockIdx.y * per; s0 < heads; s0 += kAppendAhead * step, slot += kAppendAhead * step) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = next[i];
-    if (slot + step < heads && dims) fetch(slot + step, next);
-    const bool isq = slot < a.nh, isv = slot >= a.nh + K;
-    const float* w = isq ? a.q_norm : isv ? nullptr : a.k_norm;
-    if (a.q_norm || a.k_norm) {  // per-head RMSNorm; the sum of squares over the head's lanes
-      float ss = 0.f;
+    for (int u = 0; u < kAppendAhead; ++u) {
+      const int h = slot + u * step;
+      if (s0 + u * step >= heads) break;  // the same for the whole warp
+      const bool live = h < heads && dims, isq = h < a.nh, isv = h >= a.nh + K;
+      const float* w = isq ? a.q_norm : isv ? nullptr : a.k_norm;
+      if (a.q_norm || a.k_norm) {  // per-head RMSNorm; the sum of squares over the head's lanes
+        float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-      for (int o = a.tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (live && w) {
-        const float rms = sqrtf(ss / (float)D + a.eps);
-        const float4 w0 = *(const float4*)(w + d0), w1 = *(const float4*)(w + d1);
-        const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        for (int i = 0; i < 8; ++i) ss += x[u][i] * x[u][i];
+        for (int o = a.tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (live && w) {
+          const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
+          const float4 w0 = *(const float4*)(w + d0), w1 = *(const float4*)(w + d1);
+          const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] / rms * wv[i];
+          for (int i = 0; i < 8; ++i) x[u][i] = x[u][i] * inv * wv[i];
+        }
       }
-    }
-    if (!live) continue;
-    if (turns && !isv) {
+      if (turns && !isv) {
+        if (a.interleaved) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float& p = a.interleaved ? x[2 * i] : x[i];
-        float& q = a.interleaved ? x[2 * i + 1] : x[4 + i];
-        const float p0 = p, q0 = q;
-        p = p0 * r[i].x - q0 * r[i].y;
-        q = q0 * r[i].x + p0 * r[i].y;
+          for (int i = 0; i < 4; ++i) turn(x[u][2 * i], x[u][2 * i + 1], r[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) turn(x[u][i], x[u][4 + i], r[i]);
+        }
       }
+      if (!live) continue;
+      TC* dst;
+      if (isq) {
+        dst = (TC*)a.q_out + ((int64_t)t * a.nh + h) * D;
+      } else {
+        if (place.offset < 0) continue;
+        const int hk = isv ? h - a.nh - K : h - a.nh;
+        dst = (TC*)((isv ? a.c.v : a.c.k) + place.offset + (int64_t)hk * a.c.head_bytes);
+      }
+      store_n<TC, 4>(dst + d0, x[u]);
+      store_n<TC, 4>(dst + d1, x[u] + 4);
     }
-    TC* dst;
-    if (isq) {
-      dst = (TC*)a.q_out + ((int64_t)t * a.nh + slot) * D;
-    } else {
-      if (place.offset < 0) continue;
-      const int h = isv ? slot - a.nh - K : slot - a.nh;
-      dst = (TC*)((isv ? a.c.v : a.c.k) + place.offset + (int64_t)h * a.c.head_bytes);
-    }
-    store_n<TC, 4>(dst + d0, x);
-    store_n<TC, 4>(dst + d1, x + 4);
+    fetch(slot + kAppendAhead * step);
   }
 }
 
@@ -157,7 +174,10 @@ __global__ void __launch_bounds__(kAppendThreads) pp_append_any_kernel(const App
   __shared__ RowPlace place;
   const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int D = a.c.head_dim, K = a.c.n_kv, heads = a.nh + 2 * K;
-  if (warp == 0) place_row(a, t, lane, &place);
+  if (warp == 0) {
+    const RowPlace p = place_row(a, t, lane, blockIdx.y == 0);
+    if (lane == 0) place = p;
+  }
   __syncthreads();
   if (!place.in_batch) return;
   if (a.inv_freq && tid < a.rot / 2) cs[tid] = rotation(place.pos, a.inv_freq[tid]);
@@ -389,15 +409,19 @@ __global__ void __launch_bounds__(kReorderThreads) pp_beam_reorder_kernel(const 
 template <typename TI, typename TC>
 void launch_append(const AppendArgs& a, bool vec, int rows, cudaStream_t st, int sms) {
   const int heads = a.nh + 2 * a.c.n_kv;
-  const int per = vec ? kAppendThreads / a.tph : 8;
-  // Few rows: a row's heads over several CTAs, as long as that fills the SMs.
-  int y = (heads + per - 1) / per;
-  while (y > 1 && (int64_t)rows * y > 2 * (int64_t)sms) --y;
-  const dim3 grid(rows, y);
-  if (vec)
+  if (vec) {
+    // Few rows: a row's heads over several warps, one head a lane group at the least, as long as the
+    // warps do not pass eight an SM.
+    const int per = 32 / a.tph;
+    int y = (heads + per - 1) / per;
+    while (y > 1 && (int64_t)rows * y > 8 * (int64_t)sms) y = (y + 1) / 2;
+    const dim3 grid((rows + kAppendThreads / 32 - 1) / (kAppendThreads / 32), y);
     pp_append_kernel<TI, TC><<<grid, kAppendThreads, 0, st>>>(a);
-  else
-    pp_append_any_kernel<TI, TC><<<grid, kAppendThreads, 0, st>>>(a);
+    return;
+  }
+  int y = (heads + 7) / 8;
+  while (y > 1 && (int64_t)rows * y > 2 * (int64_t)sms) --y;
+  pp_append_any_kernel<TI, TC><<<dim3(rows, y), kAppendThreads, 0, st>>>(a);
 }
 template <typename TI>
 void launch_append_to(const AppendArgs& a, uint32_t cache, bool vec, int rows, cudaStream_t st,
