@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libpotpori_b200.so")
@@ -115,14 +114,6 @@ class TreeQuery(ctypes.Structure):
         ("q_stride", ctypes.c_int64), ("n_heads", ctypes.c_uint32), ("layer", ctypes.c_uint32),
         ("mask", ctypes.c_void_p), ("mask_words", ctypes.c_uint32), ("scale", ctypes.c_float)]
 
-
-# The descriptors that change with every call as struct formats (native alignment, so the
-# structures' own): packing one is several times quicker than filling a ctypes.Structure.
-PACK_BATCH = struct.Struct("@5I3P")
-PACK_APPEND = struct.Struct("@4P2I3q2P2I2PfI")
-PACK_QUERY = struct.Struct("@3Pq2IPIf")
-assert (PACK_BATCH.size, PACK_APPEND.size, PACK_QUERY.size) == tuple(
-    map(ctypes.sizeof, (PagedBatchDesc, AppendRows, TreeQuery)))
 
 _lib = None
 

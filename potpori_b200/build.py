@@ -1,4 +1,5 @@
-"""Compile the sm_100a CUDA library in-tree (potpori_b200/libpotpori_b200.so).
+"""Compile the sm_100a CUDA library in-tree (potpori_b200/libpotpori_b200.so) and its torch binding
+(potpori_b200/_paged.so).
 
 nvcc cross-compiles for sm_100a without a GPU. The CUDA runtime is linked statically so the
 library does not depend on which libcudart another package (torch) has loaded; the driver
@@ -19,8 +20,10 @@ LIB = os.path.join(HERE, "libpotpori_b200.so")
 SOURCES = [os.path.join(HERE, "csrc", f) for f in (
     "pp_shard.cu", "pp_static_gemv.cu", "pp_prefill.cu", "pp_paged_rows.cu", "pp_tree_attn.cu",
     "pp_tree_tc.cu", "pp_beam.cu")]
-DEPS = SOURCES + glob.glob(os.path.join(HERE, "csrc", "*.cuh")) + [
-    os.path.join(ROOT, "include", "potpori_b200.h")]
+HEADER = os.path.join(ROOT, "include", "potpori_b200.h")
+DEPS = SOURCES + glob.glob(os.path.join(HERE, "csrc", "*.cuh")) + [HEADER]
+BINDING = os.path.join(HERE, "_paged.so")
+BINDING_SOURCE = os.path.join(HERE, "csrc", "pp_torch.cpp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -37,16 +40,39 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def stale() -> bool:
-    if not os.path.exists(LIB):
+def stale(target: str = LIB, deps: list = DEPS) -> bool:
+    if not os.path.exists(target):
         return True
-    t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(p) > t for p in DEPS)
+    t = os.path.getmtime(target)
+    return any(os.path.getmtime(p) > t for p in deps)
+
+
+def build_binding() -> None:
+    """potpori_b200/_paged.so: the paged operators' torch binding, linked to the library beside it."""
+    import sysconfig
+
+    from torch.utils import cpp_extension
+
+    cxx = next((c for c in ("/usr/bin/g++", shutil.which("g++")) if c and os.path.exists(c)), "c++")
+    torch_lib = cpp_extension.library_paths()[0]
+    includes = cpp_extension.include_paths() + ["/usr/local/cuda/include", sysconfig.get_paths()["include"]]
+    subprocess.run(
+        [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", BINDING_SOURCE, "-o", BINDING + ".tmp",
+         *(f"-isystem{p}" for p in includes), f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+         "-ltorch_python", f"-L{HERE}", "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
+         f"-Wl,-rpath,{torch_lib}"], check=True)
+    os.replace(BINDING + ".tmp", BINDING)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not stale():
-        return LIB
+    if force or stale():
+        build_library(verbose)
+    if force or stale(BINDING, [BINDING_SOURCE, HEADER]):
+        build_binding()
+    return LIB
+
+
+def build_library(verbose: bool = False) -> None:
     env = dict(os.environ)
     env.pop("CC", None)  # the image's CC points at a gcc without the host runtime nvcc wants
     verb = ["-Xptxas=-v"] if verbose else []
@@ -58,7 +84,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
         subprocess.run([nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB + ".tmp", *objects], check=True,
                        env=env)
     os.replace(LIB + ".tmp", LIB)
-    return LIB
 
 
 if __name__ == "__main__":
