@@ -14,8 +14,16 @@ namespace pp {
 // ---- 16-bit caches, few query vectors --------------------------------------------------------
 constexpr int kTreeThreads = 128;
 constexpr int kTreeBN = 64;
-constexpr int kTreeWholeTiles = 4;
-constexpr uint64_t kTreeTcAbove = 8;  // more query vectors of a head than this: pp_tree_tc.cu
+// Caches of up to so many tiles are not cut: cutting a unit costs the join, 3 us of a call, and a
+// tile of the narrow, tcgen05 and F32 kernels takes about 0.5, 1.2 and 2 us in a lone CTA (8 heads: 256
+// positions narrow 8.2 us whole; 128 positions F32 8.2 us cut, 6.8 whole; 512 positions tcgen05 14.4
+// us cut, 20.3 whole).
+constexpr int kWholeNarrow = 8, kWholeTc = 2, kWholeF32 = 2;
+// More than 8 query vectors a head, the narrow kernel takes in tiles of 8, reading K and V again for
+// each from L2; it starts faster and its tiles are quicker, so it still leads up to this many of its
+// tiles a CTA (32 vectors, 8 heads: 2056 positions 17.2 us against tcgen05's 19.5, 8200 positions 27.5
+// against 29.3, 8 x 2056 34.5 against 32.0, 32 x 2056 106 against 62).
+constexpr uint64_t kNarrowTiles = 16;
 
 template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -454,7 +462,7 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
       float x[RW][2];
 #pragma unroll
       for (int r = 0; r < RW; ++r) x[r][0] = x[r][1] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
       for (int d = 0; d < D; d += 4) {
         const float4 k = *(const float4*)(kt + d);
 #pragma unroll
@@ -510,17 +518,21 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
         for (int r = 0; r < BM; ++r) acc[d][r] *= al_s[r];
         // A V that a row does not see must not count for it even where it is not finite (0 * NaN):
         // such a value is added for the rows that see it and leaves the tile.
-        if (tree)
+        if (tree && (a.mask || s.n > 1)) {
+          float* column = (float*)vt + dim;
+          uint32_t odd = 0;
+#pragma unroll 8
+          for (int k = 0; k < BN; ++k) odd |= (uint32_t)!isfinite(column[k * P]) << k;
 #pragma unroll 1
-          for (int k = 0; k < BN; ++k) {
-            float* at = (float*)vt + k * P + dim;
-            const float odd = *at;
-            if (isfinite(odd)) continue;
+          for (; odd; odd &= odd - 1) {
+            const int k = __ffs(odd) - 1;
+            const float v1 = column[k * P];
 #pragma unroll
             for (int r = 0; r < BM; ++r)
-              if (vis_s[r] >> k & 1u) acc[d][r] += pt[k * PP + r] * odd;
-            *at = 0.f;
+              if (vis_s[r] >> k & 1u) acc[d][r] += pt[k * PP + r] * v1;
+            column[k * P] = 0.f;
           }
+        }
 #pragma unroll 8
         for (int k = 0; k < BN; ++k) {
           const float v1 = vt[k * P + dim];
@@ -583,20 +595,21 @@ inline TreePlan tree_plan(const pp_paged_cache& c, const pp_paged_batch& b, uint
   TreePlan p;
   p.dp = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
   const uint64_t G = n_heads / c.n_kv_heads, vectors = (uint64_t)(b.max_rows ? b.max_rows : 1) * G;
-  p.tc = c.dtype != PP_F32 && vectors > kTreeTcAbove;
   uint64_t per_sm = 2;
+  p.tc = false;
   if (c.dtype == PP_F32) {
     p.bm = vectors <= 4 ? 4 : 16;
     p.bn = kTreeFBN;
     per_sm = p.dp == 64 ? 5 : p.dp == 128 ? 3 : 1;
   } else {
+    if (p.dp == 256) per_sm = 1;
+    const uint64_t tiles8 = (vectors + 7) / 8 * b.batch * c.n_kv_heads * (((uint64_t)b.max_len + kTreeBN - 1) / kTreeBN);
+    p.tc = vectors > 8 && tiles8 > kNarrowTiles * per_sm * sms;
     p.bm = p.tc ? 128 : 8;
     p.bn = kTreeBN;
-    if (p.dp == 256) per_sm = 1;
   }
   const uint64_t units = ((uint64_t)b.rows * G / p.bm + b.batch) * c.n_kv_heads;
-  // A cache of a few tiles is not worth the second kernel.
-  p.whole = b.max_len <= (uint32_t)kTreeWholeTiles * p.bn;
+  p.whole = b.max_len <= (uint32_t)p.bn * (c.dtype == PP_F32 ? kWholeF32 : p.tc ? kWholeTc : kWholeNarrow);
   const uint64_t tiles = units * (p.whole ? 1 : ((uint64_t)b.max_len + p.bn - 1) / p.bn + 1);
   const uint64_t most = (uint64_t)sms * per_sm;
   p.ctas = (int)(tiles < most ? (tiles ? tiles : 1) : most);

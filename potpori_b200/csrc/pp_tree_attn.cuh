@@ -51,6 +51,17 @@ template <int BM, int BN, int NT>
 __device__ __forceinline__ void tile_prefix(const TreeArgs& a, uint32_t* prefix, uint32_t* scan,
                                             bool report) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.b.batch;
+  if (B == 1) {  // the usual decode: no scan
+    if (tid == 0) {
+      const int n = a.b.cu_rows[1] - a.b.cu_rows[0], len = a.b.kv_len[0];
+      const bool bad = bad_sequence(a, n, len);
+      if (bad && report && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
+      prefix[0] = 0;
+      prefix[1] = bad || n == 0 ? 0u : ((uint32_t)n * a.G + BM - 1) / BM * a.c.n_kv * (a.whole ? 1 : (len + BN - 1) / BN);
+    }
+    __syncthreads();
+    return;
+  }
   const int each = (B + NT - 1) / NT, b0 = min(B, tid * each), b1 = min(B, b0 + each);
   uint32_t sum = 0;
   for (int b = b0; b < b1; ++b) {

@@ -22,7 +22,12 @@ def rng_of(seed):
     return torch.Generator().manual_seed(seed)
 
 
-def make(rng, lengths, rows, page, heads, dim, dtype, layout="nhd", layers=0, spare=0):
+# The host's bound on the lengths chooses the kernel for 16-bit caches: the true one leaves these small
+# calls to the narrow kernel, a far one sends more than 8 query vectors a head to the tcgen05 kernel.
+FAR = 1 << 20
+
+
+def make(rng, lengths, rows, page, heads, dim, dtype, layout="nhd", layers=0, spare=0, bound=None):
     from potpori_b200.paged import PagedBatch, PagedCache
 
     pages = sum(-(-n // page) for n in lengths) + 2 + spare
@@ -31,7 +36,7 @@ def make(rng, lengths, rows, page, heads, dim, dtype, layout="nhd", layers=0, sp
     v = ref.make_pool(rng, pages, page, heads, dim, dtype, layout, layers)
     cache = PagedCache(k, v, layout)
     batch = PagedBatch(table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), ref.offsets(rows).cuda(),
-                       max_rows=max(rows), max_length=max(lengths))
+                       max_rows=max(rows), max_length=bound or max(lengths))
     return cache, batch, table
 
 
@@ -191,11 +196,12 @@ def check_attention(cache, table, layout, page, rows, lengths, seen, q, got, lse
         t += n
 
 
+@pytest.mark.parametrize("bound", [None, FAR])
 @pytest.mark.parametrize("case", range(len(TREE)))
-def test_tree_attention(gpu, case):
+def test_tree_attention(gpu, case, bound):
     dt, layout, page, K, H, D, rows, lengths, masked = TREE[case]
     rng = rng_of(100 + case)
-    cache, batch, table = make(rng, lengths, rows, page, K, D, dt, layout)
+    cache, batch, table = make(rng, lengths, rows, page, K, D, dt, layout, bound=bound)
     T, pad = sum(rows), 3
     q = (2 * torch.randn(T + pad, H, D, generator=rng)).to(dt).cuda()
     parents = [ref.random_parents(rng, n) if masked else [i - 1 for i in range(n)] for n in rows]
@@ -213,13 +219,15 @@ def test_tree_attention(gpu, case):
     assert torch.equal(cache.tree_attention(batch, q, mask=mask)[:T], got[:T])
 
 
+@pytest.mark.parametrize("bound", [None, FAR])
 @pytest.mark.parametrize("dt", [F32, BF16, F16])
 @pytest.mark.parametrize("heads", [2, 16])
-def test_tree_attention_masks(gpu, dt, heads):
+@pytest.mark.parametrize("page", [16, 24])
+def test_tree_attention_masks(gpu, dt, heads, bound, page):
     """Rows that see nothing, only the context, only others, every node; nodes past the mask."""
     rng = rng_of(7)
-    rows, lengths, page = [6, 40, 3], [6, 90, 200], 16
-    cache, batch, table = make(rng, lengths, rows, page, 2, 128, dt)
+    rows, lengths = [6, 40, 3], [6, 90, 200]
+    cache, batch, table = make(rng, lengths, rows, page, 2, 128, dt, bound=bound)
     T = sum(rows)
     nodes = [[int(j) for j in range(n) if torch.rand(1, generator=rng) < 0.3] for n in rows for _ in range(n)]
     nodes[0] = []            # no context either: an empty row
@@ -247,14 +255,16 @@ def test_tree_attention_masks(gpu, dt, heads):
     assert (got[0] == 0).all() and (lse[0] == -math.inf).all()
 
 
+@pytest.mark.parametrize("bound", [None, FAR])
 @pytest.mark.parametrize("dt", [F32, BF16, F16])
 @pytest.mark.parametrize("heads", [2, 8])
-@pytest.mark.parametrize("bad", [math.nan, math.inf])
-def test_tree_attention_nonfinite_where_unseen(gpu, dt, heads, bad):
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("page", [16, 24])
+def test_tree_attention_nonfinite_where_unseen(gpu, dt, heads, bad, bound, page):
     """Behind a sequence's last position, in pages of nobody, and in K and V of unseen nodes."""
     rng = rng_of(8)
-    rows, lengths, page = [12, 5], [70, 131], 16
-    cache, batch, table = make(rng, lengths, rows, page, 2, 128, dt)
+    rows, lengths = [12, 5], [70, 131]
+    cache, batch, table = make(rng, lengths, rows, page, 2, 128, dt, bound=bound)
     q = torch.randn(17, heads, 128, generator=rng).to(dt).cuda()
     parents = [ref.random_parents(rng, n) for n in rows]
     seen = [ref.tree_seen(p, lengths[b] - rows[b]) for b, p in enumerate(parents)]
@@ -287,16 +297,16 @@ def test_tree_attention_nonfinite_where_unseen(gpu, dt, heads, bad):
     assert torch.equal(got[blind.cuda()], want[blind.cuda()])
 
 
-@pytest.mark.parametrize("dt", [F32, BF16])
-def test_tree_attention_score_ranges(gpu, dt):
+@pytest.mark.parametrize("dt,heads,bound", [(F32, 1, None), (F32, 9, None), (BF16, 1, None), (BF16, 9, FAR)])
+def test_tree_attention_score_ranges(gpu, dt, heads, bound):
     """Scores far from zero: all very negative, one that takes all, and equal ones."""
     rng = rng_of(9)
-    cache, batch, table = make(rng, [150], [2], 16, 1, 64, dt)
+    cache, batch, table = make(rng, [150], [2], 16, 1, 64, dt, bound=bound)
     cache.k.zero_()
     cache.k[..., 0] = -200.0
     index = int(table[0, 3])
     cache.k[index, 5, 0, 0] = 200.0
-    q = torch.zeros(2, 1, 64, dtype=dt, device="cuda")
+    q = torch.zeros(2, heads, 64, dtype=dt, device="cuda")
     q[0, 0, 0], q[1, 0, 0] = 40.0, 1.0
     got = cache.tree_attention(batch, q, scale=1.0)
     assert torch.equal(got[0, 0], cache.v[index, 5, 0])
@@ -305,28 +315,52 @@ def test_tree_attention_score_ranges(gpu, dt):
     got = cache.tree_attention(batch, q)
     tol = 150 * 2.0 ** -24 + 2.0 ** -15 * v.abs().max()
     assert ((got[1, 0].cpu().double() - v.mean(0)).abs() <= tol + v.mean(0).abs() * EPS[dt]).all()
+    # Scores that rise by more than the kernels let pass without rescaling, tile after tile.
+    for j in range(150):
+        cache.k[int(table[0, j // 16]), j % 16, 0, 0] = j / 2.0
+    q[:, :, 0] = 1.0
+    got = cache.tree_attention(batch, q, scale=1.0)
+    seen = ref.tree_seen([-1, 0], 148)
+    want, _, most = ref.attention(q.cpu().double(), ref.cached(cache.k, "nhd", table, 0, 150, 16), v[:, None], seen, 1.0)
+    assert ((got.cpu().double() - want).abs() <= attention_tolerance(dt, want, most, 150, 64, v.abs().max())).all()
 
 
-def test_tree_attention_bad_descriptors(gpu):
+@pytest.mark.parametrize("dt,heads,bound", [(F32, 2, None), (BF16, 2, None), (F16, 16, None), (F16, 16, FAR)])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-3])
+def test_tree_attention_scales(gpu, dt, heads, bound, scale):
+    """Any scale, its sign and zero among them."""
+    rng = rng_of(15)
+    rows, lengths, page = [5, 3], [140, 3], 16
+    cache, batch, table = make(rng, lengths, rows, page, 2, 128, dt, bound=bound)
+    q = (2 * torch.randn(8, heads, 128, generator=rng)).to(dt).cuda()
+    lse = torch.empty(8, heads, device="cuda")
+    seen = [ref.tree_seen([i - 1 for i in range(n)], lengths[b] - n) for b, n in enumerate(rows)]
+    got = cache.tree_attention(batch, q, lse=lse, scale=scale)
+    check_attention(cache, table, "nhd", page, rows, lengths, seen, q, got, lse, scale)
+
+
+@pytest.mark.parametrize("dt,heads,bound,page", [(BF16, 4, 40, 16), (BF16, 4, 40, 8), (BF16, 10, FAR, 16), (F16, 10, FAR, 8),
+                                                 (F32, 4, 40, 16)])
+def test_tree_attention_bad_descriptors(gpu, dt, heads, bound, page):
     """A sequence whose lengths do not fit is left out, a bad page contributes nothing it could
     fault on, the rest of the batch is right."""
     from potpori_b200.paged import PagedBatch
 
     rng = rng_of(10)
-    cache, batch, table = make(rng, [40, 40, 40], [2, 2, 2], 16, 2, 128, BF16)
-    q = torch.randn(6, 4, 128, generator=rng).bfloat16().cuda()
+    cache, batch, table = make(rng, [40, 40, 40], [2, 2, 2], page, 2, 128, dt, bound=bound)
+    q = torch.randn(6, heads, 128, generator=rng).to(dt).cuda()
     want = cache.tree_attention(batch, q)
     for lengths in ([40, 49, 40], [40, 1, 40], [40, -3, 40]):
         out = torch.full_like(q, 7.0)
-        b = PagedBatch(batch.page_table, torch.tensor(lengths, dtype=torch.int32).cuda(), batch.cu_rows, 2, 40)
+        b = PagedBatch(batch.page_table, torch.tensor(lengths, dtype=torch.int32).cuda(), batch.cu_rows, 2, bound)
         cache.tree_attention(b, q, out=out)
         with pytest.raises(PPError):
             cache.check()
         assert torch.equal(out[:2], want[:2]) and torch.equal(out[4:], want[4:]) and (out[2:4] == 7.0).all()
-    for page in (-1, cache.pages, 2 ** 30):
+    for bad in (-1, cache.pages, 2 ** 30):
         t = table.clone()
-        t[1, 1] = page
-        got = cache.tree_attention(PagedBatch(t.cuda(), batch.lengths, batch.cu_rows, 2, 40), q)
+        t[1, 1] = bad
+        got = cache.tree_attention(PagedBatch(t.cuda(), batch.lengths, batch.cu_rows, 2, bound), q)
         with pytest.raises(PPError):
             cache.check()
         assert torch.equal(got[:2], want[:2]) and torch.equal(got[4:], want[4:])
@@ -365,12 +399,14 @@ def test_tree_attention_far_offsets(gpu, dt):
     k, v = (torch.randn(41, K, D, generator=rng).to(dt).cuda() for _ in range(2))
     cache.append(batch, k, v)
     q = torch.randn(41, 4, D, generator=rng).to(dt).cuda()
-    got = cache.tree_attention(batch, q)
-    cache.check()
     seen = ref.tree_seen([i - 1 for i in range(41)], 0)
     want, _, most = ref.attention(q.cpu().double(), k.cpu().double(), v.cpu().double(), seen, D ** -0.5)
     tol = attention_tolerance(dt, want, most, 41, D, v.abs().max().cpu())
-    assert ((got.cpu().double() - want).abs() <= tol).all()
+    for bound in (41, FAR):
+        b = PagedBatch(batch.page_table, batch.lengths, batch.cu_rows, 41, bound)
+        got = cache.tree_attention(b, q)
+        cache.check()
+        assert ((got.cpu().double() - want).abs() <= tol).all()
 
 
 @pytest.mark.parametrize("dt,G", [(BF16, 1), (BF16, 8), (F16, 4), (F32, 2)])
