@@ -110,8 +110,7 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
   const bool tma = maps.box != 0;
   uint8_t* ring = sm + warp * NS * C::kStage;  // the warp's
   uint64_t* bar = full + warp * NS;
-  if (smem_u32(sm) & 1023u) {  // cannot be: no join, and the caller is told
-    if (tid == 0) write_join<BM>(a, nullptr, 1);
+  if (smem_u32(sm) & 1023u) {  // cannot be; the caller is told
     if (tid == 0 && a.err) atomicOr(a.err, PAGED_TIMEOUT);
     return;
   }
@@ -120,17 +119,15 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
     fence_barrier_init();
   }
   pdl_launch_dependents();
-  tile_prefix<BM, BN, kTreeThreads>(a, prefix, scan, blockIdx.x == 0);
+  tile_prefix<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, scan, blockIdx.x == 0);
   const uint32_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
   uint32_t begin, end;
   cta_range(per, total, blockIdx.x, begin, end);
-  if (begin >= end && tid == 0) write_join<BM>(a, nullptr, per);
   RingCursor use;  // the stage of the next tile to consume
   bool ok = true;
 
   for (uint32_t w = begin; w < end;) {
-    const Segment s = segment_at<BM, BN>(a, prefix, w, end);
-    if (w == begin && tid == 0) write_join<BM>(a, &s, per);
+    const Segment s = segment_at<BN>(a, prefix, w, end);
     const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
     RowFetch<16> rows;
     BoxPlace box;
@@ -397,15 +394,13 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.c.head_dim;
 
   pdl_launch_dependents();
-  tile_prefix<BM, BN, kTreeThreads>(a, prefix, scan, blockIdx.x == 0);
+  tile_prefix<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, scan, blockIdx.x == 0);
   const uint32_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
   uint32_t begin, end;
   cta_range(per, total, blockIdx.x, begin, end);
-  if (begin >= end && tid == 0) write_join<BM>(a, nullptr, per);
 
   for (uint32_t w = begin; w < end;) {
-    const Segment s = segment_at<BM, BN>(a, prefix, w, end);
-    if (w == begin && tid == 0) write_join<BM>(a, &s, per);
+    const Segment s = segment_at<BN>(a, prefix, w, end);
     const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
     const int NR = s.n * a.G;
     RowFetch<8> ahead;  // a warp fetches 8 rows of every tile
@@ -613,7 +608,7 @@ inline TreePlan tree_plan(const pp_paged_cache& c, const pp_paged_batch& b, uint
   const uint64_t tiles = units * (p.whole ? 1 : ((uint64_t)b.max_len + p.bn - 1) / p.bn + 1);
   const uint64_t most = (uint64_t)sms * per_sm;
   p.ctas = (int)(tiles < most ? (tiles ? tiles : 1) : most);
-  p.work = 2ull * p.ctas * p.bm * (p.dp + 2) * 4 + (uint64_t)p.ctas * sizeof(JoinRec);
+  p.work = 2ull * p.ctas * p.bm * (p.dp + 2) * 4;
   return p;
 }
 
@@ -759,7 +754,6 @@ extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_pag
   a.bm = p.bm;
   a.part = (float*)work;
   a.part_ml = (float2*)(a.part + 2ll * p.ctas * p.bm * p.dp);
-  a.recs = (JoinRec*)(a.part_ml + 2ll * p.ctas * p.bm);
   a.ctas = p.ctas;
   a.whole = p.whole;
   a.dev = cache->cuda_device;

@@ -16,8 +16,6 @@
 
 namespace pp {
 
-struct JoinRec;
-
 struct TreeArgs {
   PagedView c;  // the layer
   BatchView b;
@@ -31,7 +29,6 @@ struct TreeArgs {
   float scale;
   float* part;      // [2 * ctas][BM][DP] outputs
   float2* part_ml;  // [2 * ctas][BM] (max, sum)
-  JoinRec* recs;  // [ctas]
   int32_t ctas;     // CTAs that the line of tiles is cut over
   int32_t bm;       // rows of a tile
   int32_t whole;    // units are not cut (short caches): no partials, no join
@@ -45,10 +42,9 @@ __device__ __forceinline__ bool bad_sequence(const TreeArgs& a, int n, int len) 
 }
 
 // prefix[b] = tiles (units, where they are not cut) before sequence b on the line; prefix[batch] =
-// all. By the whole CTA
-// (NT threads), scan: NT / 32 words of shared memory.
-template <int BM, int BN, int NT>
-__device__ __forceinline__ void tile_prefix(const TreeArgs& a, uint32_t* prefix, uint32_t* scan,
+// all. By the whole CTA (NT threads); a tile has 1 << bm_log rows; scan: NT / 32 words of shared memory.
+template <int BN, int NT>
+__device__ __forceinline__ void tile_prefix(const TreeArgs& a, int bm_log, uint32_t* prefix, uint32_t* scan,
                                             bool report) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.b.batch;
   if (B == 1) {  // the usual decode: no scan
@@ -57,7 +53,7 @@ __device__ __forceinline__ void tile_prefix(const TreeArgs& a, uint32_t* prefix,
       const bool bad = bad_sequence(a, n, len);
       if (bad && report && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
       prefix[0] = 0;
-      prefix[1] = bad || n == 0 ? 0u : ((uint32_t)n * a.G + BM - 1) / BM * a.c.n_kv * (a.whole ? 1 : (len + BN - 1) / BN);
+      prefix[1] = bad || n == 0 ? 0u : ((((uint32_t)n * a.G - 1) >> bm_log) + 1) * a.c.n_kv * (a.whole ? 1 : (len + BN - 1) / BN);
     }
     __syncthreads();
     return;
@@ -70,7 +66,7 @@ __device__ __forceinline__ void tile_prefix(const TreeArgs& a, uint32_t* prefix,
     if (bad_sequence(a, n, len)) {
       if (report && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
     } else if (n > 0) {
-      const uint32_t rts = ((uint32_t)n * a.G + BM - 1) / BM;  // BM is a power of two
+      const uint32_t rts = (((uint32_t)n * a.G - 1) >> bm_log) + 1;
       sum += rts * a.c.n_kv * (a.whole ? 1 : (len + BN - 1) / BN);
     }
   }
@@ -97,7 +93,7 @@ struct Segment {
   uint32_t unit0;             // place of the unit's first tile on the line
   uint32_t step;              // places on the line that the segment takes
 };
-template <int BM, int BN>
+template <int BN>
 __device__ __forceinline__ Segment segment_at(const TreeArgs& a, const uint32_t* prefix, uint32_t w,
                                               uint32_t end) {
   int lo = 0, hi = a.b.batch;  // last b with prefix[b] <= w: the one with tiles, as w < prefix[b + 1]
@@ -130,31 +126,6 @@ __device__ __forceinline__ void cta_range(uint32_t per, uint32_t total, uint32_t
                                           uint32_t& end) {
   begin = min((uint64_t)cta * per, (uint64_t)total);
   end = min(begin + per, total);
-}
-
-// What the join has to know of a unit whose last tile this CTA took and whose first one it did
-// not; parts = 0 for a CTA without such a unit. Only a CTA's first segment can be one.
-struct JoinRec {
-  int32_t parts, rows;      // partials, rows of the tile
-  int32_t first_slot, cta;  // slot of the first partial; the others are 2 * (cta + p)
-  int32_t row0, vec0, head0, see;  // first array row, vector of row 0, first head; n << 1 | (ctx > 0)
-};
-template <int BM>
-__device__ __forceinline__ void write_join(const TreeArgs& a, const Segment* s, uint32_t per) {
-  if (a.whole) return;
-  JoinRec r = {};
-  if (s && s->t0 > 0 && s->t1 == s->tiles) {
-    const uint32_t c0 = s->unit0 / per;
-    r.parts = (int)(blockIdx.x - c0) + 1;
-    r.rows = min(BM, s->n * a.G - s->rt * BM);
-    r.first_slot = (int)(c0 * per == s->unit0 ? 2 * c0 : 2 * c0 + 1);
-    r.cta = (int)c0;
-    r.row0 = s->row0;
-    r.vec0 = s->rt * BM;
-    r.head0 = s->h * a.G;
-    r.see = s->n << 1 | (s->ctx > 0);
-  }
-  a.recs[blockIdx.x] = r;
 }
 
 // Whether row (sequence row i) sees node j (0 <= j < n).
@@ -334,28 +305,60 @@ __device__ __forceinline__ void add_nonfinite(const TreeArgs& a, const Segment& 
   }
 }
 
-// Joins the partials of the units that the line was cut in. Items are spread over a grid of any
+// Joins the partials of the units that the line was cut in. A CTA of the attention whose first
+// segment ends a unit that it did not begin stands for that unit. Items are spread over a grid of any
 // size; 16 lanes take a row, DP / 16 dims each: of a unit with few partials an item is 8 rows, of one
-// with many a row, its partials dealt to the 8 groups. The kernel runs once through its code, which
-// therefore is kept short: fetching instructions is most of its time.
+// with many a row, its partials dealt to the 8 groups. What the units are follows from the lengths
+// alone, so it is found while the attention's last CTAs still run: only the partials are waited for,
+// and read once, with a running maximum.
 constexpr int kJoinMany = 8;
+struct JoinUnit {
+  int32_t parts, rows;  // partials (0: no unit), rows of the tile
+  int32_t first_slot, cta;  // slot of the first partial; the others are 2 * (cta + p)
+  int32_t row0, vec0, head0, n, ctx;  // first array row, vector of row 0, first head, nodes, context
+};
+template <int BN>
+__device__ __forceinline__ JoinUnit join_unit(const TreeArgs& a, int bm_log, const uint32_t* prefix, uint32_t per,
+                                              uint32_t total, uint32_t cta) {
+  JoinUnit u = {};
+  uint32_t begin, end;
+  cta_range(per, total, cta, begin, end);
+  if (begin >= end) return u;
+  const Segment s = segment_at<BN>(a, prefix, begin, end);
+  if (s.t0 == 0 || s.t1 < s.tiles) return u;
+  const uint32_t c0 = s.unit0 / per;
+  u.parts = (int)(cta - c0) + 1;
+  u.vec0 = s.rt << bm_log;
+  u.rows = min(1 << bm_log, s.n * a.G - u.vec0);
+  u.first_slot = (int)(c0 * per == s.unit0 ? 2 * c0 : 2 * c0 + 1);
+  u.cta = (int)c0;
+  u.row0 = s.row0;
+  u.head0 = s.h * a.G;
+  u.n = s.n;
+  u.ctx = s.ctx;
+  return u;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
-  extern __shared__ uint32_t s_items[];  // [ctas + 1] prefix of items
+  constexpr int V = DP / 16, BN = sizeof(T) == 4 ? 32 : 64;  // the attention's key tile
+  extern __shared__ uint32_t s_items[];  // [ctas + 1] items before each CTA's unit, then [batch + 1]
   __shared__ uint32_t scan[4];
   __shared__ float s_acc[8][DP];
-  __shared__ float s_l[8];
-  constexpr int V = DP / 16;
+  __shared__ float2 s_ml[8];
+  uint32_t* prefix = s_items + a.ctas + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = tid >> 4, l16 = tid & 15;
   const int each = (a.ctas + 127) / 128, c0 = min(a.ctas, tid * each), c1 = min(a.ctas, c0 + each);
-  pdl_wait();
+  const int bm_log = 31 - __clz(a.bm);
+  tile_prefix<BN, 128>(a, bm_log, prefix, scan, false);
+  const uint32_t places = prefix[a.b.batch], per = tiles_per_cta(a, places);
   {
     uint32_t sum = 0;
 #pragma unroll 1
     for (int c = c0; c < c1; ++c) {
-      const int2 pr = __ldcg((const int2*)&a.recs[c]);  // parts, rows
+      const JoinUnit u = join_unit<BN>(a, bm_log, prefix, per, places, c);
       s_items[c] = sum;
-      if (pr.x > 0) sum += pr.x > kJoinMany ? pr.y : (pr.y + 7) / 8;
+      if (u.parts > 0) sum += u.parts > kJoinMany ? u.rows : (u.rows + 7) / 8;
     }
     uint32_t inc = sum;
 #pragma unroll
@@ -374,34 +377,45 @@ __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
     __syncthreads();
   }
   const uint32_t total = s_items[a.ctas];
+  bool waited = false;
 #pragma unroll 1
-  for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
-    int lo = 0, hi = a.ctas;
+  for (uint32_t item = blockIdx.x;; item += gridDim.x) {
+    JoinUnit u = {};
+    int at = 0;
+    if (item < total) {
+      int lo = 0, hi = a.ctas;
 #pragma unroll 1
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_items[mid] <= item) lo = mid;
-      else hi = mid;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (s_items[mid] <= item) lo = mid;
+        else hi = mid;
+      }
+      u = join_unit<BN>(a, bm_log, prefix, per, places, lo);
+      at = (int)(item - s_items[lo]);
     }
-    const JoinRec rec = a.recs[lo];
-    const bool many = rec.parts > kJoinMany;
-    const int at = (int)(item - s_items[lo]), r = many ? at : at * 8 + grp;
-    const bool live = r < rec.rows;
-    const int parts = live ? rec.parts : 0;
-    auto slot = [&](int p) { return (int64_t)(p == 0 ? rec.first_slot : 2 * (rec.cta + p)) * a.bm + r; };
-    float mx = -INFINITY;
-#pragma unroll 2
-    for (int p = l16; p < parts; p += 16) mx = fmaxf(mx, __ldcg(&a.part_ml[slot(p)]).x);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float base = mx == -INFINITY ? 0.f : mx;
-    float acc[V], l = 0.f;
+    if (!waited) pdl_wait();  // by every CTA: the stream goes on when all of this grid's have ended
+    waited = true;
+    if (item >= total) break;
+    const bool many = u.parts > kJoinMany;
+    const int r = many ? at : at * 8 + grp;
+    const bool live = r < u.rows;
+    const int parts = live ? u.parts : 0;
+    float acc[V], m = -INFINITY, l = 0.f;
 #pragma unroll
     for (int d = 0; d < V; ++d) acc[d] = 0.f;
+    auto add = [&](float pm, float pl, const float* x) {  // one more partial, in order
+      const float mx = fmaxf(m, pm), base = mx == -INFINITY ? 0.f : mx;
+      const float fa = soft_exp<T>(m - base), fp = soft_exp<T>(pm - base);
+      m = mx;
+      l = l * fa + pl * fp;
+#pragma unroll
+      for (int d = 0; d < V; ++d) acc[d] = acc[d] * fa + x[d] * fp;
+    };
 #pragma unroll 4
     for (int p = many ? grp : 0; p < parts; p += many ? 8 : 1) {
-      const float2 ml = __ldcg(&a.part_ml[slot(p)]);
-      const float* o = a.part + slot(p) * DP + V * l16;
+      const int64_t slot = (int64_t)(p == 0 ? u.first_slot : 2 * (u.cta + p)) * a.bm + r;
+      const float2 ml = __ldcg(&a.part_ml[slot]);
+      const float* o = a.part + slot * DP + V * l16;
       float x[V];
 #pragma unroll
       for (int d = 0; d < V; d += 4) {
@@ -411,29 +425,22 @@ __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
         x[d + 2] = v.z;
         x[d + 3] = v.w;
       }
-      const float f = soft_exp<T>(ml.x - base);
-      l += ml.y * f;
-#pragma unroll
-      for (int d = 0; d < V; ++d) acc[d] += x[d] * f;
+      add(ml.x, ml.y, x);
     }
     if (many) {  // the groups' shares, in order
 #pragma unroll
       for (int d = 0; d < V; ++d) s_acc[grp][V * l16 + d] = acc[d];
-      if (l16 == 0) s_l[grp] = l;
+      if (l16 == 0) s_ml[grp] = make_float2(m, l);
       __syncthreads();
       if (grp == 0) {
 #pragma unroll 1
-        for (int g = 1; g < 8; ++g) {
-          l += s_l[g];
-#pragma unroll
-          for (int d = 0; d < V; ++d) acc[d] += s_acc[g][V * l16 + d];
-        }
+        for (int g = 1; g < 8; ++g) add(s_ml[g].x, s_ml[g].y, &s_acc[g][V * l16]);
       }
       __syncthreads();
     }
     if (!live || (many && grp > 0)) continue;
-    const int R = rec.vec0 + r, i = (int)a.by_g.div((uint32_t)R), row = rec.row0 + i, head = rec.head0 + (R - i * a.G);
-    const bool empty = l == 0.f && !sees_any(a, row, rec.see >> 1, rec.see & 1);
+    const int R = u.vec0 + r, i = (int)a.by_g.div((uint32_t)R), row = u.row0 + i, head = u.head0 + (R - i * a.G);
+    const bool empty = l == 0.f && !sees_any(a, row, u.n, u.ctx);
     const float inv = 1.f / l;
 #pragma unroll
     for (int d = 0; d < V; ++d) acc[d] = empty ? 0.f : acc[d] * inv;
@@ -445,7 +452,7 @@ __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
       for (int d = 0; d < V; d += 8)
         if (V * l16 + d < a.c.head_dim) store_n<T, 8>(out + d, acc + d);
     }
-    if (a.lse && l16 == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(mx, l);
+    if (a.lse && l16 == 0) a.lse[(int64_t)row * a.nh + head] = empty ? -INFINITY : soft_lse<T>(m, l);
   }
 }
 

@@ -20,7 +20,7 @@ pp_status launch_join(const TreeArgs& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(items < 148 * 8 ? items : 148 * 8);
   cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = 4 * (size_t)(a.ctas + 1);
+  cfg.dynamicSmemBytes = 4 * (size_t)(a.ctas + 1 + a.b.batch + 1);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -164,8 +164,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
   uint32_t* prefix = (uint32_t*)((uint8_t*)bars + C::kBars);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int D = a.c.head_dim;
-  if (smem_u32(sm) & 1023u) {  // cannot be (nothing is static): no join, and the caller is told
-    if (tid == 0) write_join<BM>(a, nullptr, 1);
+  if (smem_u32(sm) & 1023u) {  // cannot be (nothing is static); the caller is told
     if (tid == 0 && a.err) atomicOr(a.err, PAGED_TIMEOUT);
     return;
   }
@@ -191,7 +190,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
   }
   pdl_launch_dependents();
   tc_fence_before();
-  tile_prefix<BM, BN, kTcThreads>(a, prefix, bars->scan, blockIdx.x == 0);  // with CTA barriers
+  tile_prefix<BN, kTcThreads>(a, __builtin_ctz(BM), prefix, bars->scan, blockIdx.x == 0);  // with CTA barriers
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
   const uint32_t tO = tmem, tS = tmem + DP, tP = tmem + DP + 64;
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
     int n = 0;
     RingCursor rc;
     for (uint32_t w = begin; w < end && ok;) {
-      const Segment s = segment_at<BM, BN>(a, prefix, w, end);
+      const Segment s = segment_at<BN>(a, prefix, w, end);
       const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
       const int cnt = s.t1 - s.t0;
       // Places of tile i (V's turn), i + 1 (K's) and i + 2, looked up ahead of their copies.
@@ -256,7 +255,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
     int n = 0;
     RingCursor rc, done;
     for (uint32_t w = begin; w < end && ok;) {
-      const Segment s = segment_at<BM, BN>(a, prefix, w, end);
+      const Segment s = segment_at<BN>(a, prefix, w, end);
       const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
       const int cnt = s.t1 - s.t0;
       // Rows of tile i (V's turn), i + 1 (K's) and i + 2, looked up ahead of their copies.
@@ -326,7 +325,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         rc.next(slots);
       };
       for (uint32_t w = begin; w < end && ok;) {
-        const Segment s = segment_at<BM, BN>(a, prefix, w, end);
+        const Segment s = segment_at<BN>(a, prefix, w, end);
         const int cnt = s.t1 - s.t0;
         if (!warp_wait(&bars->q_full, seg)) {
           ok = false;
@@ -393,15 +392,13 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
     };
     Segment s;
     if (begin < end) {
-      s = segment_at<BM, BN>(a, prefix, begin, end);
+      s = segment_at<BN>(a, prefix, begin, end);
       fetch_q(s);
     }
     int n0 = 0, g = 0;  // items before this segment, tiles so far
     uint32_t seg = 0;
-    if (begin >= end && tid == 0) write_join<BM>(a, nullptr, per);
     for (uint32_t w = begin; w < end && ok;) {
       const int cnt = s.t1 - s.t0, NR = s.n * a.G;
-      if (w == begin && tid == 0) write_join<BM>(a, &s, per);
       cp_async_wait<0>();
       fence_async();
       warp_arrive(&bars->q_full, lane);
@@ -546,7 +543,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       // The last S is taken, so every product with Q is complete: the next segment's queries may come.
       Segment following = s;
       if (w + s.step < end) {
-        following = segment_at<BM, BN>(a, prefix, w + s.step, end);
+        following = segment_at<BN>(a, prefix, w + s.step, end);
         fetch_q(following);
       }
       const bool dirty = *(volatile uint32_t*)&bars->dirty == seg + 1;
