@@ -19,6 +19,12 @@ constexpr int kTreeBN = 64;
 // positions narrow 8.2 us whole; 128 positions F32 8.2 us cut, 6.8 whole; 512 positions tcgen05 14.4
 // us cut, 20.3 whole).
 constexpr int kWholeNarrow = 8, kWholeTc = 2, kWholeF32 = 2;
+// Longer caches are not cut where that loads the fullest CTA with at most a quarter and so many tiles
+// more than equal shares would (16 ragged trees of 61 nodes, 8 heads, tcgen05: 64 tiles whole against 44
+// cut 97 us against 108, 16 against 12 35 against 54, 64 against 32 105 against 80; 36 x 1030 decoded
+// rows, narrow: 17 against 13 27.2 against 28.9, 33 against 22 43.9 against 40.4; F32: 10 against 7
+// 35.9 against 31.6, 33 against 22 100 against 83).
+constexpr uint32_t kSlackNarrow = 3, kSlackTc = 12, kSlackF32 = 1;
 // More than 8 query vectors a head, the narrow kernel takes in tiles of 8, reading K and V again for
 // each from L2; it starts faster and its tiles are quicker, so it still leads up to this many of its
 // tiles a CTA (32 vectors, 8 heads: 2056 positions 17.2 us against tcgen05's 19.5, 8200 positions 27.5
@@ -62,7 +68,7 @@ struct NarrowCfg {
   static constexpr int kOPitch = DP + 4;
   static_assert(4 * BM * (kOPitch * 4 + 8) <= kRing, "the warps' outputs take the ring's place");
   // Nothing is static, so that the dynamic part starts on the 1024 bytes that the swizzle counts from.
-  static constexpr int kBars = 4 * NS * 8 + 16;
+  static constexpr int kBars = 4 * NS * 8;
   static constexpr size_t smem(int batch) { return kRing + kBars + 4 * (size_t)(batch + 1); }
 };
 // Byte offset of 16-byte unit u (dims 8 u ..) of row r in a tile of it.
@@ -102,8 +108,8 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
   extern __shared__ __align__(1024) uint8_t narrow_smem[];
   uint8_t* sm = narrow_smem;
   uint64_t* full = (uint64_t*)(sm + C::kRing);  // [4][NS]
-  uint32_t* scan = (uint32_t*)(full + 4 * NS);
-  uint32_t* prefix = scan + 4;
+  uint32_t* scan = (uint32_t*)sm;  // before anything is fetched
+  uint32_t* prefix = (uint32_t*)(full + 4 * NS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
   const int D = a.c.head_dim;
   const float sc = soft_scale<T>(a.scale);
@@ -119,15 +125,14 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
     fence_barrier_init();
   }
   pdl_launch_dependents();
-  tile_prefix<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, scan, blockIdx.x == 0);
-  const uint32_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
+  const Line line = cut_line<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, scan, blockIdx.x == 0);
   uint32_t begin, end;
-  cta_range(per, total, blockIdx.x, begin, end);
+  cta_range(line, blockIdx.x, begin, end);
   RingCursor use;  // the stage of the next tile to consume
   bool ok = true;
 
   for (uint32_t w = begin; w < end;) {
-    const Segment s = segment_at<BN>(a, prefix, w, end);
+    const Segment s = segment_at<BN>(a, line, prefix, w, end);
     const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
     RowFetch<16> rows;
     BoxPlace box;
@@ -373,7 +378,7 @@ struct TreeFCfg {
   static constexpr int kQ = BM * P * 4, kP = kTreeFBN * PP * 4, kRows = 2 * BM * 4;
   static constexpr int kPerSm = DP <= 64 ? 5 : DP <= 128 ? 3 : 1;
   static constexpr size_t smem(int batch) {
-    return kTreeFStages * kStage + kQ + kP + kRows + 16 + 4 * (size_t)(batch + 1);
+    return kTreeFStages * kStage + kQ + kP + kRows + 4 * (size_t)(batch + 1);
   }
 };
 
@@ -389,18 +394,16 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
   float* pt = qs + BM * P;  // [key][PP]
   float* al_s = pt + BN * PP;
   uint32_t* vis_s = (uint32_t*)(al_s + BM);
-  uint32_t* scan = vis_s + BM;
-  uint32_t* prefix = scan + 4;
+  uint32_t* prefix = vis_s + BM;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.c.head_dim;
 
   pdl_launch_dependents();
-  tile_prefix<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, scan, blockIdx.x == 0);
-  const uint32_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
+  const Line line = cut_line<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, (uint32_t*)ring, blockIdx.x == 0);
   uint32_t begin, end;
-  cta_range(per, total, blockIdx.x, begin, end);
+  cta_range(line, blockIdx.x, begin, end);
 
   for (uint32_t w = begin; w < end;) {
-    const Segment s = segment_at<BN>(a, prefix, w, end);
+    const Segment s = segment_at<BN>(a, line, prefix, w, end);
     const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
     const int NR = s.n * a.G;
     RowFetch<8> ahead;  // a warp fetches 8 rows of every tile
@@ -756,6 +759,7 @@ extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_pag
   a.part_ml = (float2*)(a.part + 2ll * p.ctas * p.bm * p.dp);
   a.ctas = p.ctas;
   a.whole = p.whole;
+  a.slack = cache->dtype == PP_F32 ? kSlackF32 : p.tc ? kSlackTc : kSlackNarrow;
   a.dev = cache->cuda_device;
   a.err = err;
   const cudaStream_t st = (cudaStream_t)stream;

@@ -31,7 +31,8 @@ struct TreeArgs {
   float2* part_ml;  // [2 * ctas][BM] (max, sum)
   int32_t ctas;     // CTAs that the line of tiles is cut over
   int32_t bm;       // rows of a tile
-  int32_t whole;    // units are not cut (short caches): no partials, no join
+  int32_t whole;    // units are never cut (short caches): no partials, no join
+  uint32_t slack;   // see cut_line
   int32_t dev;
   uint32_t* err;
 };
@@ -41,48 +42,91 @@ __device__ __forceinline__ bool bad_sequence(const TreeArgs& a, int n, int len) 
   return n < 0 || len < n || (int64_t)len > (int64_t)a.b.table_stride * a.c.page.d;
 }
 
-// prefix[b] = tiles (units, where they are not cut) before sequence b on the line; prefix[batch] =
-// all. By the whole CTA (NT threads); a tile has 1 << bm_log rows; scan: NT / 32 words of shared memory.
+// The line of tiles, and how it is cut: CTA c takes the places [c per, (c + 1) per).
+struct Line {
+  uint32_t places, per;
+  bool whole;  // a place is a unit, none is cut
+};
+// prefix[b] = places before sequence b on the line; prefix[batch] = all. A CTA takes equal shares of
+// the tiles, unless whole units load the fullest CTA with at most a quarter and `slack` tiles more: cutting
+// units costs second segments and the join, and keeps every SM's CTAs in each other's way to the end. By the whole CTA (NT threads); a tile has 1 << bm_log rows; scan:
+// 3 NT / 32 words of shared memory.
 template <int BN, int NT>
-__device__ __forceinline__ void tile_prefix(const TreeArgs& a, int bm_log, uint32_t* prefix, uint32_t* scan,
-                                            bool report) {
+__device__ __forceinline__ Line cut_line(const TreeArgs& a, int bm_log, uint32_t* prefix, uint32_t* scan, bool report) {
+  constexpr int W = NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.b.batch;
-  if (B == 1) {  // the usual decode: no scan
-    if (tid == 0) {
-      const int n = a.b.cu_rows[1] - a.b.cu_rows[0], len = a.b.kv_len[0];
-      const bool bad = bad_sequence(a, n, len);
-      if (bad && report && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
-      prefix[0] = 0;
-      prefix[1] = bad || n == 0 ? 0u : ((((uint32_t)n * a.G - 1) >> bm_log) + 1) * a.c.n_kv * (a.whole ? 1 : (len + BN - 1) / BN);
-    }
-    __syncthreads();
-    return;
-  }
-  const int each = (B + NT - 1) / NT, b0 = min(B, tid * each), b1 = min(B, b0 + each);
-  uint32_t sum = 0;
-  for (int b = b0; b < b1; ++b) {
+  // Units of a sequence, and its tiles
+  auto units_of = [&](int b, uint32_t& tiles, bool report) {
     const int n = a.b.cu_rows[b + 1] - a.b.cu_rows[b], len = a.b.kv_len[b];
-    prefix[b] = sum;  // inside this thread's share
+    tiles = 0;
     if (bad_sequence(a, n, len)) {
       if (report && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
-    } else if (n > 0) {
-      const uint32_t rts = (((uint32_t)n * a.G - 1) >> bm_log) + 1;
-      sum += rts * a.c.n_kv * (a.whole ? 1 : (len + BN - 1) / BN);
+      return 0u;
     }
+    if (n == 0) return 0u;
+    tiles = (len + BN - 1) / BN;
+    return ((((uint32_t)n * a.G - 1) >> bm_log) + 1) * a.c.n_kv;
+  };
+  auto cut = [&](uint32_t units, uint32_t tiles, uint32_t longest) {
+    Line l;
+    l.whole = true;
+    l.places = units;
+    l.per = max((units + a.ctas - 1) / a.ctas, 1u);
+    if (!a.whole) {
+      const uint32_t per = max((tiles + a.ctas - 1) / a.ctas, 1u);
+      if ((uint64_t)l.per * longest > (uint64_t)per + per / 4 + a.slack) l = Line{tiles, per, false};
+    }
+    return l;
+  };
+  if (B == 1) {  // the usual decode: no scan
+    uint32_t tiles;
+    const uint32_t units = units_of(0, tiles, report && tid == 0);
+    const Line l = cut(units, units * tiles, tiles);
+    if (tid == 0) {
+      prefix[0] = 0;
+      prefix[1] = l.places;
+    }
+    __syncthreads();
+    return l;
   }
-  uint32_t inc = sum;
+  const int each = (B + NT - 1) / NT, b0 = min(B, tid * each), b1 = min(B, b0 + each);
+  uint32_t units = 0, tiles = 0, longest = 0;
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) {
+    uint32_t t;
+    const uint32_t u = units_of(b, t, report);
+    units += u;
+    tiles += u * t;
+    longest = max(longest, t);
+  }
+  uint32_t iu = units, it = tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
+    const uint32_t vu = __shfl_up_sync(0xffffffffu, iu, o), vt = __shfl_up_sync(0xffffffffu, it, o);
+    if (lane >= o) iu += vu, it += vt;
   }
-  if (lane == 31) scan[warp] = inc;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 31) scan[warp] = iu, scan[W + warp] = it, scan[2 * W + warp] = longest;
   __syncthreads();
-  uint32_t before = inc - sum;
-  for (int w = 0; w < warp; ++w) before += scan[w];
-  for (int b = b0; b < b1; ++b) prefix[b] += before;
-  if (tid == NT - 1) prefix[B] = before + sum;
+  uint32_t bu = iu - units, bt = it - tiles, su = 0, st = 0;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w == warp) bu += su, bt += st;
+    su += scan[w], st += scan[W + w];
+    longest = max(longest, scan[2 * W + w]);
+  }
+  const Line l = cut(su, st, longest);
+  uint32_t at = l.whole ? bu : bt;
+#pragma unroll 1
+  for (int b = b0; b < b1; ++b) {
+    uint32_t t;
+    const uint32_t u = units_of(b, t, false);
+    prefix[b] = at;
+    at += l.whole ? u : u * t;
+  }
+  if (tid == 0) prefix[B] = l.places;
   __syncthreads();
+  return l;
 }
 
 // The tiles of one CTA inside one unit.
@@ -94,7 +138,7 @@ struct Segment {
   uint32_t step;              // places on the line that the segment takes
 };
 template <int BN>
-__device__ __forceinline__ Segment segment_at(const TreeArgs& a, const uint32_t* prefix, uint32_t w,
+__device__ __forceinline__ Segment segment_at(const TreeArgs& a, const Line& line, const uint32_t* prefix, uint32_t w,
                                               uint32_t end) {
   int lo = 0, hi = a.b.batch;  // last b with prefix[b] <= w: the one with tiles, as w < prefix[b + 1]
   while (hi - lo > 1) {
@@ -109,23 +153,19 @@ __device__ __forceinline__ Segment segment_at(const TreeArgs& a, const uint32_t*
   s.len = a.b.kv_len[lo];
   s.ctx = s.len - s.n;
   s.tiles = (s.len + BN - 1) / BN;
-  const uint32_t off = w - prefix[lo], unit = a.whole ? off : off / (uint32_t)s.tiles;
-  s.t0 = a.whole ? 0 : (int)(off - unit * s.tiles);
+  const uint32_t off = w - prefix[lo], unit = line.whole ? off : off / (uint32_t)s.tiles;
+  s.t0 = line.whole ? 0 : (int)(off - unit * s.tiles);
   s.rt = (int)a.by_kv.div(unit);
   s.h = (int)(unit - (uint32_t)s.rt * a.c.n_kv);
-  s.t1 = a.whole ? s.tiles : (int)min((uint32_t)s.tiles, s.t0 + (end - w));
+  s.t1 = line.whole ? s.tiles : (int)min((uint32_t)s.tiles, s.t0 + (end - w));
   s.unit0 = w - s.t0;
-  s.step = a.whole ? 1 : s.t1 - s.t0;
+  s.step = line.whole ? 1 : s.t1 - s.t0;
   return s;
 }
-__device__ __forceinline__ uint32_t tiles_per_cta(const TreeArgs& a, uint32_t total) {
-  return max((total + a.ctas - 1) / a.ctas, 1u);
-}
 // Range of the line that CTA `cta` takes.
-__device__ __forceinline__ void cta_range(uint32_t per, uint32_t total, uint32_t cta, uint32_t& begin,
-                                          uint32_t& end) {
-  begin = min((uint64_t)cta * per, (uint64_t)total);
-  end = min(begin + per, total);
+__device__ __forceinline__ void cta_range(const Line& line, uint32_t cta, uint32_t& begin, uint32_t& end) {
+  begin = min((uint64_t)cta * line.per, (uint64_t)line.places);
+  end = min(begin + line.per, line.places);
 }
 
 // Whether row (sequence row i) sees node j (0 <= j < n).
@@ -318,19 +358,19 @@ struct JoinUnit {
   int32_t row0, vec0, head0, n, ctx;  // first array row, vector of row 0, first head, nodes, context
 };
 template <int BN>
-__device__ __forceinline__ JoinUnit join_unit(const TreeArgs& a, int bm_log, const uint32_t* prefix, uint32_t per,
-                                              uint32_t total, uint32_t cta) {
+__device__ __forceinline__ JoinUnit join_unit(const TreeArgs& a, const Line& line, int bm_log, const uint32_t* prefix,
+                                              uint32_t cta) {
   JoinUnit u = {};
   uint32_t begin, end;
-  cta_range(per, total, cta, begin, end);
-  if (begin >= end) return u;
-  const Segment s = segment_at<BN>(a, prefix, begin, end);
+  cta_range(line, cta, begin, end);
+  if (line.whole || begin >= end) return u;
+  const Segment s = segment_at<BN>(a, line, prefix, begin, end);
   if (s.t0 == 0 || s.t1 < s.tiles) return u;
-  const uint32_t c0 = s.unit0 / per;
+  const uint32_t c0 = s.unit0 / line.per;
   u.parts = (int)(cta - c0) + 1;
   u.vec0 = s.rt << bm_log;
   u.rows = min(1 << bm_log, s.n * a.G - u.vec0);
-  u.first_slot = (int)(c0 * per == s.unit0 ? 2 * c0 : 2 * c0 + 1);
+  u.first_slot = (int)(c0 * line.per == s.unit0 ? 2 * c0 : 2 * c0 + 1);
   u.cta = (int)c0;
   u.row0 = s.row0;
   u.head0 = s.h * a.G;
@@ -343,20 +383,19 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
   constexpr int V = DP / 16, BN = sizeof(T) == 4 ? 32 : 64;  // the attention's key tile
   extern __shared__ uint32_t s_items[];  // [ctas + 1] items before each CTA's unit, then [batch + 1]
-  __shared__ uint32_t scan[4];
+  __shared__ uint32_t scan[12];
   __shared__ float s_acc[8][DP];
   __shared__ float2 s_ml[8];
   uint32_t* prefix = s_items + a.ctas + 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = tid >> 4, l16 = tid & 15;
   const int each = (a.ctas + 127) / 128, c0 = min(a.ctas, tid * each), c1 = min(a.ctas, c0 + each);
   const int bm_log = 31 - __clz(a.bm);
-  tile_prefix<BN, 128>(a, bm_log, prefix, scan, false);
-  const uint32_t places = prefix[a.b.batch], per = tiles_per_cta(a, places);
+  const Line line = cut_line<BN, 128>(a, bm_log, prefix, scan, false);
   {
     uint32_t sum = 0;
 #pragma unroll 1
     for (int c = c0; c < c1; ++c) {
-      const JoinUnit u = join_unit<BN>(a, bm_log, prefix, per, places, c);
+      const JoinUnit u = join_unit<BN>(a, line, bm_log, prefix, c);
       s_items[c] = sum;
       if (u.parts > 0) sum += u.parts > kJoinMany ? u.rows : (u.rows + 7) / 8;
     }
@@ -390,7 +429,7 @@ __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
         if (s_items[mid] <= item) lo = mid;
         else hi = mid;
       }
-      u = join_unit<BN>(a, bm_log, prefix, per, places, lo);
+      u = join_unit<BN>(a, line, bm_log, prefix, lo);
       at = (int)(item - s_items[lo]);
     }
     if (!waited) pdl_wait();  // by every CTA: the stream goes on when all of this grid's have ended

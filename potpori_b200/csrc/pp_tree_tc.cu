@@ -43,9 +43,9 @@ struct TcCfg {
   static constexpr int kSlots = DP == 64 ? 8 : 4;
   static constexpr int kPerSm = DP == 256 ? 1 : 2;
   static constexpr int kCols = DP == 256 ? 512 : 256;  // TMEM: O [DP], S [64], P hi [32], P lo [32]
-  static constexpr int kBars = 256;
+  static constexpr int kBars = 192;
   // Two CTAs share 228 KB less 1 KB each: at head_dim 128 that leaves 1 KB beside Q, four slots and
-  // the turn buffer, for the barriers and the prefix of up to 180 sequences. (More slots than four
+  // the turn buffer, for the barriers and the prefix of up to 196 sequences. (More slots than four
   // only lengthen every other load's way through memory: at the card's rate 148 x 2 x 64 KB in flight
   // are 3 us already.)
   static size_t smem(int batch) { return kQ + kTurn + kSlots * (size_t)kItem + kBars + 4 * (size_t)(batch + 1); }
@@ -54,10 +54,9 @@ struct TcCfg {
 struct TcBars {
   uint64_t full[8], free[8];
   uint64_t q_full, s_full, s_free, p_full, pv_done, end;
-  uint32_t scan[8];
   uint32_t tmem, dirty;
 };
-static_assert(sizeof(TcBars) <= 256, "barriers");
+static_assert(sizeof(TcBars) <= 192, "barriers");
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -190,13 +189,12 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
   }
   pdl_launch_dependents();
   tc_fence_before();
-  tile_prefix<BN, kTcThreads>(a, __builtin_ctz(BM), prefix, bars->scan, blockIdx.x == 0);  // with CTA barriers
+  const Line line = cut_line<BN, kTcThreads>(a, __builtin_ctz(BM), prefix, (uint32_t*)qs, blockIdx.x == 0);  // with CTA barriers
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
   const uint32_t tO = tmem, tS = tmem + DP, tP = tmem + DP + 64;
-  const uint32_t total = prefix[a.b.batch], per = tiles_per_cta(a, total);
   uint32_t begin, end;
-  cta_range(per, total, blockIdx.x, begin, end);
+  cta_range(line, blockIdx.x, begin, end);
   bool ok = true;
 
   if (warp == 4 && maps.box) {
@@ -206,7 +204,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
     int n = 0;
     RingCursor rc;
     for (uint32_t w = begin; w < end && ok;) {
-      const Segment s = segment_at<BN>(a, prefix, w, end);
+      const Segment s = segment_at<BN>(a, line, prefix, w, end);
       const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
       const int cnt = s.t1 - s.t0;
       // Places of tile i (V's turn), i + 1 (K's) and i + 2, looked up ahead of their copies.
@@ -255,7 +253,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
     int n = 0;
     RingCursor rc, done;
     for (uint32_t w = begin; w < end && ok;) {
-      const Segment s = segment_at<BN>(a, prefix, w, end);
+      const Segment s = segment_at<BN>(a, line, prefix, w, end);
       const int32_t* table = a.b.table + (int64_t)s.b * a.b.table_stride;
       const int cnt = s.t1 - s.t0;
       // Rows of tile i (V's turn), i + 1 (K's) and i + 2, looked up ahead of their copies.
@@ -325,7 +323,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         rc.next(slots);
       };
       for (uint32_t w = begin; w < end && ok;) {
-        const Segment s = segment_at<BN>(a, prefix, w, end);
+        const Segment s = segment_at<BN>(a, line, prefix, w, end);
         const int cnt = s.t1 - s.t0;
         if (!warp_wait(&bars->q_full, seg)) {
           ok = false;
@@ -392,7 +390,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
     };
     Segment s;
     if (begin < end) {
-      s = segment_at<BN>(a, prefix, begin, end);
+      s = segment_at<BN>(a, line, prefix, begin, end);
       fetch_q(s);
     }
     int n0 = 0, g = 0;  // items before this segment, tiles so far
@@ -543,7 +541,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       // The last S is taken, so every product with Q is complete: the next segment's queries may come.
       Segment following = s;
       if (w + s.step < end) {
-        following = segment_at<BN>(a, prefix, w + s.step, end);
+        following = segment_at<BN>(a, line, prefix, w + s.step, end);
         fetch_q(following);
       }
       const bool dirty = *(volatile uint32_t*)&bars->dirty == seg + 1;
