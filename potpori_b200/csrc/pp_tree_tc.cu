@@ -403,6 +403,8 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
 
       const int R = s.rt * BM + tid, i = (int)a.by_g.div((uint32_t)R), row = s.row0 + i;
       const bool idle = s.rt * BM + warp * 32 >= NR;
+      // Tiles of context alone, which most are, come first and need nothing but the softmax: one test.
+      const int plain = idle || a.scale <= 0.f ? 0 : s.ctx / BN - s.t0;
       float m = -INFINITY, l = 0.f;
       for (int t = 0; t < cnt; ++t, ++g) {
         if (!warp_wait(&bars->s_full, (uint32_t)g & 1u)) {
@@ -416,55 +418,57 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         tc_wait_ld();
         tc_fence_before();
         warp_arrive(&bars->s_free, lane);
-        const int j0 = (s.t0 + t) * BN;
-        const bool tree = j0 + BN > s.ctx;
-        const bool blind = tree && (a.mask || s.n > 1);
-        if (blind || j0 + BN > s.len) {
-          // Positions past the end hold whatever their page did: zeros there. And a V that some row
-          // is blind to must not count even where it is not finite (0 * NaN): such values leave the
-          // tile here and come back, for the rows that see them, with the output. The slot stays
-          // until this tile's product, which waits for p_full.
-          const int item = n0 + (t == cnt - 1 ? 2 * cnt - 1 : 2 * t + 2), slot = item % slots;
-          if (!warp_wait(&bars->full[slot], (uint32_t)(item / slots) & 1u)) {
-            ok = false;
-            break;
-          }
-          uint32_t found = 0;
+        if (__builtin_expect(t >= plain, 0)) {
+          const int j0 = (s.t0 + t) * BN;
+          const bool tree = j0 + BN > s.ctx;
+          const bool blind = tree && (a.mask || s.n > 1);
+          if (blind || j0 + BN > s.len) {
+            // Positions past the end hold whatever their page did: zeros there. And a V that some row
+            // is blind to must not count even where it is not finite (0 * NaN): such values leave the
+            // tile here and come back, for the rows that see them, with the output. The slot stays
+            // until this tile's product, which waits for p_full.
+            const int item = n0 + (t == cnt - 1 ? 2 * cnt - 1 : 2 * t + 2), slot = item % slots;
+            if (!warp_wait(&bars->full[slot], (uint32_t)(item / slots) & 1u)) {
+              ok = false;
+              break;
+            }
+            uint32_t found = 0;
 #pragma unroll 4
-          for (int e = tid; e < BN * UR; e += 128) {
-            uint4* p = (uint4*)(ring + (size_t)slot * C::kItem + e * 16);
-            if (j0 + ((e >> 3) & (BN - 1)) >= s.len) {
-              *p = make_uint4(0u, 0u, 0u, 0u);
-            } else if (blind) {
-              const uint4 v = *p;
-              const uint32_t b0 = nonfinite_halves<T>(v.x), b1 = nonfinite_halves<T>(v.y), b2 = nonfinite_halves<T>(v.z), b3 = nonfinite_halves<T>(v.w);
-              if (b0 | b1 | b2 | b3) {
-                found = 1;
-                *p = make_uint4(v.x & ~b0, v.y & ~b1, v.z & ~b2, v.w & ~b3);
+            for (int e = tid; e < BN * UR; e += 128) {
+              uint4* p = (uint4*)(ring + (size_t)slot * C::kItem + e * 16);
+              if (j0 + ((e >> 3) & (BN - 1)) >= s.len) {
+                *p = make_uint4(0u, 0u, 0u, 0u);
+              } else if (blind) {
+                const uint4 v = *p;
+                const uint32_t b0 = nonfinite_halves<T>(v.x), b1 = nonfinite_halves<T>(v.y), b2 = nonfinite_halves<T>(v.z), b3 = nonfinite_halves<T>(v.w);
+                if (b0 | b1 | b2 | b3) {
+                  found = 1;
+                  *p = make_uint4(v.x & ~b0, v.y & ~b1, v.z & ~b2, v.w & ~b3);
+                }
               }
             }
+            if (found) bars->dirty = seg + 1;
+            fence_async();
           }
-          if (found) bars->dirty = seg + 1;
-          fence_async();
-        }
-        if (idle) {  // no row of the warp is in the unit: its P may be anything
-          if (g > 0 && !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
-            ok = false;
-            break;
+          if (idle) {  // no row of the warp is in the unit: its P may be anything
+            if (g > 0 && !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
+              ok = false;
+              break;
+            }
+            warp_arrive(&bars->p_full, lane);
+            continue;
           }
-          warp_arrive(&bars->p_full, lane);
-          continue;
-        }
-        if (a.scale <= 0.f) {
-          const float by = a.scale < 0.f ? -1.f : 0.f;
+          if (a.scale <= 0.f) {
+            const float by = a.scale < 0.f ? -1.f : 0.f;
 #pragma unroll
-          for (int k = 0; k < 64; ++k) x[k >> 5][k & 31] *= by;
-        }
-        if (tree) {
-          const uint64_t see = seen64(a, s, row, i, j0);
+            for (int k = 0; k < 64; ++k) x[k >> 5][k & 31] *= by;
+          }
+          if (tree) {
+            const uint64_t see = seen64(a, s, row, i, j0);
 #pragma unroll
-          for (int k = 0; k < 64; ++k)
-            if (!(see >> k & 1u)) x[k >> 5][k & 31] = -INFINITY;
+            for (int k = 0; k < 64; ++k)
+              if (!(see >> k & 1u)) x[k >> 5][k & 31] = -INFINITY;
+          }
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
