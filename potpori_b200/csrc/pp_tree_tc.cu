@@ -11,8 +11,9 @@
 //    read K-major it is the B operand of Q K^T, read MN-major the B operand of P V. Where pages are
 //    not multiples of 16 positions, warps 4 and 5 fetch row by row with 16-byte asynchronous copies.
 //  * warp 6, one thread: S = Q K^T (128 x 64, both operands in shared memory) and O += P V (P in
-//    TMEM), each returned by a commit on an mbarrier. S of the next tile is issued as soon as the
-//    softmax has taken S of this one.
+//    TMEM), each returned by a commit on an mbarrier. S has two places, and P takes its S's: S of a
+//    tile is issued while the softmax works on the tile before, when the product of the one before
+//    that is complete.
 //  * warps 0-3, softmax: thread = row = TMEM lane. S of the row into 64 registers; mask; running
 //    maximum; exp2; P back to TMEM. The output in TMEM is rescaled only when a row's maximum has
 //    grown by more than 2^8 (until then the old maximum serves: P <= 256 and the sums are F32), so
@@ -42,7 +43,7 @@ struct TcCfg {
   static constexpr int kTurn = 4 * 4096;        // rows on their way out, 4 KB a softmax warp
   static constexpr int kSlots = DP == 64 ? 8 : 4;
   static constexpr int kPerSm = DP == 256 ? 1 : 2;
-  static constexpr int kCols = DP == 256 ? 512 : 256;  // TMEM: O [DP], S [64], P hi [32], P lo [32]
+  static constexpr int kCols = DP == 256 ? 512 : 256;  // TMEM: O [DP], twice S or P [64]
   static constexpr int kBars = 192;
   // Two CTAs share 228 KB less 1 KB each: at head_dim 128 that leaves 1 KB beside Q, four slots and
   // the turn buffer, for the barriers and the prefix of up to 196 sequences. (More slots than four
@@ -53,7 +54,7 @@ struct TcCfg {
 
 struct TcBars {
   uint64_t full[8], free[8];
-  uint64_t q_full, s_full, s_free, p_full, pv_done, end;
+  uint64_t q_full, s_full[2], p_full[2], pv_done, end;
   uint32_t tmem, dirty;
 };
 static_assert(sizeof(TcBars) <= 192, "barriers");
@@ -174,9 +175,10 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       mbar_init(&bars->free[i], 1);
     }
     mbar_init(&bars->q_full, 4);
-    mbar_init(&bars->s_full, 1);
-    mbar_init(&bars->s_free, 4);
-    mbar_init(&bars->p_full, 4);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->s_full[i], 1);
+      mbar_init(&bars->p_full[i], 4);
+    }
     mbar_init(&bars->pv_done, 1);
     mbar_init(&bars->end, 1);
     bars->dirty = 0;
@@ -192,7 +194,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
   const Line line = cut_line<BN, kTcThreads>(a, __builtin_ctz(BM), prefix, (uint32_t*)qs, blockIdx.x == 0);  // with CTA barriers
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
-  const uint32_t tO = tmem, tS = tmem + DP, tP = tmem + DP + 64;
+  const uint32_t tO = tmem, tS = tmem + DP;  // S of phase q at tS + 64 (q & 1), and its P in its place
   uint32_t begin, end;
   cta_range(line, blockIdx.x, begin, end);
   bool ok = true;
@@ -306,22 +308,9 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       constexpr uint32_t iqk = tc_idesc<T>(BN, false), ipv = tc_idesc<T>(DP, true);
       const uint32_t qa = (smem_u32(qs) >> 4) | tc_lead(16), ring_a = smem_u32(ring) >> 4;
       RingCursor rc;
-      uint32_t tile = 0;  // parity of the tile whose S comes next
+      uint32_t q = 0, tiles = 0;  // phases of s_full and tiles so far
       uint32_t seg = 0;
-      bool first = true;
       auto take = [&]() -> bool { return warp_wait(&bars->full[rc.slot], rc.phase); };
-      auto qk = [&]() {  // S = Q K^T from the ring's next item; dims past the head's are zero
-        const uint32_t ka = (ring_a + rc.slot * (C::kItem >> 4)) | tc_lead(16);
-        if (elect_one()) {
-#pragma unroll
-          for (int ks = 0; ks < DP / 16; ++ks)
-            tc_mma_ss(tS, qa + (ks >> 2) * (BM * 8) + (ks & 3) * 2, ka + (ks >> 2) * (BN * 8) + (ks & 3) * 2, iqk, ks != 0);
-          tc_commit(&bars->s_full);
-          tc_commit(&bars->free[rc.slot]);
-        }
-        __syncwarp();
-        rc.next(slots);
-      };
       for (uint32_t w = begin; w < end && ok;) {
         const Segment s = segment_at<BN>(a, line, prefix, w, end);
         const int cnt = s.t1 - s.t0;
@@ -329,38 +318,62 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           ok = false;
           break;
         }
-        // Step i issues S of tile i + 1, then O of tile i.
-        for (int i = -1; i < cnt; ++i) {
-          if (i + 1 < cnt) {
-            if (!take() || !(first || warp_wait(&bars->s_free, tile ^ 1u))) {
+        // Step i issues S of tile i + 1, then O of tile i. A segment has two phases of s_full more than
+        // tiles: the first one's commit tells that the product before the last is complete, the second
+        // one's that the last is.
+        for (int i = -1; i < cnt; ++i, ++q) {
+          // S of tile i + 1 takes the place of P of tile i - 1, whose product must be complete.
+          if (i >= 1 && !warp_wait(&bars->pv_done, (tiles - 1) & 1u)) {
+            ok = false;
+            break;
+          }
+          if (i + 1 < cnt) {  // S = Q K^T from the ring's next item; dims past the head's are zero
+            if (!take()) {
               ok = false;
               break;
             }
-            first = false;
-            tile ^= 1u;
             tc_fence_after();
-            qk();
+            const uint32_t ka = (ring_a + rc.slot * (C::kItem >> 4)) | tc_lead(16), to = tS + 64 * (q & 1u);
+            if (elect_one()) {
+#pragma unroll
+              for (int ks = 0; ks < DP / 16; ++ks)
+                tc_mma_ss(to, qa + (ks >> 2) * (BM * 8) + (ks & 3) * 2, ka + (ks >> 2) * (BN * 8) + (ks & 3) * 2, iqk, ks != 0);
+              tc_commit(&bars->s_full[q & 1u]);
+              tc_commit(&bars->free[rc.slot]);
+            }
+            __syncwarp();
+            rc.next(slots);
+          } else {
+            if (elect_one()) tc_commit(&bars->s_full[q & 1u]);
+            __syncwarp();
           }
           if (i < 0) continue;
-          // P of tile i: where S of tile i + 1 went out above, `tile` is already the next one's.
-          if (!take() || !warp_wait(&bars->p_full, i + 1 < cnt ? tile : tile ^ 1u)) {
+          if (!take() || !warp_wait(&bars->p_full[tiles & 1u], (tiles >> 1) & 1u)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t va = (ring_a + rc.slot * (C::kItem >> 4)) | tc_lead(BN * 128);
+          const uint32_t va = (ring_a + rc.slot * (C::kItem >> 4)) | tc_lead(BN * 128), tP = tS + 64 * (~q & 1u);
           if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < BN / 16; ++ks) {
-              tc_mma_ts(tO, tP + 8 * ks, va + ks * 128, ipv, ks == 0 ? i : 1u);
-              tc_mma_ts(tO, tP + 32 + 8 * ks, va + ks * 128, ipv, 1u);
+              tc_mma_ts(tO, tP + 32 * (ks >> 1) + 8 * (ks & 1), va + ks * 128, ipv, ks == 0 ? i : 1u);
+              tc_mma_ts(tO, tP + 32 * (ks >> 1) + 8 * (ks & 1) + 16, va + ks * 128, ipv, 1u);
             }
             tc_commit(&bars->pv_done);
             tc_commit(&bars->free[rc.slot]);
           }
           __syncwarp();
           rc.next(slots);
+          ++tiles;
         }
+        if (!ok || !warp_wait(&bars->pv_done, (tiles - 1) & 1u)) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) tc_commit(&bars->s_full[q & 1u]);
+        __syncwarp();
+        ++q;
         seg ^= 1u;
         w += s.step;
       }
@@ -393,8 +406,8 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       s = segment_at<BN>(a, line, prefix, begin, end);
       fetch_q(s);
     }
-    int n0 = 0, g = 0;  // items before this segment, tiles so far
-    uint32_t seg = 0;
+    int n0 = 0;  // items before this segment
+    uint32_t q = 0, tiles = 0, seg = 0;  // phases of s_full, tiles so far
     for (uint32_t w = begin; w < end && ok;) {
       const int cnt = s.t1 - s.t0, NR = s.n * a.G;
       cp_async_wait<0>();
@@ -406,18 +419,17 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       // Tiles of context alone, which most are, come first and need nothing but the softmax: one test.
       const int plain = idle || a.scale <= 0.f ? 0 : s.ctx / BN - s.t0;
       float m = -INFINITY, l = 0.f;
-      for (int t = 0; t < cnt; ++t, ++g) {
-        if (!warp_wait(&bars->s_full, (uint32_t)g & 1u)) {
+      for (int t = 0; t < cnt; ++t, ++q, ++tiles) {
+        if (!warp_wait(&bars->s_full[q & 1u], (q >> 1) & 1u)) {
           ok = false;
           break;
         }
         tc_fence_after();
         float x[2][32];
-        tc_ld32(tS + lanes, x[0]);
-        tc_ld32(tS + lanes + 32, x[1]);
+        const uint32_t at = tS + 64 * (q & 1u) + lanes;
+        tc_ld32(at, x[0]);
+        tc_ld32(at + 32, x[1]);
         tc_wait_ld();
-        tc_fence_before();
-        warp_arrive(&bars->s_free, lane);
         if (__builtin_expect(t >= plain, 0)) {
           const int j0 = (s.t0 + t) * BN;
           const bool tree = j0 + BN > s.ctx;
@@ -451,11 +463,8 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
             fence_async();
           }
           if (idle) {  // no row of the warp is in the unit: its P may be anything
-            if (g > 0 && !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
-              ok = false;
-              break;
-            }
-            warp_arrive(&bars->p_full, lane);
+            tc_fence_before();
+            warp_arrive(&bars->p_full[tiles & 1u], lane);
             continue;
           }
           if (a.scale <= 0.f) {
@@ -484,24 +493,32 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           l *= alpha;
         }
         const float base = m == -INFINITY ? 0.f : m;
-        // Two elements an instruction where there is one for F32 pairs.
-        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // P over S: of each 32 keys 16 columns of high parts, 16 of low ones. Two elements an
+        // instruction where there is one for F32 pairs.
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          float& v0 = x[k >> 4][(2 * k) & 31];
-          float& v1 = x[k >> 4][(2 * k + 1) & 31];
-          const float2 y = __ffma2_rn(make_float2(v0, v1), make_float2(sc, sc), make_float2(-base, -base));
-          v0 = soft_exp<T>(y.x);
-          v1 = soft_exp<T>(y.y);
-          sum[k & 1] = __fadd2_rn(sum[k & 1], make_float2(v0, v1));
+        for (int c = 0; c < 2; ++c) {
+          uint32_t p[32];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const float2 y = __ffma2_rn(make_float2(x[c][2 * k], x[c][2 * k + 1]), make_float2(sc, sc), make_float2(-base, -base));
+            const float2 v = make_float2(soft_exp<T>(y.x), soft_exp<T>(y.y));
+            sum = __fadd2_rn(sum, v);
+            p[k] = tc_pack(v.x, v.y, (T*)nullptr);
+            const float2 h = tc_unpack(p[k], (T*)nullptr);
+            const float2 rest = __fadd2_rn(v, make_float2(-h.x, -h.y));
+            p[16 + k] = tc_pack(rest.x, rest.y, (T*)nullptr);
+          }
+          tc_st32(at + 32 * c, p);
         }
-        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        if (g > 0 && !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+        l += sum.x + sum.y;
         if (rescale && t > 0) {
+          // The next phase comes when the product of the tile before this one is complete.
+          if (!warp_wait(&bars->s_full[~q & 1u], ((q + 1) >> 1) & 1u)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < DP; c += 32) {
             float o[32];
@@ -512,37 +529,25 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
             tc_st32(tO + lanes + c, *(const uint32_t(*)[32])o);
           }
         }
-        uint32_t p[32];
-#pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          float& v0 = x[k >> 4][(2 * k) & 31];
-          float& v1 = x[k >> 4][(2 * k + 1) & 31];
-          p[k] = tc_pack(v0, v1, (T*)nullptr);
-          const float2 h = tc_unpack(p[k], (T*)nullptr);
-          const float2 rest = __fadd2_rn(make_float2(v0, v1), make_float2(-h.x, -h.y));
-          v0 = rest.x;
-          v1 = rest.y;
-        }
-        tc_st32(tP + lanes, p);
-#pragma unroll
-        for (int k = 0; k < 32; ++k) p[k] = tc_pack(x[k >> 4][(2 * k) & 31], x[k >> 4][(2 * k + 1) & 31], (T*)nullptr);
-        tc_st32(tP + lanes + 32, p);
         tc_wait_st();
         tc_fence_before();
-        warp_arrive(&bars->p_full, lane);
+        warp_arrive(&bars->p_full[tiles & 1u], lane);
       }
-      if (!ok || !warp_wait(&bars->pv_done, (uint32_t)(g - 1) & 1u)) {
+      // Every product with Q and into O is complete after the segment's last phase.
+      if (!ok || !warp_wait(&bars->s_full[q & 1u], (q >> 1) & 1u) ||
+          !warp_wait(&bars->s_full[~q & 1u], ((q + 1) >> 1) & 1u)) {
         ok = false;
         break;
       }
+      q += 2;
       tc_fence_after();
       // Every softmax thread's mark of this segment is visible once all have handed their last P on;
       // the next segment's come after all have passed here (its first S waits for all of Q).
-      if (!warp_wait(&bars->p_full, (uint32_t)(g - 1) & 1u)) {
+      if (!warp_wait(&bars->p_full[~tiles & 1u], ((tiles - 1) >> 1) & 1u)) {
         ok = false;
         break;
       }
-      // The last S is taken, so every product with Q is complete: the next segment's queries may come.
+      // The next segment's queries may come.
       Segment following = s;
       if (w + s.step < end) {
         following = segment_at<BN>(a, line, prefix, w + s.step, end);
