@@ -69,7 +69,7 @@ struct NarrowCfg {
   static_assert(4 * BM * (kOPitch * 4 + 8) <= kRing, "the warps' outputs take the ring's place");
   // Nothing is static, so that the dynamic part starts on the 1024 bytes that the swizzle counts from.
   static constexpr int kBars = 4 * NS * 8;
-  static constexpr size_t smem(int batch) { return kRing + kBars + 4 * (size_t)(batch + 1); }
+  static size_t smem(int batch) { return kRing + kBars + prefix_bytes(batch); }
 };
 // Byte offset of 16-byte unit u (dims 8 u ..) of row r in a tile of it.
 __device__ __forceinline__ int narrow_unit(int r, int u) { return (u >> 3) * 2048 + r * 128 + (((u & 7) ^ (r & 7)) << 4); }
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
     fence_barrier_init();
   }
   pdl_launch_dependents();
-  const Line line = cut_line<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, scan, blockIdx.x == 0);
+  const Line line = cut_line<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, true, scan, blockIdx.x == 0);
   uint32_t begin, end;
   cta_range(line, blockIdx.x, begin, end);
   RingCursor use;  // the stage of the next tile to consume
@@ -377,8 +377,8 @@ struct TreeFCfg {
   static constexpr int kTile = kTreeFBN * P * 4, kStage = 2 * kTile;
   static constexpr int kQ = BM * P * 4, kP = kTreeFBN * PP * 4, kRows = 2 * BM * 4;
   static constexpr int kPerSm = DP <= 64 ? 5 : DP <= 128 ? 3 : 1;
-  static constexpr size_t smem(int batch) {
-    return kTreeFStages * kStage + kQ + kP + kRows + 4 * (size_t)(batch + 1);
+  static size_t smem(int batch) {
+    return kTreeFStages * kStage + kQ + kP + kRows + prefix_bytes(batch);
   }
 };
 
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kTreeThreads) pp_tree_f32_kernel(const TreeArg
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, D = a.c.head_dim;
 
   pdl_launch_dependents();
-  const Line line = cut_line<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, (uint32_t*)ring, blockIdx.x == 0);
+  const Line line = cut_line<BN, kTreeThreads>(a, __builtin_ctz(BM), prefix, true, (uint32_t*)ring, blockIdx.x == 0);
   uint32_t begin, end;
   cta_range(line, blockIdx.x, begin, end);
 

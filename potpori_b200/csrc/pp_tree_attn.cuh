@@ -42,19 +42,28 @@ __device__ __forceinline__ bool bad_sequence(const TreeArgs& a, int n, int len) 
   return n < 0 || len < n || (int64_t)len > (int64_t)a.b.table_stride * a.c.page.d;
 }
 
+// Sequences up to which a line may be put in order.
+constexpr int kOrderMost = 64;
+inline size_t prefix_bytes(int batch) { return 4 * ((size_t)batch + 1 + (batch <= kOrderMost ? batch : 0)); }
+
 // The line of tiles, and how it is cut: CTA c takes the places [c per, (c + 1) per).
 struct Line {
   uint32_t places, per;
   bool whole;  // a place is a unit, none is cut
+  const uint32_t* order;  // the sequences by falling length; null: as they come
 };
 // prefix[b] = places before sequence b on the line; prefix[batch] = all. A CTA takes equal shares of
 // the tiles, unless whole units load the fullest CTA with at most a quarter and `slack` tiles more: cutting
-// units costs second segments and the join, and keeps every SM's CTAs in each other's way to the end. By the whole CTA (NT threads); a tile has 1 << bm_log rows; scan:
+// units costs second segments and the join, and keeps every SM's CTAs in each other's way to the end. Of whole
+// units the long ones come first where each has a CTA of its own: the first CTA of every SM then takes one
+// of them and the second one of the short ones. By the whole CTA (NT threads); a tile has 1 << bm_log rows; scan:
 // 3 NT / 32 words of shared memory.
 template <int BN, int NT>
-__device__ __forceinline__ Line cut_line(const TreeArgs& a, int bm_log, uint32_t* prefix, uint32_t* scan, bool report) {
+__device__ __forceinline__ Line cut_line(const TreeArgs& a, int bm_log, uint32_t* prefix, bool sort, uint32_t* scan,
+                                         bool report) {
   constexpr int W = NT / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = a.b.batch;
+  uint32_t* order = prefix + B + 1;
   // Units of a sequence, and its tiles
   auto units_of = [&](int b, uint32_t& tiles, bool report) {
     const int n = a.b.cu_rows[b + 1] - a.b.cu_rows[b], len = a.b.kv_len[b];
@@ -68,13 +77,13 @@ __device__ __forceinline__ Line cut_line(const TreeArgs& a, int bm_log, uint32_t
     return ((((uint32_t)n * a.G - 1) >> bm_log) + 1) * a.c.n_kv;
   };
   auto cut = [&](uint32_t units, uint32_t tiles, uint32_t longest) {
-    Line l;
+    Line l = {};
     l.whole = true;
     l.places = units;
     l.per = max((units + a.ctas - 1) / a.ctas, 1u);
     if (!a.whole) {
       const uint32_t per = max((tiles + a.ctas - 1) / a.ctas, 1u);
-      if ((uint64_t)l.per * longest > (uint64_t)per + per / 4 + a.slack) l = Line{tiles, per, false};
+      if ((uint64_t)l.per * longest > (uint64_t)per + per / 4 + a.slack) l = Line{tiles, per, false, nullptr};
     }
     return l;
   };
@@ -99,6 +108,7 @@ __device__ __forceinline__ Line cut_line(const TreeArgs& a, int bm_log, uint32_t
     tiles += u * t;
     longest = max(longest, t);
   }
+  const uint32_t mine = longest;  // of a lone sequence: its tiles
   uint32_t iu = units, it = tiles;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -115,7 +125,24 @@ __device__ __forceinline__ Line cut_line(const TreeArgs& a, int bm_log, uint32_t
     su += scan[w], st += scan[W + w];
     longest = max(longest, scan[2 * W + w]);
   }
-  const Line l = cut(su, st, longest);
+  Line l = cut(su, st, longest);
+  if (sort && l.whole && !a.whole && l.per == 1 && B <= kOrderMost) {  // a thread has one sequence
+    const uint32_t own = mine;
+    if (tid < B) prefix[tid] = own, order[tid] = units;
+    __syncthreads();
+    uint32_t rank = 0, before = 0;
+#pragma unroll 4
+    for (int b = 0; b < B; ++b) {
+      const uint32_t t = prefix[b];
+      if (t > own || (t == own && b < tid)) ++rank, before += order[b];
+    }
+    __syncthreads();
+    if (tid < B) prefix[rank] = before, order[rank] = (uint32_t)tid;
+    if (tid == 0) prefix[B] = l.places;
+    __syncthreads();
+    l.order = order;
+    return l;
+  }
   uint32_t at = l.whole ? bu : bt;
 #pragma unroll 1
   for (int b = b0; b < b1; ++b) {
@@ -146,6 +173,8 @@ __device__ __forceinline__ Segment segment_at(const TreeArgs& a, const Line& lin
     if (prefix[mid] <= w) lo = mid;
     else hi = mid;
   }
+  const uint32_t off = w - prefix[lo];
+  if (line.order) lo = (int)line.order[lo];
   Segment s;
   s.b = lo;
   s.row0 = a.b.cu_rows[lo];
@@ -153,7 +182,7 @@ __device__ __forceinline__ Segment segment_at(const TreeArgs& a, const Line& lin
   s.len = a.b.kv_len[lo];
   s.ctx = s.len - s.n;
   s.tiles = (s.len + BN - 1) / BN;
-  const uint32_t off = w - prefix[lo], unit = line.whole ? off : off / (uint32_t)s.tiles;
+  const uint32_t unit = line.whole ? off : off / (uint32_t)s.tiles;
   s.t0 = line.whole ? 0 : (int)(off - unit * s.tiles);
   s.rt = (int)a.by_kv.div(unit);
   s.h = (int)(unit - (uint32_t)s.rt * a.c.n_kv);
@@ -390,7 +419,7 @@ __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = tid >> 4, l16 = tid & 15;
   const int each = (a.ctas + 127) / 128, c0 = min(a.ctas, tid * each), c1 = min(a.ctas, c0 + each);
   const int bm_log = 31 - __clz(a.bm);
-  const Line line = cut_line<BN, 128>(a, bm_log, prefix, scan, false);
+  const Line line = cut_line<BN, 128>(a, bm_log, prefix, false, scan, false);
   {
     uint32_t sum = 0;
 #pragma unroll 1

@@ -49,7 +49,7 @@ struct TcCfg {
   // the turn buffer, for the barriers and the prefix of up to 196 sequences. (More slots than four
   // only lengthen every other load's way through memory: at the card's rate 148 x 2 x 64 KB in flight
   // are 3 us already.)
-  static size_t smem(int batch) { return kQ + kTurn + kSlots * (size_t)kItem + kBars + 4 * (size_t)(batch + 1); }
+  static size_t smem(int batch) { return kQ + kTurn + kSlots * (size_t)kItem + kBars + prefix_bytes(batch); }
 };
 
 struct TcBars {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
   }
   pdl_launch_dependents();
   tc_fence_before();
-  const Line line = cut_line<BN, kTcThreads>(a, __builtin_ctz(BM), prefix, (uint32_t*)qs, blockIdx.x == 0);  // with CTA barriers
+  const Line line = cut_line<BN, kTcThreads>(a, __builtin_ctz(BM), prefix, true, (uint32_t*)qs, blockIdx.x == 0);  // with CTA barriers
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
   const uint32_t tO = tmem, tS = tmem + DP;  // S of phase q at tS + 64 (q & 1), and its P in its place
@@ -478,6 +478,9 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
             for (int k = 0; k < 64; ++k)
               if (!(see >> k & 1u)) x[k >> 5][k & 31] = -INFINITY;
           }
+          tc_st32(at, *(const uint32_t(*)[32])x[0]);
+          tc_st32(at + 32, *(const uint32_t(*)[32])x[1]);
+          tc_wait_st();
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -496,12 +499,15 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         // P over S: of each 32 keys 16 columns of high parts, 16 of low ones. Two elements an
         // instruction where there is one for F32 pairs.
         float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 32) {
+          float xc[32];
           uint32_t p[32];
+          tc_ld32(at + c, xc);
+          tc_wait_ld();
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const float2 y = __ffma2_rn(make_float2(x[c][2 * k], x[c][2 * k + 1]), make_float2(sc, sc), make_float2(-base, -base));
+            const float2 y = __ffma2_rn(make_float2(xc[2 * k], xc[2 * k + 1]), make_float2(sc, sc), make_float2(-base, -base));
             const float2 v = make_float2(soft_exp<T>(y.x), soft_exp<T>(y.y));
             sum = __fadd2_rn(sum, v);
             p[k] = tc_pack(v.x, v.y, (T*)nullptr);
@@ -509,7 +515,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
             const float2 rest = __fadd2_rn(v, make_float2(-h.x, -h.y));
             p[16 + k] = tc_pack(rest.x, rest.y, (T*)nullptr);
           }
-          tc_st32(at + 32 * c, p);
+          tc_st32(at + c, p);
         }
         l += sum.x + sum.y;
         if (rescale && t > 0) {
