@@ -18,7 +18,6 @@ using namespace pp;
 
 namespace pp {
 
-constexpr int kBeamThreads = 256;
 constexpr int kBeamMax = 64;         // beams, k
 constexpr int kBeamList = 1024;      // keys of a slice at or above its bound
 constexpr int kMergeWarps = 16;
@@ -65,14 +64,14 @@ __device__ __forceinline__ uint64_t warp_max_u64(uint64_t v) {
 }
 
 // One slice of one row: grid (slices, rows); a thread holds PER logits, in 16-byte units adjacent
-// over the threads. A bound that at least k logits reach: the k-th largest among the maxima of G >= k
-// groups (G = 32: lane l of all warps; G = 256: every thread). Logits at or above the bound, k and a
+// over the NT threads. A bound that at least k logits reach: the k-th largest among the maxima of G >= k
+// groups (G = 32: lane l of all warps; G = NT: every thread). Logits at or above the bound, k and a
 // few more, are gathered as keys and put in order by counting. Only where more than kBeamList logits
 // are equal at the bound (a slice of constants) are the k best found one by one.
-template <typename T, int G, int PER>
-__global__ void __launch_bounds__(kBeamThreads) pp_beam_rows_kernel(const BeamArgs a) {
-  constexpr int W = kBeamThreads / 32, V = 16 / (int)sizeof(T), U = PER / V, SLICE = kBeamThreads * PER;
-  __shared__ uint32_t s_top[kBeamThreads];
+template <typename T, int G, int PER, int NT>
+__global__ void __launch_bounds__(NT) pp_beam_rows_kernel(const BeamArgs a) {
+  constexpr int W = NT / 32, V = 16 / (int)sizeof(T), U = PER / V, SLICE = NT * PER;
+  __shared__ uint32_t s_top[NT];
   __shared__ SliceSum s_part[W];
   __shared__ int s_n;
   __shared__ uint64_t s_keys[kBeamList];
@@ -89,7 +88,7 @@ __global__ void __launch_bounds__(kBeamThreads) pp_beam_rows_kernel(const BeamAr
   const bool wide = ((uintptr_t)src & 15) == 0;
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const int e = (i * kBeamThreads + tid) * V;
+    const int e = (i * NT + tid) * V;
     if (wide && e + V <= n) {
       const uint4 raw = __ldcs((const uint4*)(src + e));
       const T* p = (const T*)&raw;
@@ -100,7 +99,7 @@ __global__ void __launch_bounds__(kBeamThreads) pp_beam_rows_kernel(const BeamAr
       for (int q = 0; q < V; ++q) x[i * V + q] = e + q < n ? Elem<T>::get(src[e + q]) : -INFINITY;
     }
   }
-  auto token = [&](int i) { return (uint32_t)(first + ((i / V) * kBeamThreads + tid) * V + i % V); };
+  auto token = [&](int i) { return (uint32_t)(first + ((i / V) * NT + tid) * V + i % V); };
 
   float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -190,20 +189,20 @@ __global__ void __launch_bounds__(kBeamThreads) pp_beam_rows_kernel(const BeamAr
   const int cnt = s_n;
   uint64_t* out = a.keys + slice * a.k;
   if (cnt <= kBeamList) {
-    for (int i = tid; i < cnt; i += kBeamThreads) {
+    for (int i = tid; i < cnt; i += NT) {
       const uint64_t mine = s_keys[i];
       int rank = 0;
       for (int g = 0; g < cnt; ++g) rank += s_keys[g] > mine;
       if (rank < a.k) out[rank] = mine;
     }
-    for (int i = cnt + tid; i < a.k; i += kBeamThreads) out[i] = 0;
+    for (int i = cnt + tid; i < a.k; i += NT) out[i] = 0;
   } else {
     uint64_t last = ~0ull;
 #pragma unroll 1
     for (int r = 0; r < a.k; ++r) {
       uint64_t best = 0;
 #pragma unroll 1
-      for (int e = tid; e < n; e += kBeamThreads) {
+      for (int e = tid; e < n; e += NT) {
         const uint64_t key = beam_key(Elem<T>::get(src[e]), (uint32_t)(first + e));
         if (key < last && key > best) best = key;
       }
@@ -367,30 +366,35 @@ __global__ void __launch_bounds__(32 * kMergeWarps) pp_beam_merge_kernel(const B
   }
 }
 
+constexpr uint32_t kSliceLarge = 128 * 32, kSliceSmall = 256 * 8;
 struct BeamWork {
   uint64_t sums, keys, total;
-  uint32_t per, slices;
+  uint32_t slices;
+  bool wide;
   BeamWork(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k) {
     const uint64_t rows = (uint64_t)groups * beams;
-    // 32 logits a thread; 8, so that more CTAs share it, where that is not two a SM.
-    per = rows * ((vocab + 32ull * kBeamThreads - 1) / (32ull * kBeamThreads)) >= 2 * 148 ? 32 : 8;
-    slices = (uint32_t)((vocab + (uint64_t)per * kBeamThreads - 1) / ((uint64_t)per * kBeamThreads));
+    // Slices of 4096 logits, 32 of each of 128 threads; where those are not four an SM, of 2048, 8 of
+    // each of 256, so that more warps share the work (256 rows of 151936: 38.3 us, of 8192 logits by 256
+    // threads 43, of 2048 78; 4 rows: 9.0 us in 2048s, 11.9 in 4096s).
+    const uint64_t large = (vocab + kSliceLarge - 1) / kSliceLarge;
+    wide = rows * large >= 4 * 148;
+    slices = (uint32_t)(wide ? large : (vocab + kSliceSmall - 1) / kSliceSmall);
     sums = 0;
     keys = rows * slices * sizeof(SliceSum);
     total = keys + rows * slices * k * 8;
   }
 };
 
-template <typename T, int PER>
+template <typename T, int PER, int NT>
 void launch_rows(const BeamArgs& a, dim3 grid, cudaStream_t st) {
   // Up to 16 of a slice: 32 groups; above, a group per thread.
-  if (a.k <= 16) pp_beam_rows_kernel<T, 32, PER><<<grid, kBeamThreads, 0, st>>>(a);
-  else pp_beam_rows_kernel<T, kBeamThreads, PER><<<grid, kBeamThreads, 0, st>>>(a);
+  if (a.k <= 16) pp_beam_rows_kernel<T, 32, PER, NT><<<grid, NT, 0, st>>>(a);
+  else pp_beam_rows_kernel<T, NT, PER, NT><<<grid, NT, 0, st>>>(a);
 }
 template <typename T>
-void launch_rows(const BeamArgs& a, uint32_t per, dim3 grid, cudaStream_t st) {
-  if (per == 32) launch_rows<T, 32>(a, grid, st);
-  else launch_rows<T, 8>(a, grid, st);
+void launch_rows(const BeamArgs& a, bool wide, dim3 grid, cudaStream_t st) {
+  if (wide) launch_rows<T, 32, 128>(a, grid, st);
+  else launch_rows<T, 8, 256>(a, grid, st);
 }
 
 }  // namespace pp
@@ -439,9 +443,9 @@ extern "C" pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t 
   a.err = err;
   const cudaStream_t st = (cudaStream_t)stream;
   const dim3 grid(a.slices, groups * beams);
-  if (dtype == PP_F32) launch_rows<float>(a, w.per, grid, st);
-  else if (dtype == PP_BF16) launch_rows<__nv_bfloat16>(a, w.per, grid, st);
-  else launch_rows<__half>(a, w.per, grid, st);
+  if (dtype == PP_F32) launch_rows<float>(a, w.wide, grid, st);
+  else if (dtype == PP_BF16) launch_rows<__nv_bfloat16>(a, w.wide, grid, st);
+  else launch_rows<__half>(a, w.wide, grid, st);
   const pp_status r = launch_status("pp_beam_select");
   if (r != PP_OK) return r;
   const size_t base = (size_t)beams * k * 8 + (size_t)beams * 8, copy = (size_t)a.slices * k * 8;

@@ -30,7 +30,7 @@ struct AppendArgs {
   uint32_t* err;
 };
 
-constexpr int kAppendThreads = 256;
+constexpr int kAppendThreads = 128, kAppendAnyThreads = 256;
 
 // cos and sin of position * inv_freq. The angle in turns is formed in 64 bits and reduced to
 // (-0.5, 0.5] before it is rounded, so the error stays near 2^-24 of a turn up to positions of
@@ -78,7 +78,7 @@ __device__ __forceinline__ RowPlace place_row(const AppendArgs& a, int t, int la
 // rotated dims lane j holds both halves' run j, so that a pair never leaves its lane, of the others 8
 // in a row (interleaved pairs: all dims 8 in a row). kAppendAhead heads a lane are in flight at once,
 // the first of them before the row's place is known.
-constexpr int kAppendAhead = 4;
+constexpr int kAppendAhead = 2;
 template <typename TI, typename TC>
 __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendArgs a) {
   __shared__ float2 cs_all[kAppendThreads / 32][128];
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendA
 // The same for rows whose pointers, strides or rotation do not fit 8-element units: a warp per
 // head, lane l the dims l, l + 32, ...
 template <typename TI, typename TC>
-__global__ void __launch_bounds__(kAppendThreads) pp_append_any_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendAnyThreads) pp_append_any_kernel(const AppendArgs a) {
   __shared__ float2 cs[128];
   __shared__ RowPlace place;
   const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -413,15 +413,19 @@ void launch_append(const AppendArgs& a, bool vec, int rows, cudaStream_t st, int
     // Few rows: a row's heads over several warps, one head a lane group at the least, as long as the
     // warps do not pass eight an SM.
     const int per = 32 / a.tph;
-    int y = (heads + per - 1) / per;
-    while (y > 1 && (int64_t)rows * y > 8 * (int64_t)sms) y = (y + 1) / 2;
+    // Many rows: 8 passes of a warp (8192 rows of 48 heads: by 24 passes 55.5 us, 12 49.0, 8 48.5, 6
+    // 50.0, 4 52.7).
+    const int passes = (heads + per - 1) / per, least = (passes + 7) / 8;
+    int y = passes;
+    while (y > least && (int64_t)rows * y > 8 * (int64_t)sms) y = (y + 1) / 2;
+    if (y < least) y = least;
     const dim3 grid((rows + kAppendThreads / 32 - 1) / (kAppendThreads / 32), y);
     pp_append_kernel<TI, TC><<<grid, kAppendThreads, 0, st>>>(a);
     return;
   }
   int y = (heads + 7) / 8;
   while (y > 1 && (int64_t)rows * y > 2 * (int64_t)sms) --y;
-  pp_append_any_kernel<TI, TC><<<dim3(rows, y), kAppendThreads, 0, st>>>(a);
+  pp_append_any_kernel<TI, TC><<<dim3(rows, y), kAppendAnyThreads, 0, st>>>(a);
 }
 template <typename TI>
 void launch_append_to(const AppendArgs& a, uint32_t cache, bool vec, int rows, cudaStream_t st,
