@@ -240,7 +240,16 @@ __global__ void __launch_bounds__(32 * kMergeWarps) pp_beam_merge_kernel(const B
     const bool fin = a.finished && a.finished[row];
     bool bad = !(score < INFINITY);
     double lse = 0;
+    const uint64_t* keys = a.keys + row * a.slices * a.k;
     if (!fin) {
+      // A copy of the row's keys in shared memory where it fits (a pop then waits for shared memory,
+      // not for L2), on its way while lse is formed.
+      if (a.staged) {
+        uint64_t* mine = s_stage + (int64_t)warp * a.slices * a.k;
+        for (int i = lane; i < a.slices * a.k; i += 32)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(mine + i)), "l"(keys + i) : "memory");
+        keys = mine;
+      }
       const SliceSum* sums = a.sums + row * a.slices;
       float m = -INFINITY;
       for (int s = lane; s < a.slices; s += 32) m = fmaxf(m, __ldcg((const float2*)&sums[s]).x);
@@ -254,6 +263,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) pp_beam_merge_kernel(const B
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       bad |= isnan(sum);
       lse = (double)m + log(sum);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
     }
     if (bad && lane == 0 && a.err) atomicOr(a.err, PAGED_NONFINITE);
     const int state = bad || score == -INFINITY ? 2 : fin ? 1 : 0;
@@ -262,15 +273,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) pp_beam_merge_kernel(const B
       s_lse[b] = lse;
     }
     if (state != 0) continue;
-    // The row's k best keys, from a copy in shared memory where it fits (a pop then waits for
-    // shared memory, not for L2).
-    const uint64_t* keys = a.keys + row * a.slices * a.k;
-    if (a.staged) {
-      uint64_t* mine = s_stage + (int64_t)warp * a.slices * a.k;
-      for (int i = lane; i < a.slices * a.k; i += 32) mine[i] = keys[i];
-      __syncwarp();
-      keys = mine;
-    }
+    // The row's k best keys.
     if (a.slices <= 32 * kCursors) {
       int at[kCursors] = {};
       uint64_t head[kCursors];
