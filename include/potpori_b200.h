@@ -326,9 +326,11 @@ pp_status pp_shard_read_taps(pp_shard* shard, uint32_t m, float* f32, uint16_t* 
  * of their own. Arguments that the host can see are checked before the launch (PP_E_INVALID,
  * PP_E_UNSUPPORTED; message in pp_last_error(NULL)). What only the device sees is checked there:
  * *err (device memory, zero before the call, or NULL) gets bit value 1 when a length or a page table
- * entry points outside the table or the cache. Such a position is neither read nor written, and
- * a sequence whose kv_len is below its number of rows or above table_stride * page_size is left
- * out whole; value 4 when a bounded wait on the device expired (the output is then undefined). No call reads a position at or past kv_len, whatever the page holds there. */
+ * entry points outside the table or the cache, or cu_rows outside the row arrays. Such a position is
+ * neither read nor written, and a sequence whose kv_len is below its number of rows or above
+ * table_stride * page_size is left out whole (its output rows keep what they held); value 4 when a
+ * bounded wait on the device expired (the output is then undefined). No call reads a position at or
+ * past kv_len, whatever the page holds there. */
 
 /* A cache: `layers` layers of n_pages pages of page_size positions. Element (layer, page, row,
  * head, dim) of K is at k + layer * layer_stride + page * page_stride + row * row_stride +
@@ -348,9 +350,10 @@ typedef struct pp_paged_cache {
  * the call's row arrays, n_b of them (0 is fine), which are the last n_b of its kv_len[b] cached
  * positions; position s is row s % page_size of page page_table[b * table_stride + s / page_size].
  * cu_rows ([batch + 1], not decreasing, cu_rows[0] = 0), kv_len ([batch]) and page_table are
- * device memory. `rows` bounds cu_rows[batch]: rows of the arrays past cu_rows[batch] are padding
- * and are neither read nor written. max_rows and max_len are the host's bounds on n_b and kv_len:
- * they choose kernels and grids, results do not depend on them. batch <= 4096. */
+ * device memory. `rows` is the length of the row arrays: rows past cu_rows[batch] are padding and
+ * are neither read nor written. max_rows and max_len are the host's bounds on n_b and kv_len: they
+ * choose kernels and grids, and results depend on them by rounding alone. batch <= 4096,
+ * rows <= 2^24. */
 typedef struct pp_paged_batch {
   uint32_t batch, rows, max_rows, max_len, table_stride;
   const int32_t* cu_rows;
@@ -411,7 +414,9 @@ typedef struct pp_tree_query {
  * row that sees nothing gives zeros. NaN and infinities in K or V of unseen positions have no
  * effect. Nodes past 32 * mask_words are unseen. The result of a row does not depend on
  * atomics' order: equal calls give equal bits. `work` (16-byte aligned) holds the partial results
- * of split caches: at least pp_tree_attention_work_bytes. */
+ * of split caches: at least pp_tree_attention_work_bytes (0: the arguments are refused). Limits:
+ * n_heads <= 1024 n_kv_heads; max_rows <= 2^20; table_stride * page_size < 2^31; and
+ * (rows * n_heads / n_kv_heads / 4 + batch) * n_kv_heads * (table_stride * page_size / 32 + 1) < 2^31. */
 uint64_t pp_tree_attention_work_bytes(const pp_paged_cache* cache, const pp_paged_batch* batch,
                                       uint32_t n_heads);
 pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_paged_batch* batch,

@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kCommitThreads) pp_tree_commit_kernel(const Co
   const int b = blockIdx.y, tid = threadIdx.x;
   const int first = a.b.cu_rows[b], n = a.b.cu_rows[b + 1] - first, len = a.b.kv_len[b];
   const bool lead = blockIdx.x == 0;
-  const bool bad = n < 0 || n > a.max_rows || len < n ||
+  const bool bad = n < 0 || n > a.max_rows || len < n || first < 0 || first > a.b.rows - n ||
                    (int64_t)len > (int64_t)a.b.table_stride * a.c.page.d;
   if (n <= 0 || bad) {
     if (lead) {

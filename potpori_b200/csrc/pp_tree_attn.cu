@@ -696,7 +696,7 @@ inline const char* tree_problem(const pp_paged_cache* c, const pp_paged_batch* b
   if (const char* m = batch_problem(b)) return m;
   if (n_heads == 0 || n_heads % c->n_kv_heads || n_heads / c->n_kv_heads > 1024)
     return "n_heads must be a multiple of n_kv_heads, at most 1024 times it";
-  if (b->max_rows > (1u << 20)) return "max_rows out of range";
+  if (b->max_rows > (uint32_t)kTreeMostRows) return "max_rows out of range";
   // The line of tiles is counted in 32 bits, whatever the device's lengths turn out to be.
   const uint64_t G = n_heads / c->n_kv_heads;
   const uint64_t units = ((uint64_t)b->rows * G / 4 + b->batch) * c->n_kv_heads;

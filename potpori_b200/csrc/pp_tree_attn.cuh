@@ -16,6 +16,8 @@
 
 namespace pp {
 
+constexpr int kTreeMostRows = 1 << 20;  // of a sequence: times the group they stay below 2^31
+
 struct TreeArgs {
   PagedView c;  // the layer
   BatchView b;
@@ -37,9 +39,9 @@ struct TreeArgs {
   uint32_t* err;
 };
 
-// A sequence whose lengths do not fit its table is left out.
-__device__ __forceinline__ bool bad_sequence(const TreeArgs& a, int n, int len) {
-  return n < 0 || len < n || (int64_t)len > (int64_t)a.b.table_stride * a.c.page.d;
+// A sequence whose rows do not fit the arrays or whose lengths do not fit its table is left out.
+__device__ __forceinline__ bool bad_sequence(const TreeArgs& a, int first, int n, int len) {
+  return n < 0 || n > kTreeMostRows || first < 0 || first > a.b.rows - n || len < n || (int64_t)len > (int64_t)a.b.table_stride * a.c.page.d;
 }
 
 // Sequences up to which a line may be put in order.
@@ -66,9 +68,9 @@ __device__ __forceinline__ Line cut_line(const TreeArgs& a, int bm_log, uint32_t
   uint32_t* order = prefix + B + 1;
   // Units of a sequence, and its tiles
   auto units_of = [&](int b, uint32_t& tiles, bool report) {
-    const int n = a.b.cu_rows[b + 1] - a.b.cu_rows[b], len = a.b.kv_len[b];
+    const int first = a.b.cu_rows[b], n = a.b.cu_rows[b + 1] - first, len = a.b.kv_len[b];
     tiles = 0;
-    if (bad_sequence(a, n, len)) {
+    if (bad_sequence(a, first, n, len)) {
       if (report && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
       return 0u;
     }

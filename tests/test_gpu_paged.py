@@ -427,6 +427,58 @@ def test_tree_attention_splits_agree(gpu, dt, G):
         assert torch.equal(cache.tree_attention(batch, q, mask=mask), got)
 
 
+@pytest.mark.parametrize("dt,heads,bound", [(BF16, 4, 40), (F16, 16, FAR), (F32, 4, 40)])
+def test_rows_past_the_arrays(gpu, dt, heads, bound):
+    """cu_rows that reaches past the row arrays, or before them: that sequence is left out, by the
+    attention and by the commit."""
+    from potpori_b200.paged import PagedBatch
+
+    rng = rng_of(24)
+    cache, batch, table = make(rng, [40, 40, 40], [2, 2, 2], 16, 2, 128, dt, bound=bound)
+    q = torch.randn(6, heads, 128, generator=rng).to(dt).cuda()
+    want = cache.tree_attention(batch, q)
+    ints = torch.zeros(6, dtype=torch.int32).cuda()
+    for cu, left in (([0, 2, 4, 8], slice(4, 6)), ([0, 2, 4, 2 ** 31 - 1], slice(4, 6)), ([-2, 2, 4, 6], slice(0, 2))):
+        b = PagedBatch(batch.page_table, batch.lengths, torch.tensor(cu, dtype=torch.int32).cuda(), 8, bound)
+        out = torch.full_like(q, 7.0)
+        cache.tree_attention(b, q, out=out)
+        with pytest.raises(PPError):
+            cache.check()
+        keep = torch.ones(6, dtype=torch.bool, device="cuda")
+        keep[left] = False
+        assert torch.equal(out[keep], want[keep]) and (out[left] == 7.0).all()
+        path, accepted, correction, new_len = cache.tree_commit(b, ints, ints - 1, ints + 1)
+        with pytest.raises(PPError):
+            cache.check()
+        off = left.start // 2
+        assert [int(x) for x in (accepted[off], correction[off], new_len[off])] == [0, -1, 40]
+        assert (path[off] == -1).all() and all(int(path[b, 0]) == 0 for b in range(3) if b != off)
+
+
+@pytest.mark.parametrize("dt,G,bound", [(BF16, 1, None), (BF16, 4, FAR), (F16, 5, FAR), (F32, 2, None)])
+@pytest.mark.parametrize("long", [3000, 260])
+def test_tree_attention_ragged_batch(gpu, dt, G, bound, long):
+    """Many short sequences around a long one: CTAs that take parts of several units, or (none much
+    longer than the rest) whole units by falling length."""
+    rng = rng_of(25)
+    B = 30
+    rows = [int(torch.randint(0, 21, (1,), generator=rng)) if dt != BF16 or G > 1 else 1 for _ in range(B)]
+    lengths = [n + int(torch.randint(100, 240, (1,), generator=rng)) for n in rows]
+    rows[17], lengths[17] = max(rows[17], 1), long
+    cache, batch, table = make(rng, lengths, rows, 16, 4, 64, dt, bound=bound)
+    parents = [ref.random_parents(rng, n) for n in rows]
+    seen = [ref.tree_seen(p, lengths[b] - rows[b]) for b, p in enumerate(parents)]
+    bits = [s[i, lengths[b] - rows[b]:].nonzero()[:, 0].tolist() for b, s in enumerate(seen) for i in range(rows[b])]
+    mask = ref.mask_words(bits, 1).cuda()
+    T = sum(rows)
+    q = (2 * torch.randn(T, 4 * G, 64, generator=rng)).to(dt).cuda()
+    lse = torch.empty(T, 4 * G, device="cuda")
+    got = cache.tree_attention(batch, q, mask=mask, lse=lse)
+    cache.check()
+    check_attention(cache, table, "nhd", 16, rows, lengths, seen, q, got, lse, 64 ** -0.5)
+    assert torch.equal(cache.tree_attention(batch, q, mask=mask), got)
+
+
 def test_large_batch(gpu):
     """More sequences than a CTA has threads, many without rows."""
     rng = rng_of(14)
