@@ -72,27 +72,27 @@ __device__ __forceinline__ RowPlace place_row(const AppendArgs& a, int t, int la
   return r;
 }
 
-// A warp per row and share of its heads; nothing is shared between warps, so that the row's chain of
-// dependent loads (sequence, length, page) of one hides behind the copies of others. The warp forms
-// the row's rotary_dim / 2 angles once. tph lanes take a head, 8 dims each, as two runs of 4: of the
+// A CTA of one to four warps per row and share of its heads: one warp finds the row's place, all form
+// its rotary_dim / 2 angles once. tph lanes take a head, 8 dims each, as two runs of 4: of the
 // rotated dims lane j holds both halves' run j, so that a pair never leaves its lane, of the others 8
 // in a row (interleaved pairs: all dims 8 in a row). kAppendAhead heads a lane are in flight at once,
-// the first of them before the row's place is known.
+// the first of them before the row's place is known. Many rows are bound by the instructions issued
+// (two thirds of the slots where each warp formed the angles for itself), then by the bytes.
 constexpr int kAppendAhead = 2;
 template <typename TI, typename TC>
 __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendArgs a) {
-  __shared__ float2 cs_all[kAppendThreads / 32][128];
+  __shared__ float2 cs[128];
+  __shared__ RowPlace s_place;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t = blockIdx.x * (kAppendThreads / 32) + warp;
-  if (t >= a.b.rows) return;
-  float2* cs = cs_all[warp];
+  const int t = blockIdx.x;
   const int D = a.c.head_dim, K = a.c.n_kv, heads = a.nh + 2 * K;
   const int per = 32 / a.tph, j = lane % a.tph;
   const bool dims = 8 * j < D, turns = 8 * j < a.rot;
   const int d0 = turns && !a.interleaved ? 4 * j : 8 * j;
   const int d1 = turns && !a.interleaved ? a.rot / 2 + 4 * j : 8 * j + 4;
-  const int step = per * gridDim.y;
-  int slot = blockIdx.y * per + lane / a.tph;
+  const int share = blockIdx.y * (blockDim.x >> 5) + warp, step = per * gridDim.y * (blockDim.x >> 5);
+  int slot = share * per + lane / a.tph;
+  const float inv_dim = 1.f / (float)D;
   float x[kAppendAhead][8];
   auto fetch = [&](int first) {
 #pragma unroll
@@ -112,16 +112,26 @@ __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendA
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
   fetch(slot);
-  const RowPlace place = place_row(a, t, lane, blockIdx.y == 0);
+  if (warp == 0) {
+    const RowPlace p = place_row(a, t, lane, blockIdx.y == 0);
+    if (lane == 0) s_place = p;
+  }
+  __syncthreads();
+  const RowPlace place = s_place;
   if (!place.in_batch) return;
-  for (int i = lane; i < a.rot / 2; i += 32) cs[i] = rotation(place.pos, a.inv_freq[i]);
-  __syncwarp();
+  for (int i = threadIdx.x; i < a.rot / 2; i += blockDim.x) cs[i] = rotation(place.pos, a.inv_freq[i]);
+  __syncthreads();
   float2 r[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) r[i] = turns ? cs[4 * j + i] : make_float2(1.f, 0.f);
 
+  const float* held = nullptr;  // the norm's weights in wv
+  float wv[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) wv[i] = 0.f;
+
 #pragma unroll 1
-  for (int s0 = blockIdx.y * per; s0 < heads; s0 += kAppendAhead * step, slot += kAppendAhead * step) {
+  for (int s0 = share * per; s0 < heads; s0 += kAppendAhead * step, slot += kAppendAhead * step) {
 #pragma unroll
     for (int u = 0; u < kAppendAhead; ++u) {
       const int h = slot + u * step;
@@ -134,9 +144,12 @@ __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendA
         for (int i = 0; i < 8; ++i) ss += x[u][i] * x[u][i];
         for (int o = a.tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         if (live && w) {
-          const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
-          const float4 w0 = *(const float4*)(w + d0), w1 = *(const float4*)(w + d1);
-          const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+          if (w != held) {
+            held = w;
+            load_n<float, 4>(w + d0, wv);
+            load_n<float, 4>(w + d1, wv + 4);
+          }
+          const float inv = rsqrtf(ss * inv_dim + a.eps);
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[u][i] = x[u][i] * inv * wv[i];
         }
@@ -410,17 +423,13 @@ template <typename TI, typename TC>
 void launch_append(const AppendArgs& a, bool vec, int rows, cudaStream_t st, int sms) {
   const int heads = a.nh + 2 * a.c.n_kv;
   if (vec) {
-    // Few rows: a row's heads over several warps, one head a lane group at the least, as long as the
-    // warps do not pass eight an SM.
-    const int per = 32 / a.tph;
-    // Many rows: 8 passes of a warp (8192 rows of 48 heads: by 24 passes 55.5 us, 12 49.0, 8 48.5, 6
-    // 50.0, 4 52.7).
-    const int passes = (heads + per - 1) / per, least = (passes + 7) / 8;
-    int y = passes;
-    while (y > least && (int64_t)rows * y > 8 * (int64_t)sms) y = (y + 1) / 2;
-    if (y < least) y = least;
-    const dim3 grid((rows + kAppendThreads / 32 - 1) / (kAppendThreads / 32), y);
-    pp_append_kernel<TI, TC><<<grid, kAppendThreads, 0, st>>>(a);
+    // Up to four warps a row, with equal numbers of passes. Few rows: over several CTAs, a pass a warp at
+    // the least, as long as the warps do not pass eight an SM.
+    const int per = 32 / a.tph, passes = (heads + per - 1) / per;
+    const int rounds = (passes + 3) / 4, warps = (passes + rounds - 1) / rounds;
+    int y = rounds;
+    while (y > 1 && (int64_t)rows * y * warps > 8 * (int64_t)sms) y = (y + 1) / 2;
+    pp_append_kernel<TI, TC><<<dim3(rows, y), 32 * warps, 0, st>>>(a);
     return;
   }
   int y = (heads + 7) / 8;
