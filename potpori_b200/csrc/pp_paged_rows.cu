@@ -75,12 +75,12 @@ __device__ __forceinline__ RowPlace place_row(const AppendArgs& a, int t, int la
 // A CTA of one to four warps per row and share of its heads: one warp finds the row's place, all form
 // its rotary_dim / 2 angles once. tph lanes take a head, 8 dims each, as two runs of 4: of the
 // rotated dims lane j holds both halves' run j, so that a pair never leaves its lane, of the others 8
-// in a row (interleaved pairs: all dims 8 in a row). kAppendAhead heads a lane are in flight at once,
-// the first of them before the row's place is known. Many rows are bound by the instructions issued
-// (two thirds of the slots where each warp formed the angles for itself), then by the bytes.
-constexpr int kAppendAhead = 2;
+// in a row (interleaved pairs: all dims 8 in a row). A lane's first head is on its way before the
+// row's place is known, the next one while this one leaves; more of them in flight, or more CTAs on an
+// SM, gained nothing (6400 rows of 48 heads: 48.8 us at 64 registers, 49.5 with three heads ahead, 50.2
+// with two, 53.8 at 32 registers: 4.8 TB/s of the 6.5 that a copy reaches).
 template <typename TI, typename TC>
-__global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 8) pp_append_kernel(const AppendArgs a) {
   __shared__ float2 cs[128];
   __shared__ RowPlace s_place;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -93,24 +93,18 @@ __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendA
   const int share = blockIdx.y * (blockDim.x >> 5) + warp, step = per * gridDim.y * (blockDim.x >> 5);
   int slot = share * per + lane / a.tph;
   const float inv_dim = 1.f / (float)D;
-  float x[kAppendAhead][8];
-  auto fetch = [&](int first) {
-#pragma unroll
-    for (int u = 0; u < kAppendAhead; ++u) {
-      const int h = first + u * step;
-      if (h >= heads || !dims) continue;
-      const TI* src;
-      if (h < a.nh) src = (const TI*)a.q + (int64_t)t * a.q_stride + h * D;
-      else if (h < a.nh + K) src = (const TI*)a.k + (int64_t)t * a.k_stride + (h - a.nh) * D;
-      else src = (const TI*)a.v + (int64_t)t * a.v_stride + (h - a.nh - K) * D;
-      load_n<TI, 4>(src + d0, x[u]);
-      load_n<TI, 4>(src + d1, x[u] + 4);
-    }
+  float x[8];
+  auto fetch = [&](int h) {
+    if (h >= heads || !dims) return;
+    const TI* src;
+    if (h < a.nh) src = (const TI*)a.q + (int64_t)t * a.q_stride + h * D;
+    else if (h < a.nh + K) src = (const TI*)a.k + (int64_t)t * a.k_stride + (h - a.nh) * D;
+    else src = (const TI*)a.v + (int64_t)t * a.v_stride + (h - a.nh - K) * D;
+    load_n<TI, 4>(src + d0, x);
+    load_n<TI, 4>(src + d1, x + 4);
   };
 #pragma unroll
-  for (int u = 0; u < kAppendAhead; ++u)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
   fetch(slot);
   if (warp == 0) {
     const RowPlace p = place_row(a, t, lane, blockIdx.y == 0);
@@ -131,51 +125,42 @@ __global__ void __launch_bounds__(kAppendThreads) pp_append_kernel(const AppendA
   for (int i = 0; i < 8; ++i) wv[i] = 0.f;
 
 #pragma unroll 1
-  for (int s0 = share * per; s0 < heads; s0 += kAppendAhead * step, slot += kAppendAhead * step) {
+  for (int s0 = share * per; s0 < heads; s0 += step, slot += step) {  // s0: the warp's first, so it stays together
+    const bool live = slot < heads && dims, isq = slot < a.nh, isv = slot >= a.nh + K;
+    const float* w = isq ? a.q_norm : isv ? nullptr : a.k_norm;
+    if (a.q_norm || a.k_norm) {  // per-head RMSNorm; the sum of squares over the head's lanes
+      float ss = 0.f;
 #pragma unroll
-    for (int u = 0; u < kAppendAhead; ++u) {
-      const int h = slot + u * step;
-      if (s0 + u * step >= heads) break;  // the same for the whole warp
-      const bool live = h < heads && dims, isq = h < a.nh, isv = h >= a.nh + K;
-      const float* w = isq ? a.q_norm : isv ? nullptr : a.k_norm;
-      if (a.q_norm || a.k_norm) {  // per-head RMSNorm; the sum of squares over the head's lanes
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[u][i] * x[u][i];
-        for (int o = a.tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (live && w) {
-          if (w != held) {
-            held = w;
-            load_n<float, 4>(w + d0, wv);
-            load_n<float, 4>(w + d1, wv + 4);
-          }
-          const float inv = rsqrtf(ss * inv_dim + a.eps);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[u][i] = x[u][i] * inv * wv[i];
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+      for (int o = a.tph >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (live && w) {
+        if (w != held) {
+          held = w;
+          load_n<float, 4>(w + d0, wv);
+          load_n<float, 4>(w + d1, wv + 4);
         }
-      }
-      if (turns && !isv) {
-        if (a.interleaved) {
+        const float inv = rsqrtf(ss * inv_dim + a.eps);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) turn(x[u][2 * i], x[u][2 * i + 1], r[i]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) turn(x[u][i], x[u][4 + i], r[i]);
-        }
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * wv[i];
       }
-      if (!live) continue;
-      TC* dst;
-      if (isq) {
-        dst = (TC*)a.q_out + ((int64_t)t * a.nh + h) * D;
-      } else {
-        if (place.offset < 0) continue;
-        const int hk = isv ? h - a.nh - K : h - a.nh;
-        dst = (TC*)((isv ? a.c.v : a.c.k) + place.offset + (int64_t)hk * a.c.head_bytes);
-      }
-      store_n<TC, 4>(dst + d0, x[u]);
-      store_n<TC, 4>(dst + d1, x[u] + 4);
     }
-    fetch(slot + kAppendAhead * step);
+    if (turns && !isv) {
+      if (a.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turn(x[2 * i], x[2 * i + 1], r[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turn(x[i], x[4 + i], r[i]);
+      }
+    }
+    if (live && (isq || place.offset >= 0)) {
+      const int hk = isv ? slot - a.nh - K : slot - a.nh;
+      TC* dst = isq ? (TC*)a.q_out + ((int64_t)t * a.nh + slot) * D
+                    : (TC*)((isv ? a.c.v : a.c.k) + place.offset + (int64_t)hk * a.c.head_bytes);
+      store_n<TC, 4>(dst + d0, x);
+      store_n<TC, 4>(dst + d1, x + 4);
+    }
+    fetch(slot + step);
   }
 }
 
