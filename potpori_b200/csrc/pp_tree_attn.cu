@@ -1,5 +1,6 @@
-// pp_tree_attention: the kernels for caches of 16-bit types (mma.sync) and of F32 (CUDA cores),
-// and the entry point. The work split and the join of partials are in pp_tree_attn.cuh.
+// pp_tree_attention: the kernels for few query vectors over caches of 16-bit types (mma.sync: the bytes
+// of the cache bound it) and for F32 caches (CUDA cores), the choice of kernel and the entry point. The
+// kernel for many query vectors is in pp_tree_tc.cu, the work split and the join in pp_tree_attn.cuh.
 #include <cuda_runtime.h>
 
 #include "../../include/potpori_b200.h"
@@ -14,22 +15,22 @@ namespace pp {
 // ---- 16-bit caches, few query vectors --------------------------------------------------------
 constexpr int kTreeThreads = 128;
 constexpr int kTreeBN = 64;
-// Caches of up to so many tiles are not cut: cutting a unit costs the join, 3 us of a call, and a
-// tile of the narrow, tcgen05 and F32 kernels takes about 0.5, 1.2 and 2 us in a lone CTA (8 heads: 256
-// positions narrow 8.2 us whole; 128 positions F32 8.2 us cut, 6.8 whole; 512 positions tcgen05 14.4
-// us cut, 20.3 whole).
-constexpr int kWholeNarrow = 8, kWholeTc = 2, kWholeF32 = 2;
-// Longer caches are not cut where that loads the fullest CTA with at most a quarter and so many tiles
-// more than equal shares would (16 ragged trees of 61 nodes, 8 heads, tcgen05: 64 tiles whole against 44
-// cut 97 us against 108, 16 against 12 35 against 54, 64 against 32 105 against 80; 36 x 1030 decoded
-// rows, narrow: 17 against 13 27.2 against 28.9, 33 against 22 43.9 against 40.4; F32: 10 against 7
-// 35.9 against 31.6, 33 against 22 100 against 83).
+// Caches of up to so many tiles are never cut, which saves the join's launch, about 1 us (one decoded
+// row, 8 heads, narrow: 256 positions 8.0 us whole against 8.6, 512 11.9 against 9.4; F32: 64 positions
+// 6.8 against 7.4, 128 10.9 against 7.2; 240 vectors, tcgen05: 128 positions 10.9 against 11.9).
+constexpr int kWholeNarrow = 4, kWholeTc = 2, kWholeF32 = 2;
+// Longer ones are not where that loads the fullest CTA with at most a quarter and so many tiles, or six
+// times the equal share, more (fullest CTA whole against equal share; ragged trees of 61 nodes, 8 heads,
+// tcgen05: 64 against 44 tiles 97 us against 108, 16 against 12 35 against 54, 8 against 2 18.8
+// against 23.1, 8 against 1 17.8 against 15.3, 24 against 5 36 against 30, 64 against 32 105 against 80; decoded rows,
+// narrow: 17 against 13 27.2 against 28.9, 4 against 1 9.5 against 10.7, 16 against 6 21.3 against 17.5;
+// F32: 3 against 2 14.0 against 14.4, 10 against 7 35.9 against 31.6).
 constexpr uint32_t kSlackNarrow = 3, kSlackTc = 12, kSlackF32 = 1;
 // More than 8 query vectors a head, the narrow kernel takes in tiles of 8, reading K and V again for
 // each from L2; it starts faster and its tiles are quicker, so it still leads up to this many of its
-// tiles a CTA (32 vectors, 8 heads: 2056 positions 17.2 us against tcgen05's 19.5, 8200 positions 27.5
-// against 29.3, 8 x 2056 34.5 against 32.0, 32 x 2056 106 against 62).
-constexpr uint64_t kNarrowTiles = 16;
+// tiles a CTA (32 vectors, 8 heads, narrow against tcgen05: 2056 positions 14.0 us against 17.3, 4104 18.1
+// against 21.1, 8200 24.6 against 23.8, 16392 40.7 against 30.5, 32 x 2056 102 against 64).
+constexpr uint64_t kNarrowTiles = 12;
 
 template <typename T>
 __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -94,7 +95,10 @@ __device__ __forceinline__ void narrow_copy(const TreeArgs& a, const RowFetch<16
 // products' M dimension and the vectors N, S^T = K Q^T and O^T = V^T P^T on mma.sync, half the
 // products and half the accumulators of a 16-row tile; at 8 rows the cache's bytes bound it, not the
 // tensor cores. A warp fetches (TMA, 16-row boxes) and consumes its own 16 keys of every 64-key
-// tile, so the loop has no CTA barrier. P^T turns from S^T's layout to an operand's by movmatrix.
+// tile, so the loop has no CTA barrier. P^T turns from S^T's layout to an operand's by movmatrix; it is
+// carried as two parts of the cache's type, hi + lo, for one alone would add as much error as the
+// rounding of the output. 64 decoded rows over 4096 to 8192 positions, 8 heads of 128, BF16, pages of 16:
+// 250 to 254 us for 1.63 GB, 6.4 to 6.5 TB/s, what a copy reaches; one row over 131072: 93 us, 5.8.
 __device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
@@ -368,7 +372,9 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
 // CUDA cores: on these tensor cores three products of split halves would be needed to keep F32,
 // at the rate of an F32 multiply-add and with a worse sum. BM query vectors (4 for a decoded token,
 // 16 else), 32-key tiles, four warps. Scores: warp w the rows w BM / 4 .., lane = key, so the softmax
-// of a row stays in its warp; output: thread = dim, all rows.
+// of a row stays in its warp; output: thread = dim, all rows. One row over 42 positions, 16 heads on 8:
+// 7.0 us, the chain of launch, lengths, page and rows; 48 rows over 515 to 1030: 83 us, 3.7 TB/s, the
+// multiply-adds and their shared-memory operands.
 constexpr int kTreeFBN = 32, kTreeFStages = 2;
 template <int DP, int BM>
 struct TreeFCfg {

@@ -11,6 +11,9 @@
 // unit writes its rows; where a unit spans CTAs each writes a partial (running maximum, sum,
 // unnormalised output) and a second kernel joins them in order (no atomics, so equal calls give
 // equal bits).
+// Lengths are read on the device, so a captured call follows new ones. What every call pays beside its
+// tiles: 1 to 2 us from the launch to the cut, 2 to 4 until the first keys are there, 3 to 5 for the
+// partials' way out and 3 to 8 for the join.
 #pragma once
 #include "pp_paged.cuh"
 
@@ -55,11 +58,12 @@ struct Line {
   const uint32_t* order;  // the sequences by falling length; null: as they come
 };
 // prefix[b] = places before sequence b on the line; prefix[batch] = all. A CTA takes equal shares of
-// the tiles, unless whole units load the fullest CTA with at most a quarter and `slack` tiles more: cutting
-// units costs second segments and the join, and keeps every SM's CTAs in each other's way to the end. Of whole
-// units the long ones come first where each has a CTA of its own: the first CTA of every SM then takes one
-// of them and the second one of the short ones. By the whole CTA (NT threads); a tile has 1 << bm_log rows; scan:
-// 3 NT / 32 words of shared memory.
+// the tiles, unless whole units load the fullest CTA with at most a quarter and `slack` tiles (or 6
+// times the share) more: cutting units costs second segments and the join, and keeps every SM's CTAs in
+// each other's way to the end. With `sort` whole units of long sequences come first where each unit has
+// a CTA of its own, so that they start on empty SMs and the short ones fill up (16 ragged trees of 61
+// nodes over 2048 to 4096 positions: 91.1 us against 92.7); `batch` words behind prefix then. By the
+// whole CTA (NT threads); a tile has 1 << bm_log rows; scan: 3 NT / 32 words of shared memory.
 template <int BN, int NT>
 __device__ __forceinline__ Line cut_line(const TreeArgs& a, int bm_log, uint32_t* prefix, bool sort, uint32_t* scan,
                                          bool report) {
@@ -85,7 +89,8 @@ __device__ __forceinline__ Line cut_line(const TreeArgs& a, int bm_log, uint32_t
     l.per = max((units + a.ctas - 1) / a.ctas, 1u);
     if (!a.whole) {
       const uint32_t per = max((tiles + a.ctas - 1) / a.ctas, 1u);
-      if ((uint64_t)l.per * longest > (uint64_t)per + per / 4 + a.slack) l = Line{tiles, per, false, nullptr};
+      const uint64_t slack = a.slack < 6ull * per ? a.slack : 6ull * per;
+      if ((uint64_t)l.per * longest > (uint64_t)per + per / 4 + slack) l = Line{tiles, per, false, nullptr};
     }
     return l;
   };
@@ -381,7 +386,9 @@ __device__ __forceinline__ void add_nonfinite(const TreeArgs& a, const Segment& 
 // size; 16 lanes take a row, DP / 16 dims each: of a unit with few partials an item is 8 rows, of one
 // with many a row, its partials dealt to the 8 groups. What the units are follows from the lengths
 // alone, so it is found while the attention's last CTAs still run: only the partials are waited for,
-// and read once, with a running maximum.
+// and read once, with a running maximum (with descriptors left by the attention and a pass for the
+// maximum first, the 37 partials of a tree of 24 over 131072 positions took 12 us behind the last CTA,
+// now 3 to 7; they are 20 MB from L2).
 constexpr int kJoinMany = 8;
 struct JoinUnit {
   int32_t parts, rows;  // partials (0: no unit), rows of the tile
