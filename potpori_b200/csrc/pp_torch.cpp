@@ -209,6 +209,7 @@ struct Cache {
     a.layer = (uint32_t)layer;
     if (mask) {
       const int64_t words = mask->dim() == 2 ? mask->size(1) : 0;
+      if (rows && words == 0) refuse("mask: [rows, words] int32 expected");
       a.mask = (const uint32_t*)pointer("mask", *mask, index, at::kInt, {rows, words});
       a.mask_words = (uint32_t)(words < INT32_MAX ? words : INT32_MAX);
     }

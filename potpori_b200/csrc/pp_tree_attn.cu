@@ -69,7 +69,7 @@ struct NarrowCfg {
   static constexpr int kOPitch = DP + 4;
   static_assert(4 * BM * (kOPitch * 4 + 8) <= kRing, "the warps' outputs take the ring's place");
   // Nothing is static, so that the dynamic part starts on the 1024 bytes that the swizzle counts from.
-  static constexpr int kBars = 4 * NS * 8;
+  static constexpr int kBars = 4 * NS * 8 + 12 * (kTreeThreads / 32);
   static size_t smem(int batch) { return kRing + kBars + prefix_bytes(batch); }
 };
 // Byte offset of 16-byte unit u (dims 8 u ..) of row r in a tile of it.
@@ -112,8 +112,8 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
   extern __shared__ __align__(1024) uint8_t narrow_smem[];
   uint8_t* sm = narrow_smem;
   uint64_t* full = (uint64_t*)(sm + C::kRing);  // [4][NS]
-  uint32_t* scan = (uint32_t*)sm;  // before anything is fetched
-  uint32_t* prefix = (uint32_t*)(full + 4 * NS);
+  uint32_t* scan = (uint32_t*)(full + 4 * NS);
+  uint32_t* prefix = scan + 3 * (kTreeThreads / 32);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g4 = lane >> 2, t4 = lane & 3;
   const int D = a.c.head_dim;
   const float sc = soft_scale<T>(a.scale);

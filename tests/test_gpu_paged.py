@@ -479,6 +479,15 @@ def test_tree_attention_ragged_batch(gpu, dt, G, bound, long):
     assert torch.equal(cache.tree_attention(batch, q, mask=mask), got)
 
 
+def test_masks_without_words_are_refused(gpu):
+    rng = rng_of(26)
+    cache, batch, _ = make(rng, [20], [3], 16, 2, 64, BF16)
+    q = torch.randn(3, 4, 64, generator=rng).bfloat16().cuda()
+    for mask in (torch.zeros(3, 0, dtype=torch.int32).cuda(), torch.zeros(3, dtype=torch.int32).cuda()):
+        with pytest.raises(PPError):
+            cache.tree_attention(batch, q, mask=mask)
+
+
 def test_large_batch(gpu):
     """More sequences than a CTA has threads, many without rows."""
     rng = rng_of(14)
