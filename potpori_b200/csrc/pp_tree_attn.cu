@@ -621,8 +621,8 @@ inline TreePlan tree_plan(const pp_paged_cache& c, const pp_paged_batch& b, uint
   return p;
 }
 
-// Tensor maps of the layer's K and V; box 0 (16-byte copies then) where they do not fit.
-inline TreeMaps tree_maps(const pp_paged_cache& c, const PagedView& v, int most) noexcept {
+// Tensor maps of the layer's K and V, boxes of least .. most rows; box 0 (16-byte copies then) where they do not fit.
+inline TreeMaps tree_maps(const pp_paged_cache& c, const PagedView& v, int least, int most) noexcept {
   TreeMaps m = {};
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -635,7 +635,7 @@ inline TreeMaps tree_maps(const pp_paged_cache& c, const PagedView& v, int most)
       p = nullptr;
     return (Encode)p;
   }();
-  if (!encode || c.dtype == PP_F32 || c.page_size % 16) return m;
+  if (!encode || c.dtype == PP_F32 || c.page_size % least) return m;
   int box = most;
   while (c.page_size % box) box >>= 1;
   // Heads, rows and pages by ascending stride; a dimension of one element takes any stride.
@@ -774,7 +774,7 @@ extern "C" pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_pag
     if (p.dp == 128) return run_tree_f32<128>(a, st);
     return run_tree_f32<256>(a, st);
   }
-  const TreeMaps m = tree_maps(*cache, a.c, p.tc ? 64 : 16);
+  const TreeMaps m = tree_maps(*cache, a.c, p.tc ? 8 : 16, p.tc ? 64 : 16);
   if (p.tc) return run_tree_tc(a, m, cache->dtype, p.dp, st);
   if (cache->dtype == PP_BF16) return run_tree_16<__nv_bfloat16>(a, m, p.dp, st);
   return run_tree_16<__half>(a, m, p.dp, st);

@@ -235,8 +235,8 @@ struct RingCursor {
   }
 };
 
-// K and V of the layer as tensor maps (TMA), for 16-bit caches with pages of a multiple of 16
-// positions: 64-dim boxes of `box` rows of one page, 128-byte swizzled. Dimension 0 is the head's dim;
+// K and V of the layer as tensor maps (TMA), for 16-bit caches with pages of a multiple of 8
+// positions (16 for the narrow kernel): 64-dim boxes of `box` rows of one page, 128-byte swizzled. Dimension 0 is the head's dim;
 // heads, rows and pages are the dimensions at_head, at_row and at_page in order of their strides.
 // A box at page n_pages is out of range and reads zeros: so do absent pages.
 struct TreeMaps {

@@ -5,11 +5,13 @@
 //
 // One CTA, 224 threads, two CTAs on an SM (one at head_dim 256), so that one's softmax runs under
 // the other's products:
-//  * warp 4, producer: the K and V tiles by TMA, in boxes of 16, 32 or 64 rows of one page, into a
-//    ring of tile-sized slots, in the order in which the products need them (K0, K1, V0, K2, V1, ...).
+//  * warps 4 and 5, producers: the K and V tiles by TMA, in boxes of 8 to 64 rows of one page and 64
+//    dims, into a ring of tile-sized slots, in the order in which the products need them (K0, K1, V0,
+//    K2, V1, ...). A box costs some 54 clocks whatever its size (the trees below: pages of 64
+//    positions 89 us, 32 92, 16 119, 24, in boxes of 8, 165; 24 row by row 265).
 //    A slot holds 64-dim blocks of 64 rows x 128 bytes, the 16-byte unit u of row r at u ^ (r & 7):
 //    read K-major it is the B operand of Q K^T, read MN-major the B operand of P V. Where pages are
-//    not multiples of 16 positions, warps 4 and 5 fetch row by row with 16-byte asynchronous copies.
+//    not multiples of 8 positions, warps 4 and 5 fetch row by row with 16-byte asynchronous copies.
 //  * warp 6, one thread: S = Q K^T (128 x 64, both operands in shared memory) and O += P V (P in
 //    TMEM), each returned by a commit on an mbarrier. S has two places, and P takes its S's: S of a
 //    tile is issued while the softmax works on the tile before, when the product of the one before
@@ -23,7 +25,7 @@
 // What bounds it: a tile's way through the softmax. Of 2000 to 2200 clocks a tile and CTA (two CTAs on
 // the SM) 950 to 1150 are the exponentials and the two parts of P (64 exponentials a thread are 512 clocks
 // of the SM's special units, and the other CTA wants them too), 250 to 380 the maximum, 470 to 570 the wait for S,
-// whose products share the tensor core, two thirds busy, with the other CTA's. Left out one by one, on
+// whose products share the tensor core, about half busy, with the other CTA's. Left out one by one, on
 // trial, neither half of the products nor the exponentials nor memory gave more than 5 %; two softmax
 // warps a row were slower. 16 ragged trees of 61 nodes over 2048 to 4096 positions, 8 heads of 128, F16:
 // 91 us, 550 TFLOP/s; one tree of 24 over 131072, BF16: 109 us, 4.9 TB/s, of which the tiles run at
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
 
   if (tid == 0) {
     for (int i = 0; i < slots; ++i) {
-      mbar_init(&bars->full[i], maps.box ? 1 : 2);
+      mbar_init(&bars->full[i], maps.box && DP == 64 ? 1 : 2);
       mbar_init(&bars->free[i], 1);
     }
     mbar_init(&bars->q_full, 4);
@@ -207,9 +209,11 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
   cta_range(line, blockIdx.x, begin, end);
   bool ok = true;
 
-  if (warp == 4 && maps.box) {
-    // ---- producer, by TMA: lane g looks row group g of a tile up (box rows, one page)
-    constexpr int NB = DP / 64;
+  constexpr int kFetchers = DP == 64 ? 1 : 2;  // warps that fetch by TMA, each its share of the dims
+  if (warp >= 4 && warp < 4 + kFetchers && maps.box) {
+    // ---- producers, by TMA: lane g looks row group g of a tile up (box rows, one page)
+    constexpr int NB = DP / 64 / kFetchers;
+    const int i0 = (warp - 4) * NB;  // 64-dim blocks i0 .. i0 + NB - 1
     const int groups = BN / maps.box;
     int n = 0;
     RingCursor rc;
@@ -231,7 +235,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           break;
         }
         uint8_t* dst = ring + (size_t)slot * C::kItem;
-        if (elect_one()) mbar_arrive_expect_tx(&bars->full[slot], C::kItem);
+        if (elect_one()) mbar_arrive_expect_tx(&bars->full[slot], C::kItem / kFetchers);
         __syncwarp();
 #pragma unroll 1
         for (int g = 0; g < groups; ++g) {
@@ -240,7 +244,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
           if (elect_one())
 #pragma unroll
             for (int i = 0; i < NB; ++i)
-              tma_box(dst + i * (BN * 128) + g * maps.box * 128, isv ? &maps.v : &maps.k, &bars->full[slot], maps, 64 * i,
+              tma_box(dst + (i0 + i) * (BN * 128) + g * maps.box * 128, isv ? &maps.v : &maps.k, &bars->full[slot], maps, 64 * (i0 + i),
                       s.h, row, page);
           __syncwarp();
         }

@@ -488,6 +488,23 @@ def test_masks_without_words_are_refused(gpu):
             cache.tree_attention(batch, q, mask=mask)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 8, 12, 40])
+def test_tree_attention_small_pages(gpu, page, dim):
+    """Many vectors a head over pages that end inside a tile: by boxes of 8 rows, or row by row."""
+    rng = rng_of(27 + page)
+    rows, lengths = [40, 3], [333, 70]
+    cache, batch, table = make(rng, lengths, rows, page, 2, dim, F16, "hnd", bound=FAR)
+    parents = [ref.random_parents(rng, n) for n in rows]
+    seen = [ref.tree_seen(p, lengths[b] - rows[b]) for b, p in enumerate(parents)]
+    bits = [s[i, lengths[b] - rows[b]:].nonzero()[:, 0].tolist() for b, s in enumerate(seen) for i in range(rows[b])]
+    q = torch.randn(43, 8, dim, generator=rng).half().cuda()
+    lse = torch.empty(43, 8, device="cuda")
+    got = cache.tree_attention(batch, q, mask=ref.mask_words(bits, 2).cuda(), lse=lse)
+    cache.check()
+    check_attention(cache, table, "hnd", page, rows, lengths, seen, q, got, lse, dim ** -0.5)
+
+
 def test_large_batch(gpu):
     """More sequences than a CTA has threads, many without rows."""
     rng = rng_of(14)
