@@ -385,7 +385,7 @@ typedef struct pp_append_rows {
  * of src/qwen/model.rs:265-302, for a batch over pages): every k row, RMS-normed by head when
  * k_norm is given, rotated and rounded once to the cache's type, and every v row rounded, go to
  * their positions; q rows, normed and rotated likewise, to q_out (q_out may be q where the types
- * and strides agree). The angle position * inv_freq is formed in 64 bits, so far positions
+ * and strides agree, never k or v). The angle position * inv_freq is formed in 64 bits, so far positions
  * rotate as exactly as near ones. A draft tree gives each node its depth as position. Two rows
  * written to the same cache slot (one page in two sequences' tables) leave either there. */
 pp_status pp_paged_append(const pp_paged_cache* cache, const pp_paged_batch* batch,
@@ -433,7 +433,7 @@ pp_status pp_tree_attention(const pp_paged_cache* cache, const pp_paged_batch* b
  * accepted[b]. In every layer the path's K/V rows move to the front of the tree's, in order, so
  * the first new_len[b] positions are a contiguous cache. A sequence without rows gives accepted 0,
  * correction -1 and its kv_len. max_rows must bound n_b (a longer tree is left out, error bit 1;
- * <= 1024), path_stride >= max_rows; new_len must not be the batch's kv_len. */
+ * <= 1024), path_stride >= max_rows; outputs must not be inputs. */
 pp_status pp_tree_commit(const pp_paged_cache* cache, const pp_paged_batch* batch,
                          const int32_t* tokens, const int32_t* parents, const int32_t* picks,
                          int32_t* path, uint32_t path_stride, int32_t* accepted,
@@ -447,8 +447,8 @@ pp_status pp_tree_commit(const pp_paged_cache* cache, const pp_paged_batch* batc
  * chosen; a beam with finished[g][b] != 0 (NULL: none) has one candidate, token `pad` at its score
  * unchanged; a beam whose score or any of whose logits is NaN or +inf is left out and sets bit 2
  * of *err. Where fewer than k candidates remain the rest are -inf, -1, -1. Values are formed
- * and compared in 64 bits. work: 16-byte aligned, pp_beam_select_work_bytes. cuda_device: the
- * device of the pointers and the stream. */
+ * and compared in 64 bits. out_scores must not be scores. work: 16-byte aligned,
+ * pp_beam_select_work_bytes. cuda_device: the device of the pointers and the stream. */
 uint64_t pp_beam_select_work_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k);
 pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t row_stride,
                          const float* scores, const uint8_t* finished, int32_t pad,

@@ -429,6 +429,7 @@ extern "C" pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t 
   const BeamWork w(groups, beams, vocab, k);
   if ((uintptr_t)work % 16 || work_bytes < w.total)
     return paged_fail(PP_E_INVALID, "work must be 16-byte aligned and pp_beam_select_work_bytes long");
+  if (out_scores == scores) return paged_fail(PP_E_INVALID, "out_scores must not be scores");
   DeviceScope dev(cuda_device);
   if (!dev.ok) return paged_fail(PP_E_CUDA, "cannot use the device");
   BeamArgs a = {};

@@ -458,6 +458,7 @@ extern "C" pp_status pp_paged_append(const pp_paged_cache* cache, const pp_paged
     return paged_fail(PP_E_INVALID, "rows must be aligned to their element");
   if (r->q_out == r->q && r->q && (r->dtype != cache->dtype || (batch->rows > 1 && r->q_stride != nh * D)))
     return paged_fail(PP_E_INVALID, "q_out may be q only with equal types and adjacent rows");
+  if (r->q_out && (r->q_out == r->k || r->q_out == r->v)) return paged_fail(PP_E_INVALID, "q_out must not be k or v");
   if (batch->rows == 0) return PP_OK;
   DeviceScope dev(cache->cuda_device);
   const int sms = dev.ok ? sm_count(cache->cuda_device) : 0;
@@ -508,8 +509,10 @@ extern "C" pp_status pp_tree_commit(const pp_paged_cache* cache, const pp_paged_
     return paged_fail(PP_E_UNSUPPORTED, "trees of more than 1024 nodes");
   if (path_stride < batch->max_rows || path_stride == 0 || path_stride > (1u << 24))
     return paged_fail(PP_E_INVALID, "path_stride must be at least max_rows and 1");
-  if (new_len == batch->kv_len || accepted == batch->kv_len || correction == batch->kv_len)
-    return paged_fail(PP_E_INVALID, "outputs must not be the batch's kv_len");
+  const int32_t* const inputs[] = {tokens, parents, picks, batch->kv_len, batch->cu_rows, batch->page_table};
+  for (const int32_t* in : inputs)  // which every CTA of a sequence reads
+    if (in == path || in == accepted || in == correction || in == new_len)
+      return paged_fail(PP_E_INVALID, "outputs must not be inputs (tokens, parents, picks, kv_len, cu_rows, the table)");
   DeviceScope dev(cache->cuda_device);
   const int sms = dev.ok ? sm_count(cache->cuda_device) : 0;
   if (!sms) return paged_fail(PP_E_CUDA, "cannot use the cache's device");
@@ -544,8 +547,10 @@ extern "C" pp_status pp_beam_reorder(const pp_paged_cache* cache, const int32_t*
   if (groups == 0 || groups > 65535 || old_beams == 0 || old_beams > 65535 || new_beams == 0 ||
       new_beams > 65535 || table_stride == 0 || table_stride > 0x7fffffffu)
     return paged_fail(PP_E_INVALID, "groups, beams and the table's width must be positive, at most 65535 beams and groups");
-  if (new_table == table || new_len == len || new_len == beams || taken == beams || taken == len)
-    return paged_fail(PP_E_INVALID, "outputs must not be the inputs");
+  const int32_t* const inputs[] = {table, len, beams, spare};
+  for (const int32_t* in : inputs)
+    if (in == new_table || in == new_len || in == taken)
+      return paged_fail(PP_E_INVALID, "outputs must not be the inputs");
   DeviceScope dev(cache->cuda_device);
   const int sms = dev.ok ? sm_count(cache->cuda_device) : 0;
   if (!sms) return paged_fail(PP_E_CUDA, "cannot use the cache's device");

@@ -109,6 +109,26 @@ def test_work_and_commit_and_beam_refusals():
         refused(L.pp_beam_reorder(*{**order, **bad}.values()))
 
 
+def test_outputs_that_are_inputs_are_refused():
+    """Other CTAs of the call still read them."""
+    L = _lib.load()
+    c, b = ctypes.byref(cache()), ctypes.byref(batch())
+    ok = dict(c=c, b=b, tokens=FAKE + 1024, parents=FAKE + 2048, picks=FAKE + 4096, path=FAKE + 8192, stride=8,
+              accepted=FAKE + 8200, correction=FAKE + 8208, lengths=FAKE + 8216, err=None, stream=None)
+    for bad in (dict(path=FAKE + 1024), dict(accepted=FAKE + 2048), dict(correction=FAKE + 4096), dict(lengths=FAKE + 1024)):
+        refused(L.pp_tree_commit(*{**ok, **bad}.values()), "inputs")
+    refused(L.pp_beam_select(FAKE, _lib.PP_F32, 1000, FAKE, None, 0, 2, 4, 1000, 4, FAKE, FAKE + 64, FAKE + 128, FAKE,
+                             1 << 30, None, 0, None), "scores")
+    for out in ("k", "v"):
+        r = rows()
+        r.q_out = getattr(r, out)
+        refused(L.pp_paged_append(c, b, ctypes.byref(r), None, None), "q_out")
+    order = dict(c=c, t=FAKE, l=FAKE + 8, g=1, old=4, new=4, stride=8, beams=FAKE + 16, spare=FAKE + 48, nt=FAKE + 24,
+                 nl=FAKE + 32, taken=FAKE + 40, err=None, stream=None)
+    for bad in (dict(taken=FAKE + 48), dict(nl=FAKE + 48), dict(nt=FAKE + 8)):
+        refused(L.pp_beam_reorder(*{**order, **bad}.values()), "inputs")
+
+
 def test_work_bytes():
     L = _lib.load()
     small = L.pp_tree_attention_work_bytes(ctypes.byref(cache()), ctypes.byref(batch(batch=1, rows=1, max_len=10)), 4)
