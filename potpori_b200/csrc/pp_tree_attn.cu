@@ -14,7 +14,7 @@ namespace pp {
 
 // ---- 16-bit caches, few query vectors --------------------------------------------------------
 constexpr int kTreeThreads = 128;
-constexpr int kTreeBN = 64;
+constexpr int kTreeBN = kTreeTile<__half>;
 // Caches of up to so many tiles are never cut, which saves the join's launch, about 1 us (one decoded
 // row, 8 heads, narrow: 256 positions 8.0 us whole against 8.6, 512 11.9 against 9.4; F32: 64 positions
 // 6.8 against 7.4, 128 10.9 against 7.2; 240 vectors, tcgen05: 128 positions 10.9 against 11.9).
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
 // of a row stays in its warp; output: thread = dim, all rows. One row over 42 positions, 16 heads on 8:
 // 7.0 us, the chain of launch, lengths, page and rows; 48 rows over 515 to 1030: 83 us, 3.7 TB/s, the
 // multiply-adds and their shared-memory operands.
-constexpr int kTreeFBN = 32, kTreeFStages = 2;
+constexpr int kTreeFBN = kTreeTile<float>, kTreeFStages = 2;
 template <int DP, int BM>
 struct TreeFCfg {
   static constexpr int P = DP + 4;  // row pitch: 16-byte columns of consecutive rows in other banks

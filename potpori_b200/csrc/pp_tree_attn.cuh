@@ -19,6 +19,9 @@
 
 namespace pp {
 
+// Keys of a tile, of the attention's kernels and of the join.
+template <typename T>
+constexpr int kTreeTile = sizeof(T) == 4 ? 32 : 64;
 constexpr int kTreeMostRows = 1 << 20;  // of a sequence: times the group they stay below 2^31
 
 struct TreeArgs {
@@ -419,7 +422,7 @@ __device__ __forceinline__ JoinUnit join_unit(const TreeArgs& a, const Line& lin
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(128) pp_tree_join_kernel(const TreeArgs a) {
-  constexpr int V = DP / 16, BN = sizeof(T) == 4 ? 32 : 64;  // the attention's key tile
+  constexpr int V = DP / 16, BN = kTreeTile<T>;
   extern __shared__ uint32_t s_items[];  // [ctas + 1] items before each CTA's unit, then [batch + 1]
   __shared__ uint32_t scan[12];
   __shared__ float s_acc[8][DP];

@@ -43,7 +43,7 @@ using namespace pp;
 namespace pp {
 
 constexpr int kTcThreads = 224;  // 7 warps: 14 on an SM leave 128 registers a thread
-constexpr int kTcBM = 128, kTcBN = 64;
+constexpr int kTcBM = 128, kTcBN = kTreeTile<__half>;
 constexpr int kTcLag = 3;  // items a producer keeps in flight behind the one it issues
 
 template <int DP>
