@@ -410,8 +410,10 @@ typedef struct pp_tree_query {
  * whose bit j % 32 of mask word j / 32 of its row is set, whatever order the tree has; without a
  * mask the rows are a chain and row i sees nodes 0..i (a verify chunk; one row is plain decode).
  *   out = softmax over the seen positions of (q . k * scale) times v
- * Query heads h * n_heads / n_kv_heads .. share cached head h. Sums and the softmax are F32. A
- * row that sees nothing gives zeros. NaN and infinities in K or V of unseen positions have no
+ * Query heads h * n_heads / n_kv_heads .. share cached head h. Sums and the softmax are F32; into the
+ * products with v a weight goes, for 16-bit caches, as two parts of the cache's type (BF16: 2^-16 of
+ * itself is left out; F16: 2^-22 of itself and 2^-38 of the row's largest). A row that sees nothing
+ * gives zeros. NaN and infinities in K or V of unseen positions have no
  * effect. Nodes past 32 * mask_words are unseen. The result of a row does not depend on
  * atomics' order: equal calls give equal bits. `work` (16-byte aligned) holds the partial results
  * of split caches: at least pp_tree_attention_work_bytes (0: the arguments are refused). Limits:

@@ -234,14 +234,13 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
       for (int sh = 4; sh < 32; sh <<= 1)
 #pragma unroll
         for (int q = 0; q < 2; ++q) mx[q] = fmaxf(mx[q], __shfl_xor_sync(0xffffffffu, mx[q], sh));
-      // The old maximum serves until a score passes it by 2^8: P stays small enough, and the output
-      // need not be rescaled at every small step.
-      const bool grown = mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f || (m[0] == -INFINITY && mx[0] > m[0]) ||
-                         (m[1] == -INFINITY && mx[1] > m[1]);
+      // The old base serves until a score passes its maximum by more than the lag: P stays small enough,
+      // and the output need not be rescaled at every small step.
+      const bool grown = soft_outgrown<T>(mx[0], m[0]) || soft_outgrown<T>(mx[1], m[1]);
       if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const float mn = fmaxf(m[q], mx[q]);
+          const float mn = fmaxf(m[q], soft_base<T>(mx[q]));
           const float alpha = soft_exp<T>(m[q] - (mn == -INFINITY ? 0.f : mn));
           m[q] = mn;
           l[q] *= alpha;

@@ -17,9 +17,10 @@
 //    tile is issued while the softmax works on the tile before, when the product of the one before
 //    that is complete.
 //  * warps 0-3, softmax: thread = row = TMEM lane. S of the row into 64 registers; mask; running
-//    maximum; then, 32 columns at a time from TMEM again (no spills that way), exp2 and P. The output in TMEM is rescaled only when a row's maximum has
-//    grown by more than 2^8 (until then the old maximum serves: P <= 256 and the sums are F32), so
-//    after the first tiles hardly ever. At the end of a segment the rows leave from TMEM.
+//    maximum; then, 32 columns at a time from TMEM again (no spills that way), exp2 and P. The output in
+//    TMEM is rescaled only when a row's maximum has grown by more than 2^kSoftLag (until then the old base
+//    serves: P stays in range and the sums are F32), so after the first tiles hardly ever. At the end of a
+//    segment the rows leave from TMEM.
 // P is carried as two parts of the cache's type, hi + lo, and both multiply V: rounded to one part
 // it would add as much error as the rounding of the output.
 // What bounds it: a tile's way through the softmax. Of 2000 to 2200 clocks a tile and CTA (two CTAs on
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       const bool idle = s.rt * BM + warp * 32 >= NR;
       // Tiles of context alone, which most are, come first and need nothing but the softmax: one test.
       const int plain = idle || a.scale <= 0.f ? 0 : s.ctx / BN - s.t0;
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, high = -INFINITY, l = 0.f;  // base, maximum and sum of the row
       for (int t = 0; t < cnt; ++t, ++q, ++tiles) {
         if (!warp_wait(&bars->s_full[q & 1u], (q >> 1) & 1u)) {
           ok = false;
@@ -497,12 +498,13 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int k = 0; k < 64; ++k) top[k & 3] = fmaxf(top[k & 3], x[k >> 5][k & 31]);
-        const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;  // scale > 0
-        const bool grown = mx > m + 8.f || (m == -INFINITY && mx > m);
+        const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        // scale > 0; rounded up for F16, as no exponent below may pass what this one says
+        high = fmaxf(high, __is_same(T, __half) ? __fmul_ru(most, sc) : most * sc);
         float alpha = 1.f;
-        const bool rescale = __any_sync(0xffffffffu, grown);
-        if (rescale) {
-          const float mn = fmaxf(m, mx);
+        const bool rescale = __any_sync(0xffffffffu, soft_outgrown<T>(high, m));
+        if (rescale) {  // all of the warp's rows to their maxima, so that the next time is further off
+          const float mn = fmaxf(m, soft_base<T>(high));
           alpha = soft_exp<T>(m - (mn == -INFINITY ? 0.f : mn));
           m = mn;
           l *= alpha;

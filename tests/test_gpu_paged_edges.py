@@ -1,0 +1,137 @@
+"""The paged operators where their arithmetic or their rules are at the edge: small probabilities,
+sums whose parts cancel, infinities that a row sees, rows past the arrays, many rows, many sequences.
+
+Bounds of the attention's error are taken per output from sum_j p_j |v_j|, which is what a relative error
+of the weights or of the sums acts on, so a lost share of the softmax shows.
+"""
+import math
+
+import pytest
+import torch
+
+import paged_reference as ref
+from paged_reference import EPS, TINY
+from potpori_b200 import _lib
+from potpori_b200._lib import PPError
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+FAR = 1 << 20  # a host's bound on the lengths that sends more than 8 vectors a head to the tcgen05 kernel
+
+
+def rng_of(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def make(rng, lengths, rows, page, heads, dim, dtype, bound=None):
+    from potpori_b200.paged import PagedBatch, PagedCache
+
+    pages = sum(-(-n // page) for n in lengths) + 2
+    table = ref.make_table(rng, lengths, page, pages)
+    k = ref.make_pool(rng, pages, page, heads, dim, dtype)
+    v = ref.make_pool(rng, pages, page, heads, dim, dtype)
+    batch = PagedBatch(table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), ref.offsets(rows).cuda(),
+                       max_rows=max(rows), max_length=bound or max(lengths))
+    return PagedCache(k, v), batch, table
+
+
+def fill(pool, table, b, values):
+    """Positions 0.. of sequence b take values [n, heads, dim]."""
+    at = torch.arange(len(values), device="cuda")
+    page = pool.shape[1]
+    pool[table[b].cuda().long()[at // page], at % page] = values.to(pool.dtype).cuda()
+
+
+def exact(q, k, v, seen, scale):
+    """q [n, H, D], k and v [len, K, D], seen [n, len] or None (all), float64 on the device: out, lse, and
+    what errors act on: sum p |v|, sum |v| / sum of exp(s - max) [n, H, D], the largest sum |q k| scale."""
+    n, H, D = q.shape
+    G = H // k.shape[1]
+    out, lse = torch.zeros(n, H, D, dtype=torch.float64, device="cuda"), torch.zeros(n, H, dtype=torch.float64, device="cuda")
+    weight, floor, most = torch.zeros_like(out), torch.zeros_like(out), 0.0
+    for h in range(H):
+        kh, vh = k[:, h // G], v[:, h // G]
+        s = q[:, h] @ kh.T * scale
+        most = max(most, float((q[:, h].abs() @ kh.abs().T).max()) * abs(scale))
+        if seen is not None:
+            s = s.masked_fill(~seen, -math.inf)
+        top = s.max(-1, keepdim=True).values
+        p = torch.exp(s - top)
+        total = p.sum(-1, keepdim=True)
+        out[:, h], weight[:, h] = p @ vh / total, p @ vh.abs() / total
+        floor[:, h] = vh.abs().sum(0) / total
+        lse[:, h] = (top + torch.log(total))[:, 0]
+    return out, lse, weight, floor, most
+
+
+def bound_of(dtype, terms, dim, steps):
+    """What an output may be off by. A score is an F32 sum of dim products, scaled and taken from the maximum
+    (3 roundings of its magnitude), which moves a weight and its share; exponentials 2^-21; a weight's
+    second 16-bit part leaves out 2^-16 of a BF16 weight, 2^-22 of an F16 one, but an F16 part has steps
+    of 2^-24, half of which is 2^-38 where weights are taken at 2^13; `steps` additions one after the other
+    each cut or round at 2^-23. Then the output's rounding."""
+    out, _, weight, floor, most = terms
+    rel = 2 * (dim + 3) * 2.0 ** -24 * most + 2.0 ** -20 + steps * 2.0 ** -23 + {F32: 0, BF16: 2.0 ** -16, F16: 2.0 ** -22}[dtype]
+    return out.abs() * EPS[dtype] + TINY[dtype] + rel * weight + (2.0 ** -38 * floor if dtype == F16 else 0)
+
+
+# (type, heads a cached head, host's bound): the F32, the narrow and the tcgen05 kernel. 12 vectors a head and
+# FAR take the tcgen05 kernel, 1 vector the narrow one.
+KERNELS = [(F32, 1, None), (BF16, 1, None), (F16, 1, None), (BF16, 12, FAR), (F16, 12, FAR)]
+
+
+@pytest.mark.parametrize("dt,G,bound", KERNELS)
+@pytest.mark.parametrize("sink_v", [0.0, 3.0])
+@pytest.mark.parametrize("length", [200, 131072])
+@pytest.mark.parametrize("spread", [0.0, 0.5])
+def test_small_probabilities_count(gpu, dt, G, bound, sink_v, length, spread):
+    """One key 17.5 nats above all the others, whose weights are 2^-25 of its own: they are what the
+    output consists of where that key's V is zero."""
+    rng = rng_of(50)
+    cache, batch, table = make(rng, [length], [1], 64, 1, 64, dt, bound=bound)
+    k = torch.zeros(length, 1, 64)
+    k[:, 0, 0] = spread * torch.randn(length, generator=rng)
+    k[5, 0, 0] = 17.5
+    v = 256 + 32 * torch.randn(length, 1, 64, generator=rng)
+    v[5] = sink_v
+    fill(cache.k, table, 0, k)
+    fill(cache.v, table, 0, v)
+    q = torch.zeros(1, G, 64, dtype=dt, device="cuda")
+    q[:, :, 0] = 1.0
+    lse = torch.empty(1, G, device="cuda")
+    got = cache.tree_attention(batch, q, scale=1.0, lse=lse)
+    cache.check()
+    terms = exact(q.double(), k.to(dt).double().cuda(), v.to(dt).double().cuda(), None, 1.0)
+    # At 131072 the tiles of 64 (32) keys are cut over at least 148 CTAs: at most 14 (28) of them in a CTA, 8 additions
+    # each (32 in the F32 kernel), and at most 740 partials; at 200 there are 4 (7).
+    steps = (28 * 32 + 740) if length > 200 else 7 * 32
+    off = (got.double() - terms[0]).abs()
+    tol = bound_of(dt, terms, 1, steps)  # one product a score, the rest are zeros
+    assert (off <= tol).all(), (float((off / tol).max()), float((off / terms[0].abs()).max()))
+    assert ((lse.double() - terms[1]).abs() <= (steps + 64) * 2.0 ** -24 + 2.0 ** -20 + terms[1].abs() * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("dt,G,bound", KERNELS)
+@pytest.mark.parametrize("scale", [1.0, -1.0, 2.0 ** -4, 2.0 ** -10])
+@pytest.mark.parametrize("step", [0.0, 1.0])
+def test_scores_of_many_digits(gpu, dt, G, bound, scale, step):
+    """Scores near 2^26, where F32 values are 4 or 8 apart, equal or rising with the position: outputs are means of
+    V with weights of some kind, never infinite. Equal scores give the plain mean."""
+    rng = rng_of(58)
+    n = 300
+    cache, batch, table = make(rng, [n], [1], 16, 1, 64, dt, bound=bound)
+    k = torch.zeros(n, 1, 64)
+    k[:, 0, 0], k[:, 0, 1] = 30720.0, step * torch.arange(n)
+    v = 1 + torch.rand(n, 1, 64, generator=rng)
+    fill(cache.k, table, 0, k)
+    fill(cache.v, table, 0, v)
+    q = torch.zeros(1, G, 64, dtype=dt, device="cuda")
+    q[:, :, 0], q[:, :, 1] = 2048.0, 16.0
+    lse = torch.empty(1, G, device="cuda")
+    got = cache.tree_attention(batch, q, scale=scale, lse=lse).double()
+    v = v.to(dt).double().cuda()
+    slack = 2 * EPS[dt] + 2.0 ** -14
+    assert (got >= v.min() * (1 - slack)).all() and (got <= v.max() * (1 + slack)).all() and torch.isfinite(lse).all()
+    if step == 0:
+        assert ((got[0] - v.mean(0)).abs() <= v.mean(0) * slack).all()
