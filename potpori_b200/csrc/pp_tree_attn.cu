@@ -320,9 +320,14 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
     const bool whole = s.t0 == 0 && s.t1 == s.tiles;
     const int64_t slot = 2 * (int64_t)blockIdx.x + (w == begin ? 0 : 1);
     const int live = min(BM, s.n * a.G - s.rt * BM);
-    if (dirty) {
+    if (dirty) {  // into the output of the warp with the row's largest base, whose weight below is 1
       add_nonfinite<T>(a, s, live, max(s.ctx, s.t0 * BN), min(s.len, s.t1 * BN), tid, kTreeThreads,
-                       [&](int r, int d) -> float& { return os[r * C::kOPitch + d]; });
+                       [&](int r, int d) -> float& {
+                         int k = 0;
+                         for (int j = 1; j < 4; ++j)
+                           if (ml[j * BM + r].x > ml[k * BM + r].x) k = j;
+                         return os[(k * BM + r) * C::kOPitch + d];
+                       });
       __syncthreads();
     }
 #pragma unroll 1

@@ -383,8 +383,8 @@ __device__ __forceinline__ float soft_lse(float m, float l) {
 }
 
 // Adds the non-finite values of a tree's V rows [j0, j1) (positions) to the outputs that see them: the
-// kernels' products saw zeros in their place. o(r, d) is the output of vector r of the tile, dim d; a
-// weight is positive, so the sum is what the value is. By NT threads over (vector, dim); kept small,
+// kernels' products saw zeros in their place. o(r, d) is the output of vector r of the tile, dim d; its
+// weight there must be positive, so that the sum is what the value is. By NT threads over (vector, dim); kept small,
 // it hardly ever runs.
 template <typename T, typename O>
 __device__ __forceinline__ void add_nonfinite(const TreeArgs& a, const Segment& s, int rows, int j0, int j1, int tid, int nt, O o) {

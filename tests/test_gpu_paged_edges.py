@@ -135,3 +135,31 @@ def test_scores_of_many_digits(gpu, dt, G, bound, scale, step):
     assert (got >= v.min() * (1 - slack)).all() and (got <= v.max() * (1 + slack)).all() and torch.isfinite(lse).all()
     if step == 0:
         assert ((got[0] - v.mean(0)).abs() <= v.mean(0) * slack).all()
+
+
+@pytest.mark.parametrize("dt,heads,bound", [(F32, 2, None), (BF16, 2, None), (F16, 2, None), (BF16, 16, FAR), (F16, 16, FAR)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("ctx", [0, 3000])
+def test_seen_nonfinite_nodes(gpu, dt, heads, bound, bad, ctx):
+    """A node's V that is not finite gives its own value to every row that sees the node, whichever
+    keys the row sees beside it, and nothing to the others."""
+    rng = rng_of(53)
+    n = 40
+    cache, batch, table = make(rng, [ctx + n], [n], 16, 2, 128, dt, bound=bound)
+    q = torch.randn(n, heads, 128, generator=rng).to(dt).cuda()
+    # Row i sees node i alone, the multiples of five node 21 too, and all of the context.
+    bits = [[i] + ([21] if i % 5 == 0 else []) for i in range(n)]
+    mask = ref.mask_words(bits, 2).cuda()
+    want = cache.tree_attention(batch, q, mask=mask)
+    p, at = int(table[0, (ctx + 21) // 16]), (ctx + 21) % 16
+    cache.v[p, at, 0, 3:90:5] = bad
+    got = cache.tree_attention(batch, q, mask=mask)
+    sees = torch.tensor([21 in x for x in bits]).cuda()
+    hit = torch.zeros(128, dtype=torch.bool, device="cuda")
+    hit[3:90:5] = True
+    first = heads // 2
+    assert torch.equal(got[~sees], want[~sees]) and torch.equal(got[:, first:], want[:, first:])
+    mine = got[sees][:, :first]
+    assert torch.equal(mine[..., ~hit], want[sees][:, :first][..., ~hit])
+    mine = mine[..., hit]
+    assert torch.isnan(mine).all() if math.isnan(bad) else (mine == bad).all()
