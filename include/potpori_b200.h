@@ -415,7 +415,7 @@ typedef struct pp_tree_query {
  * itself is left out; F16: 2^-22 of itself and 2^-38 of the row's largest). A row that sees nothing
  * gives zeros. NaN and infinities in K or V of unseen positions have no effect. A node's value
  * of V that is not finite is the output of the rows that see it (or NaN where its weight is zero in
- * F32). Nodes past 32 * mask_words are unseen. The result of a row does not depend on
+ * F32); the context's gives every row itself or NaN. Nodes past 32 * mask_words are unseen. The result of a row does not depend on
  * atomics' order: equal calls give equal bits. `work` (16-byte aligned) holds the partial results
  * of split caches: at least pp_tree_attention_work_bytes (0: the arguments are refused). Limits:
  * n_heads <= 1024 n_kv_heads; max_rows <= 2^20; table_stride * page_size < 2^31; and

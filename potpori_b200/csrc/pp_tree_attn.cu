@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
     const int64_t slot = 2 * (int64_t)blockIdx.x + (w == begin ? 0 : 1);
     const int live = min(BM, s.n * a.G - s.rt * BM);
     if (dirty) {  // into the output of the warp with the row's largest base, whose weight below is 1
-      add_nonfinite<T>(a, s, live, max(s.ctx, s.t0 * BN), min(s.len, s.t1 * BN), tid, kTreeThreads,
+      add_nonfinite<T>(a, s, live, max(s.ctx & ~15, s.t0 * BN), min(s.len, s.t1 * BN), tid, kTreeThreads,
                        [&](int r, int d) -> float& {
                          int k = 0;
                          for (int j = 1; j < 4; ++j)

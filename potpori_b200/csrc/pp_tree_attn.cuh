@@ -382,10 +382,10 @@ __device__ __forceinline__ float soft_lse(float m, float l) {
   return (sizeof(T) == 4 ? m : m * 0.69314718055994531f) + logf(l);
 }
 
-// Adds the non-finite values of a tree's V rows [j0, j1) (positions) to the outputs that see them: the
-// kernels' products saw zeros in their place. o(r, d) is the output of vector r of the tile, dim d; its
-// weight there must be positive, so that the sum is what the value is. By NT threads over (vector, dim); kept small,
-// it hardly ever runs.
+// Adds the non-finite values of V at the positions [j0, j1), the tree's and those of the context that
+// share its first tile, to the outputs that see them: the kernels' products saw zeros in their place.
+// o(r, d) is the output of vector r of the tile, dim d; its weight there must be positive, so that the
+// sum is what the value is. By NT threads over (vector, dim); kept small, it hardly ever runs.
 template <typename T, typename O>
 __device__ __forceinline__ void add_nonfinite(const TreeArgs& a, const Segment& s, int rows, int j0, int j1, int tid, int nt, O o) {
   const int D = a.c.head_dim;
@@ -401,7 +401,7 @@ __device__ __forceinline__ void add_nonfinite(const TreeArgs& a, const Segment& 
       const float f = Elem<T>::get(v[d]);
       if (isfinite(f)) continue;
       const int i = (int)a.by_g.div((uint32_t)(s.rt * a.bm + r));
-      if (sees_node(a, s.row0 + i, i, j - s.ctx)) o(r, d) += f;
+      if (j < s.ctx || sees_node(a, s.row0 + i, i, j - s.ctx)) o(r, d) += f;
     }
   }
 }

@@ -581,10 +581,10 @@ __global__ void __launch_bounds__(kTcThreads, TcCfg<DP>::kPerSm) pp_tree_tc_kern
       const float inv = 1.f / l;
       if (dirty) {  // column after column in TMEM: a value is the same for every lane of the warp
 #pragma unroll 1
-        for (int j = max(s.ctx, s.t0 * BN); j < min(s.len, s.t1 * BN); ++j) {
+        for (int j = max(s.ctx & ~(BN - 1), s.t0 * BN); j < min(s.len, s.t1 * BN); ++j) {
           const int64_t off = paged_offset(a.c, a.b.table + (int64_t)s.b * a.b.table_stride, a.b.table_stride, j);
           if (off < 0) continue;
-          const bool see = live && sees_node(a, row, i, j - s.ctx);
+          const bool see = live && (j < s.ctx || sees_node(a, row, i, j - s.ctx));
           const T* src = (const T*)(a.c.v + off + (int64_t)s.h * a.c.head_bytes);
 #pragma unroll 1
           for (int d = 0; d < D; ++d) {

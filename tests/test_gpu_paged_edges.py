@@ -163,3 +163,27 @@ def test_seen_nonfinite_nodes(gpu, dt, heads, bound, bad, ctx):
     assert torch.equal(mine[..., ~hit], want[sees][:, :first][..., ~hit])
     mine = mine[..., hit]
     assert torch.isnan(mine).all() if math.isnan(bad) else (mine == bad).all()
+
+
+@pytest.mark.parametrize("dt,heads,bound", [(F32, 2, None), (BF16, 2, None), (F16, 2, None), (BF16, 16, FAR), (F16, 16, FAR)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("index", [0, 70, 3071, 3099])
+@pytest.mark.parametrize("masked", [False, True])
+def test_nonfinite_context(gpu, dt, heads, bound, bad, index, masked):
+    """A V of the context that is not finite reaches every row, wherever its position lies: before the
+    tree's first tile or in it, next to the first node."""
+    rng = rng_of(59)
+    n, ctx = 12, 3100
+    cache, batch, table = make(rng, [ctx + n], [n], 16, 2, 128, dt, bound=bound)
+    q = torch.randn(n, heads, 128, generator=rng).to(dt).cuda()
+    mask = ref.mask_words([[i] for i in range(n)], 1).cuda() if masked else None
+    want = cache.tree_attention(batch, q, mask=mask)
+    p, at = int(table[0, index // 16]), index % 16
+    cache.v[p, at, 0, 3:90:5] = bad
+    got = cache.tree_attention(batch, q, mask=mask)
+    hit = torch.zeros(128, dtype=torch.bool, device="cuda")
+    hit[3:90:5] = True
+    first = heads // 2
+    assert torch.equal(got[:, first:], want[:, first:]) and torch.equal(got[:, :first][..., ~hit], want[:, :first][..., ~hit])
+    mine = got[:, :first][..., hit]
+    assert (torch.isnan(mine) if math.isnan(bad) else torch.isnan(mine) | (mine == bad)).all()
