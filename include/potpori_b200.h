@@ -327,9 +327,10 @@ pp_status pp_shard_read_taps(pp_shard* shard, uint32_t m, float* f32, uint16_t* 
  * PP_E_UNSUPPORTED; message in pp_last_error(NULL)). What only the device sees is checked there:
  * *err (device memory, zero before the call, or NULL) gets bit value 1 when a length or a page table
  * entry points outside the table or the cache, or cu_rows outside the row arrays. Such a position is
- * neither read nor written, and a sequence whose kv_len is below its number of rows or above
- * table_stride * page_size is left out whole (its output rows keep what they held); value 4 when a
- * bounded wait on the device expired (the output is then undefined). No call reads a position at or
+ * neither read nor written, and a sequence whose rows lie outside the arrays, or whose kv_len is below
+ * its number of rows or above table_stride * page_size, is left out whole (its output rows, q_out's
+ * among them, keep what they held); value 4 when a bounded wait on the device expired (the output is
+ * then undefined). No call reads a position at or
  * past kv_len, whatever the page holds there. */
 
 /* A cache: `layers` layers of n_pages pages of page_size positions. Element (layer, page, row,

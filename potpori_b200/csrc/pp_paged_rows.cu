@@ -51,9 +51,11 @@ __device__ __forceinline__ void turn(float& a, float& b, float2 r) {
 }
 
 // Where row t goes: its sequence, cache index and page, by a warp. `report`: this warp marks a bad one.
+// Rows of nobody, and of a sequence whose rows do not fit the arrays or whose length does not fit its
+// table, are left out whole, q too.
 struct RowPlace {
   int64_t offset;  // -1: no valid page
-  int32_t in_batch, pos;
+  int32_t live, pos;
 };
 __device__ __forceinline__ RowPlace place_row(const AppendArgs& a, int t, int lane, bool report) {
   const int given = a.positions ? a.positions[t] : 0;
@@ -61,12 +63,13 @@ __device__ __forceinline__ RowPlace place_row(const AppendArgs& a, int t, int la
   RowPlace r = {-1, 0, 0};
   if (b >= 0) {
     const int first = a.b.cu_rows[b], n = a.b.cu_rows[b + 1] - first, len = a.b.kv_len[b];
-    const int index = len - n + (t - first);
-    r.in_batch = 1;
-    r.pos = a.positions ? given : index;
     const int64_t room = (int64_t)a.b.table_stride * a.c.page.d;
-    if (len >= n && len <= room)
+    if (first >= 0 && n > t - first && n <= a.b.rows - first && len >= n && len <= room) {
+      const int index = len - n + (t - first);
+      r.live = 1;
+      r.pos = a.positions ? given : index;
       r.offset = paged_offset(a.c, a.b.table + (int64_t)b * a.b.table_stride, a.b.table_stride, index);
+    }
     if (r.offset < 0 && report && lane == 0 && a.err) atomicOr(a.err, PAGED_BAD_PAGE);
   }
   return r;
@@ -112,7 +115,7 @@ __global__ void __launch_bounds__(kAppendThreads, 8) pp_append_kernel(const Appe
   }
   __syncthreads();
   const RowPlace place = s_place;
-  if (!place.in_batch) return;
+  if (!place.live) return;
   for (int i = threadIdx.x; i < a.rot / 2; i += blockDim.x) cs[i] = rotation(place.pos, a.inv_freq[i]);
   __syncthreads();
   float2 r[4];
@@ -177,7 +180,7 @@ __global__ void __launch_bounds__(kAppendAnyThreads) pp_append_any_kernel(const 
     if (lane == 0) place = p;
   }
   __syncthreads();
-  if (!place.in_batch) return;
+  if (!place.live) return;
   if (a.inv_freq && tid < a.rot / 2) cs[tid] = rotation(place.pos, a.inv_freq[tid]);
   __syncthreads();
   for (int slot = blockIdx.y * 8 + warp; slot < heads; slot += 8 * gridDim.y) {

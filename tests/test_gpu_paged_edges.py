@@ -187,3 +187,39 @@ def test_nonfinite_context(gpu, dt, heads, bound, bad, index, masked):
     assert torch.equal(got[:, first:], want[:, first:]) and torch.equal(got[:, :first][..., ~hit], want[:, :first][..., ~hit])
     mine = got[:, :first][..., hit]
     assert (torch.isnan(mine) if math.isnan(bad) else torch.isnan(mine) | (mine == bad)).all()
+
+
+@pytest.mark.parametrize("vector", [True, False])
+def test_append_rows_past_the_arrays(gpu, vector):
+    """cu_rows that reaches past the row arrays, or before them, and lengths that do not fit: append leaves
+    the sequence out whole, its rows of q_out too, and marks it; the others are written."""
+    from potpori_b200.paged import PagedBatch
+
+    rng = rng_of(54)
+    cache, batch, table = make(rng, [40, 40, 40], [2, 2, 2], 16, 2, 64, BF16)
+    wide = torch.randn(6, 4 + 2, 64 + (0 if vector else 1), generator=rng).bfloat16().cuda()
+    rows = [wide.flatten(1)[:, a:a + h * 64].unflatten(1, (h, 64)) for a, h in ((0, 2), (128, 2), (256, 2))]
+    q, k, v = rows
+    freq = (1e4 ** (-torch.arange(0, 64, 2, dtype=torch.float64) / 64)).cuda()
+    before = cache.k.clone(), cache.v.clone()
+    whole = cache.append(batch, k, v, q=q, inv_freq=freq)
+    cache.check()
+    after = cache.k.clone(), cache.v.clone()
+    cases = [([0, 2, 4, 8], [40, 40, 40], 2), ([0, 2, 4, 2 ** 31 - 1], [40, 40, 40], 2), ([-2, 2, 4, 6], [40, 40, 40], 0),
+             ([0, 2, 4, 6], [40, 1, 40], 1), ([0, 2, 4, 6], [40, 49, 40], 1), ([0, 2, 4, 6], [40, -3, 40], 1)]
+    for cu, lengths, left in cases:
+        cache.k.copy_(before[0])
+        cache.v.copy_(before[1])
+        b = PagedBatch(batch.page_table, torch.tensor(lengths, dtype=torch.int32).cuda(),
+                       torch.tensor(cu, dtype=torch.int32).cuda(), 8, 40)
+        out = torch.full((6, 2, 64), 7.0, dtype=BF16, device="cuda")
+        cache.append(b, k, v, q=q, inv_freq=freq, out=out)
+        with pytest.raises(PPError):
+            cache.check()
+        for pool, old, new in ((cache.k, before[0], after[0]), (cache.v, before[1], after[1])):
+            for s in range(3):
+                pages = table[s].long().cuda()
+                assert torch.equal(pool[pages], (old if s == left else new)[pages]), (cu, lengths, s)
+        for s in range(3):
+            rows_of = slice(2 * s, 2 * s + 2)
+            assert (out[rows_of] == 7.0).all() if s == left else torch.equal(out[rows_of], whole[rows_of]), (cu, lengths, s)
