@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import PP_E_INVALID, PP_E_TIMEOUT, PPError
+from ._lib import PP_E_INVALID, PP_E_NONFINITE, PP_E_TIMEOUT, PPError
 
 _lib.load()  # the library that the binding calls; raises where it was never built
 from . import _paged  # noqa: E402
@@ -63,11 +63,15 @@ class PagedCache(_paged.Cache):
         self.kv_heads, self.head_dim = k.shape[head], k.shape[-1]
 
     def check(self) -> None:
-        """Raises when a call on this cache met a length or a page outside the table or the
-        cache, or a device wait that ran out (synchronises), and clears the mark."""
+        """Raises when a call on this cache met rows outside the row tensors, a length or a page
+        outside the table or the cache, or a device wait that ran out, or a ``beam_select`` that
+        was given ``err`` left a beam out (synchronises), and clears the marks. The first of
+        timeout, bad descriptor and beam gives the status; the message names all."""
         bits = int(self.err.item())
         if bits:
             self.err.zero_()
-            if bits & 4:
-                raise PPError(PP_E_TIMEOUT, "a wait on the device expired: outputs are undefined")
-            raise PPError(PP_E_INVALID, "a length or page table entry outside the table or the cache")
+            found = [(status, text) for bit, status, text in (
+                (4, PP_E_TIMEOUT, "a wait on the device expired: outputs are undefined"),
+                (1, PP_E_INVALID, "rows, a length or a page table entry outside the arrays, the table or the cache"),
+                (2, PP_E_NONFINITE, "a beam was left out for a NaN or +inf")) if bits & bit]
+            raise PPError(found[0][0], "; ".join(text for _, text in found))

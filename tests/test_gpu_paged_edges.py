@@ -223,3 +223,26 @@ def test_append_rows_past_the_arrays(gpu, vector):
         for s in range(3):
             rows_of = slice(2 * s, 2 * s + 2)
             assert (out[rows_of] == 7.0).all() if s == left else torch.equal(out[rows_of], whole[rows_of]), (cu, lengths, s)
+
+
+def test_check_tells_beams_from_pages(gpu):
+    """The error word that beam_select shares with a cache: a beam left out is not reported as a bad page."""
+    from potpori_b200.paged import PagedBatch, beam_select
+
+    rng = rng_of(55)
+    cache, batch, table = make(rng, [20], [2], 16, 2, 64, BF16)
+    logits = torch.zeros(1, 2, 100, device="cuda")
+    logits[0, 1, 7] = math.nan
+    scores = torch.zeros(1, 2, device="cuda")
+    beam_select(logits, scores, 2, err=cache.err)
+    with pytest.raises(PPError) as e:
+        cache.check()
+    assert e.value.status == _lib.PP_E_NONFINITE and "beam" in str(e.value) and "page" not in str(e.value)
+    cache.check()
+    k = torch.zeros(2, 2, 64, dtype=BF16, device="cuda")
+    cache.append(PagedBatch(torch.full_like(batch.page_table, -1), batch.lengths, batch.cu_rows, 2, 20), k, k)
+    beam_select(logits, scores, 2, err=cache.err)
+    with pytest.raises(PPError) as e:
+        cache.check()
+    assert e.value.status == _lib.PP_E_INVALID and "beam" in str(e.value) and "page" in str(e.value)
+    cache.check()
