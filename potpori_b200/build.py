@@ -1,5 +1,6 @@
 """Compile the sm_100a CUDA library in-tree (potpori_b200/libpotpori_b200.so) and its torch binding
-(potpori_b200/_paged.so).
+(potpori_b200/_paged.so). The binding alone needs torch and a host compiler: where torch is not installed,
+the library is built and the binding left out.
 
 nvcc cross-compiles for sm_100a without a GPU. The CUDA runtime is linked statically so the
 library does not depend on which libcudart another package (torch) has loaded; the driver
@@ -8,9 +9,13 @@ API entry point it needs (tensor-map encoding) is fetched at run time.
 from __future__ import annotations
 
 import glob
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
+import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
@@ -24,6 +29,7 @@ HEADER = os.path.join(ROOT, "include", "potpori_b200.h")
 DEPS = SOURCES + glob.glob(os.path.join(HERE, "csrc", "*.cuh")) + [HEADER]
 BINDING = os.path.join(HERE, "_paged.so")
 BINDING_SOURCE = os.path.join(HERE, "csrc", "pp_torch.cpp")
+BINDING_BUILT_FOR = os.path.join(HERE, "_paged.built")  # the torch and Python that _paged.so was built for
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -47,10 +53,23 @@ def stale(target: str = LIB, deps: list = DEPS) -> bool:
     return any(os.path.getmtime(p) > t for p in deps)
 
 
-def build_binding() -> None:
-    """potpori_b200/_paged.so: the paged operators' torch binding, linked to the library beside it."""
-    import sysconfig
+def binding_abi() -> "str | None":
+    """The torch and Python that a binding is built for; None without torch."""
+    if importlib.util.find_spec("torch") is None:
+        return None
+    return f"torch {importlib.metadata.version('torch')} {sysconfig.get_config_var('SOABI')}"
 
+
+def binding_stale(abi: str) -> bool:
+    """Older than its sources, or built for another torch or Python, whose C++ ABI may differ."""
+    if stale(BINDING, [BINDING_SOURCE, HEADER]) or not os.path.exists(BINDING_BUILT_FOR):
+        return True
+    with open(BINDING_BUILT_FOR) as f:
+        return f.read() != abi
+
+
+def build_binding(abi: str) -> None:
+    """potpori_b200/_paged.so: the paged operators' torch binding, linked to the library beside it."""
     from torch.utils import cpp_extension
 
     cxx = next((c for c in ("/usr/bin/g++", shutil.which("g++")) if c and os.path.exists(c)), "c++")
@@ -62,13 +81,18 @@ def build_binding() -> None:
          "-ltorch_python", f"-L{HERE}", "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
          f"-Wl,-rpath,{torch_lib}"], check=True)
     os.replace(BINDING + ".tmp", BINDING)
+    with open(BINDING_BUILT_FOR, "w") as f:
+        f.write(abi)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if force or stale():
         build_library(verbose)
-    if force or stale(BINDING, [BINDING_SOURCE, HEADER]):
-        build_binding()
+    abi = binding_abi()
+    if abi is None:
+        print("torch is not installed: potpori_b200.paged is left out", file=sys.stderr)
+    elif force or binding_stale(abi):
+        build_binding(abi)
     return LIB
 
 
@@ -87,6 +111,5 @@ def build_library(verbose: bool = False) -> None:
 
 
 if __name__ == "__main__":
-    import sys
     build(force=True, verbose="-v" in sys.argv)
     print(LIB)

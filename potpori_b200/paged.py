@@ -19,8 +19,12 @@ from . import _lib
 from ._lib import PP_E_INVALID, PP_E_NONFINITE, PP_E_TIMEOUT, PPError
 
 _lib.load()  # the library that the binding calls; raises where it was never built
-from . import _paged  # noqa: E402
-from ._paged import beam_select  # noqa: E402,F401
+try:
+    from . import _paged  # noqa: E402
+    from ._paged import beam_select  # noqa: E402,F401
+except ImportError as e:
+    raise ImportError("potpori_b200/_paged.so is absent or was built for another torch or Python: run "
+                      f"`python -m potpori_b200.build` where torch is installed ({e})") from e
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
