@@ -373,18 +373,19 @@ __global__ void __launch_bounds__(32 * kMergeWarps) pp_beam_merge_kernel(const B
 }
 
 constexpr uint32_t kSliceLarge = 128 * 32, kSliceSmall = 256 * 8;
+// Slices of 4096 logits, 32 of each of 128 threads; where those are not four an SM, of 2048, 8 of each
+// of 256, so that more warps share the work (256 rows of 151936: 38.3 us, of 8192 logits by 256 threads
+// 43, of 2048 78; 4 rows: 9.0 us in 2048s, 11.9 in 4096s).
+inline bool beam_wide(uint32_t groups, uint32_t beams, uint32_t vocab, int sms) {
+  return (uint64_t)groups * beams * ((vocab + kSliceLarge - 1) / kSliceLarge) >= 4ull * sms;
+}
 struct BeamWork {
   uint64_t sums, keys, total;
   uint32_t slices;
-  bool wide;
-  BeamWork(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k) {
+  BeamWork(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k, bool wide) {
     const uint64_t rows = (uint64_t)groups * beams;
-    // Slices of 4096 logits, 32 of each of 128 threads; where those are not four an SM, of 2048, 8 of
-    // each of 256, so that more warps share the work (256 rows of 151936: 38.3 us, of 8192 logits by 256
-    // threads 43, of 2048 78; 4 rows: 9.0 us in 2048s, 11.9 in 4096s).
-    const uint64_t large = (vocab + kSliceLarge - 1) / kSliceLarge;
-    wide = rows * large >= 4 * 148;
-    slices = (uint32_t)(wide ? large : (vocab + kSliceSmall - 1) / kSliceSmall);
+    const uint32_t size = wide ? kSliceLarge : kSliceSmall;
+    slices = (uint32_t)(((uint64_t)vocab + size - 1) / size);
     sums = 0;
     keys = rows * slices * sizeof(SliceSum);
     total = keys + rows * slices * k * 8;
@@ -406,7 +407,7 @@ void launch_rows(const BeamArgs& a, bool wide, dim3 grid, cudaStream_t st) {
 }  // namespace pp
 
 extern "C" uint64_t pp_beam_select_work_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k) {
-  return BeamWork(groups, beams, vocab, k).total;
+  return BeamWork(groups, beams, vocab, k, false).total;  // the smaller slices need more, whatever the device
 }
 
 extern "C" pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t row_stride,
@@ -426,12 +427,14 @@ extern "C" pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t 
   if (row_stride < (int64_t)vocab && (uint64_t)groups * beams > 1)
     return paged_fail(PP_E_INVALID, "row_stride shorter than the vocabulary");
   if ((uintptr_t)logits % dtype_bytes(dtype)) return paged_fail(PP_E_INVALID, "misaligned logits");
-  const BeamWork w(groups, beams, vocab, k);
-  if ((uintptr_t)work % 16 || work_bytes < w.total)
+  if ((uintptr_t)work % 16 || work_bytes < pp_beam_select_work_bytes(groups, beams, vocab, k))
     return paged_fail(PP_E_INVALID, "work must be 16-byte aligned and pp_beam_select_work_bytes long");
   if (out_scores == scores) return paged_fail(PP_E_INVALID, "out_scores must not be scores");
   DeviceScope dev(cuda_device);
-  if (!dev.ok) return paged_fail(PP_E_CUDA, "cannot use the device");
+  const int sms = dev.ok ? sm_count(cuda_device) : 0;
+  if (!sms) return paged_fail(PP_E_CUDA, "cannot use the device");
+  const bool wide = beam_wide(groups, beams, vocab, sms);
+  const BeamWork w(groups, beams, vocab, k, wide);
   BeamArgs a = {};
   a.logits = logits;
   a.row_stride = row_stride;
@@ -450,9 +453,9 @@ extern "C" pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t 
   a.err = err;
   const cudaStream_t st = (cudaStream_t)stream;
   const dim3 grid(a.slices, groups * beams);
-  if (dtype == PP_F32) launch_rows<float>(a, w.wide, grid, st);
-  else if (dtype == PP_BF16) launch_rows<__nv_bfloat16>(a, w.wide, grid, st);
-  else launch_rows<__half>(a, w.wide, grid, st);
+  if (dtype == PP_F32) launch_rows<float>(a, wide, grid, st);
+  else if (dtype == PP_BF16) launch_rows<__nv_bfloat16>(a, wide, grid, st);
+  else launch_rows<__half>(a, wide, grid, st);
   const pp_status r = launch_status("pp_beam_select");
   if (r != PP_OK) return r;
   const size_t base = (size_t)beams * k * 8 + (size_t)beams * 8, copy = (size_t)a.slices * k * 8;

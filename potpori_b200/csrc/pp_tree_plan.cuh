@@ -16,9 +16,9 @@ pp_status launch_tree(const TreeArgs& a, int threads, size_t smem, cudaStream_t 
 // The join starts while the last CTAs of the attention still run and waits for them on the device.
 template <typename T, int DP>
 pp_status launch_join(const TreeArgs& a, cudaStream_t st) {
-  const int items = a.ctas * a.bm;
+  const int items = a.ctas * a.bm, most = 8 * sm_count(a.dev);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(items < 148 * 8 ? items : 148 * 8);
+  cfg.gridDim = dim3(items < most ? items : most);
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 4 * (size_t)(a.ctas + 1 + a.b.batch + 1);
   cfg.stream = st;
