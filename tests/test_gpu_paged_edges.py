@@ -137,6 +137,52 @@ def test_scores_of_many_digits(gpu, dt, G, bound, scale, step):
         assert ((got[0] - v.mean(0)).abs() <= v.mean(0) * slack).all()
 
 
+@pytest.mark.parametrize("dt,G,bound", KERNELS)
+def test_weights_whose_values_cancel(gpu, dt, G, bound):
+    """V alternates between +1000 and -1000 and neighbours have nearly equal scores, so that the output is
+    a small difference of the weights: those must be good to far more than the output's type."""
+    rng = rng_of(51)
+    n = 70
+    cache, batch, table = make(rng, [n], [1], 16, 1, 64, dt, bound=bound)
+    q = torch.randn(1, G, 64, generator=rng).to(dt)
+    k = torch.randn(n // 2, 1, 64, generator=rng).repeat_interleave(2, 0) + 0.01 * torch.randn(n, 1, 64, generator=rng)
+    v = torch.where(torch.arange(n)[:, None, None] % 2 == 0, 1000.0, -1000.0).expand(n, 1, 64)
+    fill(cache.k, table, 0, k)
+    fill(cache.v, table, 0, v)
+    got = cache.tree_attention(batch, q.cuda())
+    terms = exact(q.double().cuda(), k.to(dt).double().cuda(), v.to(dt).double().cuda(), None, 0.125)
+    off, tol = (got.double() - terms[0]).abs(), bound_of(dt, terms, 64, 3 * 32)
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+@pytest.mark.parametrize("dt,G,bound", [(F32, 2, None), (BF16, 1, None), (F16, 1, None), (BF16, 8, FAR), (F16, 8, FAR)])
+@pytest.mark.parametrize("length", [20000, 150])
+def test_shares_of_a_split_cache(gpu, dt, G, bound, length):
+    """V around 1: a share of the softmax that a split or a join lost or counted twice is a bias."""
+    rng = rng_of(52)
+    rows, lengths = [24, 3], [length, length // 3]
+    cache, batch, table = make(rng, lengths, rows, 64, 1, 128, dt, bound=bound)
+    parents = [ref.random_parents(rng, n) for n in rows]
+    seen = [ref.tree_seen(p, lengths[b] - rows[b]) for b, p in enumerate(parents)]
+    bits = [s[i, lengths[b] - rows[b]:].nonzero()[:, 0].tolist() for b, s in enumerate(seen) for i in range(rows[b])]
+    q = torch.randn(27, G, 128, generator=rng).to(dt).cuda()
+    ks = [torch.randn(n, 1, 128, generator=rng) for n in lengths]
+    vs = [1 + 0.25 * torch.randn(n, 1, 128, generator=rng) for n in lengths]
+    for b in range(2):
+        fill(cache.k, table, b, ks[b])
+        fill(cache.v, table, b, vs[b])
+    got = cache.tree_attention(batch, q, mask=ref.mask_words(bits, 1).cuda())
+    cache.check()
+    t = 0
+    for b, n in enumerate(rows):
+        terms = exact(q[t:t + n].double(), ks[b].to(dt).double().cuda(), vs[b].to(dt).double().cuda(), seen[b].cuda(), 128 ** -0.5)
+        # In a CTA: all tiles of a short cache, of a long one its share over at least 100 CTAs; then the partials.
+        steps = 7 * 32 if length == 150 else 10 * 32 + 740
+        off, tol = (got[t:t + n].double() - terms[0]).abs(), bound_of(dt, terms, 128, steps)
+        assert (off <= tol).all(), (b, float((off / tol).max()))
+        t += n
+
+
 @pytest.mark.parametrize("dt,heads,bound", [(F32, 2, None), (BF16, 2, None), (F16, 2, None), (BF16, 16, FAR), (F16, 16, FAR)])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("ctx", [0, 3000])
@@ -246,3 +292,75 @@ def test_check_tells_beams_from_pages(gpu):
         cache.check()
     assert e.value.status == _lib.PP_E_INVALID and "beam" in str(e.value) and "page" in str(e.value)
     cache.check()
+
+
+def test_shard_refuses_f16_parameters(gpu):
+    """PP_F16 is the paged operators' alone: a shard's loader knows F32 and BF16."""
+    import ctypes
+
+    import numpy as np
+
+    from potpori_b200.config import QwenConfig
+    from potpori_b200.shard import Shard
+
+    cfg = QwenConfig(layers=2, hidden=256, intermediate=512, head_dim=128, n_heads=4, n_kv_heads=2, vocab_size=64,
+                     rms_norm_eps=1e-6, rope_theta=1e6)
+    shard = Shard(cfg, (0, 2), 8, 2)
+    name = b"model.layers.0.mlp.gate_proj.weight"
+    data = np.zeros(512 * 256, np.uint16)
+    L, p = _lib.load(), data.ctypes.data_as(ctypes.c_void_p)
+    for dtype in (_lib.PP_F16, 3):
+        assert L.pp_shard_set_tensor(shard.handle, name, dtype, p, data.size) == _lib.PP_E_INVALID
+        assert "parameters are PP_F32 or PP_BF16" in _lib.last_error(shard.handle)
+    assert L.pp_shard_set_tensor(shard.handle, name, _lib.PP_BF16, p, data.size) == _lib.PP_OK
+
+
+@pytest.mark.parametrize("dt,G,bound", [(F32, 2, None), (BF16, 1, None), (BF16, 4, FAR), (F16, 2, FAR)])
+@pytest.mark.parametrize("rows,lengths", [([300], [300]), ([300, 77], [700, 1100]), ([520], [3000]), ([1], [9])])
+def test_prompt_rows(gpu, dt, G, bound, rows, lengths):
+    """A chain of many rows, with and without context, alone and beside others."""
+    rng = rng_of(56)
+    cache, batch, table = make(rng, lengths, rows, 16, 2, 64, dt, bound=bound)
+    T = sum(rows)
+    q = torch.randn(T, 2 * G, 64, generator=rng).to(dt).cuda()
+    got = cache.tree_attention(batch, q, lse=(lse := torch.empty(T, 2 * G, device="cuda")))
+    cache.check()
+    t = 0
+    for b, n in enumerate(rows):
+        k, v = (ref.cached(p, "nhd", table, b, lengths[b], 16).cuda() for p in (cache.k, cache.v))
+        seen = torch.ones(n, lengths[b], dtype=torch.bool, device="cuda").tril(lengths[b] - n)
+        terms = exact(q[t:t + n].double(), k, v, seen, 0.125)
+        steps = -(-lengths[b] // 16) * 16 + 740  # no more than every key's, however it is cut
+        off, tol = (got[t:t + n].double() - terms[0]).abs(), bound_of(dt, terms, 64, steps)
+        assert (off <= tol).all(), (b, float((off / tol).max()))
+        assert ((lse[t:t + n].double() - terms[1]).abs() <= (steps + 2 * 64 * terms[4]) * 2.0 ** -24 + 2.0 ** -20 + terms[1].abs() * 2.0 ** -22).all()
+        t += n
+
+
+@pytest.mark.parametrize("sequences", [70, 210])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_many_sequences_of_many_vectors(gpu, sequences, dim):
+    """The tcgen05 kernel with more sequences than a line is put in order for, and with more than the shared
+    memory of two CTAs on an SM has room for."""
+    rng = rng_of(57)
+    rows = [int(torch.randint(0, 6, (1,), generator=rng)) for _ in range(sequences)]
+    lengths = [n + int(torch.randint(0, 260, (1,), generator=rng)) for n in rows]
+    cache, batch, table = make(rng, lengths, rows, 16, 1, dim, BF16, bound=FAR)
+    T = sum(rows)
+    parents = [ref.random_parents(rng, n) if n else [] for n in rows]
+    seen = [ref.tree_seen(p, lengths[b] - rows[b]) for b, p in enumerate(parents)]
+    bits = [s[i, lengths[b] - rows[b]:].nonzero()[:, 0].tolist() for b, s in enumerate(seen) for i in range(rows[b])]
+    q = torch.randn(T, 12, dim, generator=rng).bfloat16().cuda()
+    mask = ref.mask_words(bits, 1).cuda()
+    got = cache.tree_attention(batch, q, mask=mask)
+    cache.check()
+    pools = cache.k.cpu().double(), cache.v.cpu().double()
+    t = 0
+    for b, n in enumerate(rows):
+        if n:
+            k, v = (ref.cached(p, "nhd", table, b, lengths[b], 16).cuda() for p in pools)
+            terms = exact(q[t:t + n].double(), k, v, seen[b].cuda(), dim ** -0.5)
+            off, tol = (got[t:t + n].double() - terms[0]).abs(), bound_of(BF16, terms, dim, 9 * 16 + 8)
+            assert (off <= tol).all(), (b, float((off / tol).max()))
+        t += n
+    assert torch.equal(cache.tree_attention(batch, q, mask=mask), got)
