@@ -419,7 +419,7 @@ typedef struct pp_tree_query {
  * F32); the context's gives every row itself or NaN. Nodes past 32 * mask_words are unseen. The result of a row does not depend on
  * atomics' order: equal calls give equal bits. `work` (16-byte aligned) holds the partial results
  * of split caches: at least pp_tree_attention_work_bytes (0: the arguments are refused). Limits:
- * n_heads <= 1024 n_kv_heads; max_rows <= 2^20; table_stride * page_size < 2^31; and
+ * n_heads <= 1024 n_kv_heads; max_rows <= 2^20; table_stride * page_size <= 2^31 - 4096; and
  * (rows * n_heads / n_kv_heads / 4 + batch) * n_kv_heads * (table_stride * page_size / 32 + 1) < 2^31. */
 uint64_t pp_tree_attention_work_bytes(const pp_paged_cache* cache, const pp_paged_batch* batch,
                                       uint32_t n_heads);

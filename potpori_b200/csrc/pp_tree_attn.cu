@@ -711,7 +711,7 @@ inline const char* tree_problem(const pp_paged_cache* c, const pp_paged_batch* b
   const uint64_t G = n_heads / c->n_kv_heads;
   const uint64_t units = ((uint64_t)b->rows * G / 4 + b->batch) * c->n_kv_heads;
   const uint64_t longest = (uint64_t)b->table_stride * c->page_size;
-  if (longest > 0x7fffffffull) return "a page table of more than 2^31 positions";
+  if (longest > kTreeMostPositions) return "a page table of more than 2^31 - 4096 positions";
   if (units * (longest / 32 + 1) > 0x7fffffffull) return "rows times positions out of range";
   return nullptr;
 }

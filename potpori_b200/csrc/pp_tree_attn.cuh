@@ -23,6 +23,8 @@ namespace pp {
 template <typename T>
 constexpr int kTreeTile = sizeof(T) == 4 ? 32 : 64;
 constexpr int kTreeMostRows = 1 << 20;  // of a sequence: times the group they stay below 2^31
+// Of a page table: places are counted in 32 bits, a few tiles past a sequence's end among them.
+constexpr uint64_t kTreeMostPositions = (1ull << 31) - 4096;
 
 struct TreeArgs {
   PagedView c;  // the layer
