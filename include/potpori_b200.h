@@ -330,8 +330,8 @@ pp_status pp_shard_read_taps(pp_shard* shard, uint32_t m, float* f32, uint16_t* 
  * neither read nor written, and a sequence whose rows lie outside the arrays, or whose kv_len is below
  * its number of rows or above table_stride * page_size, is left out whole (its output rows, q_out's
  * among them, keep what they held); value 4 when a bounded wait on the device expired (the output is
- * then undefined). No call reads a position at or
- * past kv_len, whatever the page holds there. */
+ * then undefined). What a page holds at
+ * or past kv_len has no effect. */
 
 /* A cache: `layers` layers of n_pages pages of page_size positions. Element (layer, page, row,
  * head, dim) of K is at k + layer * layer_stride + page * page_stride + row * row_stride +
@@ -351,8 +351,8 @@ typedef struct pp_paged_cache {
  * the call's row arrays, n_b of them (0 is fine), which are the last n_b of its kv_len[b] cached
  * positions; position s is row s % page_size of page page_table[b * table_stride + s / page_size].
  * cu_rows ([batch + 1], not decreasing, cu_rows[0] = 0), kv_len ([batch]) and page_table are
- * device memory. `rows` is the length of the row arrays: rows past cu_rows[batch] are padding and
- * are neither read nor written. max_rows and max_len are the host's bounds on n_b and kv_len: they
+ * device memory. `rows` is the length of the row arrays: rows past cu_rows[batch] are padding: what
+ * they hold has no effect, and their outputs are not written. max_rows and max_len are the host's bounds on n_b and kv_len: they
  * choose kernels and grids, and results depend on them by rounding alone. batch <= 4096,
  * rows <= 2^24. */
 typedef struct pp_paged_batch {
@@ -450,8 +450,11 @@ pp_status pp_tree_commit(const pp_paged_cache* cache, const pp_paged_batch* batc
  * lower token: out_scores (F32), out_beams, out_tokens, each [groups][k]. A logit of -inf is never
  * chosen; a beam with finished[g][b] != 0 (NULL: none) has one candidate, token `pad` at its score
  * unchanged; a beam whose score or any of whose logits is NaN or +inf is left out and sets bit 2
- * of *err. Where fewer than k candidates remain the rest are -inf, -1, -1. Values are formed
- * and compared in 64 bits. out_scores must not be scores. work: 16-byte aligned,
+ * of *err. Where fewer than k candidates remain the rest are -inf, -1, -1. The log of
+ * the sum is good to about 2^-21 (exponentials and the sums of up to 4096 logits are F32); from there
+ * values are formed and compared in 64 bits, so a beam's candidates keep the order of their logits and
+ * two equal rows of logits tie, while beams whose sums are equal only in exact arithmetic may go either
+ * way. out_scores must not be scores. work: 16-byte aligned,
  * pp_beam_select_work_bytes. cuda_device: the device of the pointers and the stream. */
 uint64_t pp_beam_select_work_bytes(uint32_t groups, uint32_t beams, uint32_t vocab, uint32_t k);
 pp_status pp_beam_select(const void* logits, pp_dtype dtype, int64_t row_stride,

@@ -251,8 +251,9 @@ constexpr int kCommitBatch = 8;  // rows a thread holds between its loads and it
 // few hundred cycles) and moves the path's rows in its planes. A thread keeps one 16-byte unit of
 // a row and moves it down row after row: the rows before the first gap stay, and as path[d] >= d
 // and both ascend, a row is written only after every row that it covers has been read. 64 trees,
-// 36 layers, 61 MB: 14.6 us, 4.2 TB/s; one tree of 8, 28 layers: 3.7 us, the chain from the tokens to
-// the pages.
+// 36 layers, 61 MB: 22 us over changing caches, 2.8 TB/s (17 to 19 over the same one again and again),
+// for every plane's CTA walks the tree again and nine of them fill an SM; one tree of 8, 28 layers: 3.7
+// to 4.3 us, the chain from the tokens to the pages.
 __global__ void __launch_bounds__(kCommitThreads) pp_tree_commit_kernel(const CommitArgs a) {
   __shared__ int32_t follow[kCommitMaxRows];  // the node that continues a path ending here
   __shared__ int32_t path[kCommitMaxRows];
@@ -350,8 +351,8 @@ constexpr int kReorderBatch = 4;  // units a lane holds between its loads and it
 
 // Grid (slices of the 2 * layers planes, new beams, groups). Only beams that take their spare
 // page copy: lanes over the 16-byte units of a row, warps over the rows, four loads before
-// their stores. 32 x 8 beams, 36 layers: 72 us for 225 MB of rows read and written, 6.2 TB/s; 4
-// beams, 28 layers: 3.9 us.
+// their stores. 32 x 8 beams, 36 layers: 73 to 76 us for 400 to 450 MB read and written, 5.5 to 5.9 TB/s;
+// 4 beams, 28 layers: 3.9 us.
 __global__ void __launch_bounds__(kReorderThreads) pp_beam_reorder_kernel(const ReorderArgs a) {
   const int j = blockIdx.y, g = blockIdx.z, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int32_t* mine = a.beams + (int64_t)g * a.new_beams;

@@ -15,6 +15,7 @@ namespace pp {
 // ---- 16-bit caches, few query vectors --------------------------------------------------------
 constexpr int kTreeThreads = 128;
 constexpr int kTreeBN = kTreeTile<__half>;
+// The bounds below were measured with 8 cached heads of 128 and hold for other heads and dims unmeasured.
 // Caches of up to so many tiles are never cut, which saves the join's launch, about 1 us (one decoded
 // row, 8 heads, narrow: 256 positions 8.0 us whole against 8.6, 512 11.9 against 9.4; F32: 64 positions
 // 6.8 against 7.4, 128 10.9 against 7.2; 240 vectors, tcgen05: 128 positions 10.9 against 11.9).
@@ -373,12 +374,13 @@ __global__ void __launch_bounds__(kTreeThreads, NarrowCfg<DP>::kPerSm)
 }
 
 // ---- F32 caches ----------------------------------------------------------------------------
-// CUDA cores: on these tensor cores three products of split halves would be needed to keep F32,
-// at the rate of an F32 multiply-add and with a worse sum. BM query vectors (4 for a decoded token,
+// CUDA cores: the F32 products and sums of the definition. (Three tensor-core products of split halves
+// would come near F32, and many vectors a head would gain by them: not built.) BM query vectors (4 for a decoded token,
 // 16 else), 32-key tiles, four warps. Scores: warp w the rows w BM / 4 .., lane = key, so the softmax
 // of a row stays in its warp; output: thread = dim, all rows. One row over 42 positions, 16 heads on 8:
-// 7.0 us, the chain of launch, lengths, page and rows; 48 rows over 515 to 1030: 83 us, 3.7 TB/s, the
-// multiply-adds and their shared-memory operands.
+// 7.0 us, the chain of launch, lengths, page and rows; 48 rows over 515 to 1030: 83 us, 3.7 TB/s, 64 over
+// 2048 to 4096: 366 us, 4.5 TB/s, the multiply-adds and their shared-memory operands. Trees read K and V
+// again for every 16 vectors: 16 of 61 nodes over 2048 to 4096 positions 4.5 ms, 11 TFLOP/s.
 constexpr int kTreeFBN = kTreeTile<float>, kTreeFStages = 2;
 template <int DP, int BM>
 struct TreeFCfg {

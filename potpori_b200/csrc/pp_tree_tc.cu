@@ -8,7 +8,7 @@
 //  * warps 4 and 5, producers: the K and V tiles by TMA, in boxes of 8 to 64 rows of one page and 64
 //    dims, into a ring of tile-sized slots, in the order in which the products need them (K0, K1, V0,
 //    K2, V1, ...). A box costs some 54 clocks whatever its size (the trees below: pages of 64
-//    positions 89 us, 32 92, 16 119, 24, in boxes of 8, 165; 24 row by row 265).
+//    positions 92 to 98 us, 32 92, 16 122, 24, in boxes of 8, 165; 7, row by row, 279).
 //    A slot holds 64-dim blocks of 64 rows x 128 bytes, the 16-byte unit u of row r at u ^ (r & 7):
 //    read K-major it is the B operand of Q K^T, read MN-major the B operand of P V. Where pages are
 //    not multiples of 8 positions, warps 4 and 5 fetch row by row with 16-byte asynchronous copies.
@@ -29,8 +29,9 @@
 // whose products share the tensor core, about half busy, with the other CTA's. Left out one by one, on
 // trial, neither half of the products nor the exponentials nor memory gave more than 5 %; two softmax
 // warps a row were slower. 16 ragged trees of 61 nodes over 2048 to 4096 positions, 8 heads of 128, F16:
-// 91 us, 550 TFLOP/s; one tree of 24 over 131072, BF16: 109 us, 4.9 TB/s, of which the tiles run at
-// 6.5 TB/s.
+// 92 us replayed on a cool card, 545 TFLOP/s, 109 to 114 call after call at the power cap; one tree of
+// 24 over 131072, BF16: 107 to 113 us, 4.8 TB/s, of which the tiles run at 6.5 TB/s, and 127 to 137.
+// With heads of 256 the trees of 61 take 216 us (464 TFLOP/s), of 64 85.
 // Every wait is bounded; one that expires sets bit 4 of the caller's error word, and the CTA still
 // lets its copies and products land and frees its TMEM before it leaves.
 #include <cuda_runtime.h>
@@ -57,7 +58,8 @@ struct TcCfg {
   static constexpr int kCols = DP == 256 ? 512 : 256;  // TMEM: O [DP], twice S or P [64]
   static constexpr int kBars = 192;
   // Two CTAs share 228 KB less 1 KB each: at head_dim 128 that leaves 1 KB beside Q, four slots and
-  // the turn buffer, for the barriers and the prefix of up to 196 sequences. (More slots than four
+  // the turn buffer, for the barriers and the prefix of up to 196 sequences; above, an SM
+  // holds one CTA (trees of 24 over 300 to 600: 190 sequences 128 us, 210 197). (More slots than four
   // only lengthen every other load's way through memory: at the card's rate 148 x 2 x 64 KB in flight
   // are 3 us already.)
   static size_t smem(int batch) { return kQ + kTurn + kSlots * (size_t)kItem + kBars + prefix_bytes(batch); }
