@@ -57,7 +57,12 @@ def binding_abi() -> "str | None":
     """The torch and Python that a binding is built for; None without torch."""
     if importlib.util.find_spec("torch") is None:
         return None
-    return f"torch {importlib.metadata.version('torch')} {sysconfig.get_config_var('SOABI')}"
+    try:
+        version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:  # a source tree on the path
+        import torch
+        version = torch.__version__
+    return f"torch {version} {sysconfig.get_config_var('SOABI')}"
 
 
 def binding_stale(abi: str) -> bool:

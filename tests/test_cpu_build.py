@@ -38,3 +38,15 @@ def test_binding_is_rebuilt_for_another_torch(monkeypatch, tmp_path):
     (tmp_path / "built").write_text(abi.replace("torch ", "torch 1."))
     b.build()
     assert built == [abi, abi]
+
+
+def test_torch_without_package_metadata(monkeypatch):
+    import importlib.metadata
+
+    import torch
+
+    def absent(name):
+        raise importlib.metadata.PackageNotFoundError(name)
+
+    monkeypatch.setattr(importlib.metadata, "version", absent)
+    assert b.binding_abi().startswith(f"torch {torch.__version__} ")
